@@ -13,6 +13,8 @@ F32, BF16 = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SIGMOID = 0, 1, 2, 3
 MAX_RANKS = 64
 GEMM_MAX_LIST = 16
+RELBIAS_MAX_SIDE, RELBIAS_MAX_REACH = 64, 1024
+RELBIAS_MAX_DISTANCE = 1 << 20
 
 
 class HapmiError(RuntimeError):
@@ -51,6 +53,11 @@ class GemmArgs(ctypes.Structure):
         ("a_relu", ctypes.c_int), ("b_relu", ctypes.c_int),
         ("drop_state", ctypes.c_void_p), ("drop_stream_id", ctypes.c_int64), ("drop_p", ctypes.c_float),
     ]
+
+
+class RelBias(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("ld", ctypes.c_int64), ("n_buckets", ctypes.c_int),
+                ("bidirectional", ctypes.c_int), ("starts_host", ctypes.c_void_p)]
 
 
 _HEADER = os.path.join(_HERE, "..", "include", "hapmi.h")

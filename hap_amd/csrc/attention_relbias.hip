@@ -1,0 +1,619 @@
+// Fused scaled-dot-product attention with a learned relative position bias, bf16, head_dim 64, on the packed projection
+// qkv[b, S, 3*H*64], forward and backward.
+//
+//   s_ij = scale * <q_i, k_j> + T[bucket(j - i), h],   p = softmax_j(s),   o_i = sum_j p_ij v_j,   lse_i = log sum_j exp s_ij
+//   ds_ij = p_ij (<do_i, v_j> - delta_i),  delta_i = <do_i, o_i>
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+//   dT[u, h] = sum over the batch and all visible pairs with bucket(j - i) = u of ds_ij
+//
+// bucket() depends on the relative position only and is constant from distance R = the last bucket's first distance on, so
+// a head's bias is a vector over the window [-R, R], which every block expands into LDS once.  The vector is kept divided
+// by `scale` and handed to the QK matrix instructions as their initial accumulator: the bias costs LDS reads and no vector
+// arithmetic.  The score layout is that of the kernels without a bias (each lane owns one query column in forward and dQ,
+// one key column in dK / dV; consecutive registers are consecutive keys / queries, so a lane's window reads are runs of
+// four consecutive words and the 32 columns of a half wave read 32 consecutive addresses).
+//
+// dT: ds_ij is summed along the diagonals j - i of a 32 x 32 score block by LDS float additions into a window-long array of
+// the wave AND lane half: within one instruction a half wave's 32 columns go to 32 different words, a wave's LDS operations
+// complete in order and nobody else adds to that array, so the result is the same bits every time.  The eight arrays are
+// added in order at the block's end, the blocks' windows and the buckets' ranges by a second kernel, in order.
+#include "common.h"
+#include "attention_tile.h"
+
+namespace {
+
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int REL_MAX_SIDE = HAPMI_RELBIAS_MAX_SIDE;
+constexpr int REL_MAX_REACH = HAPMI_RELBIAS_MAX_REACH;
+// A 64 x 32 block of scores spans 95 diagonals: the window carries this many saturated entries on either side, and the
+// offset of a block that lies wholly beyond the window is clamped so that it reads nothing else.
+constexpr int MARGIN = 95;
+constexpr float HIDDEN = -1e30f;              // a bias at or below this hides the pair (the type's lowest value included)
+
+struct RelArgs {
+    const float *table;                       // [buckets, ld], column = head
+    int64_t ld;
+    int side, bidir, R;                       // buckets per side; R: first distance of the last bucket, >= 1
+    int starts[REL_MAX_SIDE];                 // first distance of every bucket of a side, starts[0] = 0
+    __device__ __forceinline__ int window() const { return 2 * R + 1 + 2 * MARGIN; }
+    __device__ __forceinline__ int bucket(int rel) const {
+        const int d = bidir ? (rel < 0 ? -rel : rel) : (rel < 0 ? -rel : 0);
+        int k = 0;
+        for (int i = 1; i < side; ++i) k += d >= starts[i] ? 1 : 0;
+        return k + (bidir && rel > 0 ? side : 0);
+    }
+    // the head's bias / scale over the window; REV: entry i belongs to relative position -(i - R - MARGIN)
+    template <bool REV> __device__ __forceinline__ void expand(float *win, int head, float scale) const {
+        for (int i = threadIdx.x; i < window(); i += AT_THREADS) {
+            int rel = i - R - MARGIN;
+            rel = rel < -R ? -R : (rel > R ? R : rel);
+            const float t = table[(int64_t)bucket(REV ? -rel : rel) * ld + head];
+            win[i] = t <= HIDDEN ? -INFINITY : t / scale;
+        }
+    }
+    // word of the window that the lane's row 0 of a block of ROWS x 32 scores reads; D = first row - first column
+    template <int ROWS> __device__ __forceinline__ int at(int D, int c, int h) const {
+        D = D < -R - (ROWS - 1) ? -R - (ROWS - 1) : (D > R + 31 ? R + 31 : D);
+        return D + R + MARGIN + 4 * h - c;
+    }
+};
+
+// initial accumulator of a 32 x 32 score block: rows of the block are runs of four words
+__device__ __forceinline__ f32x16 bias_tile(const float *w) {
+    f32x16 a;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[g * 4 + e] = w[g * 8 + e];
+    return a;
+}
+
+__device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) {
+    if (!lengths) return S;
+    const int n = lengths[b];
+    return n < 0 ? 0 : (n > S ? S : n);
+}
+
+// ---------------------------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------------------------
+template <bool CAUSAL, bool DROP>
+__global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArgs rel, const bf16_t *qkv, bf16_t *out, float *lse,
+                                                               const int32_t *lengths, int S, int H, float scale,
+                                                               const uint32_t *keep_rows, float keep_scale) {
+    constexpr int NST = 3;                                    // one tile is multiplied while two are on their way
+    __shared__ __attribute__((aligned(16))) char Ks3[NST][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char Vs3[NST][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) uint32_t keep_s[DROP ? NST : 1][AT_THREADS];
+    extern __shared__ float win[];
+    const TransposedReader tr;
+    const int E = H * HD, ld = 3 * E;
+    const int blk = BlockOrder<CAUSAL>::row_block(true), bh = BlockOrder<CAUSAL>::batch_head();
+    const int b = bh / H, hh = bh % H;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int n = row_length(lengths, b, S);
+    const int qw = blk * 128 + wave * 32, q = qw + c;
+    const bf16_t *Q = qkv + (int64_t)b * S * ld + hh * HD;
+    const bf16_t *K = Q + E, *V = Q + 2 * E;
+
+    const int q_blk_end = blk * 128 + 128;
+    const int kv_end = blk * 128 >= n ? 0 : ((CAUSAL && q_blk_end < n) ? q_blk_end : n);
+    f32x16 ot[2] = {zero16(), zero16()};
+    float m = -INFINITY, lsum = 0.f;                          // running maximum in units of log 2
+    if (kv_end > 0) {
+        frag_t qf[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) qf[s] = load_row_frag(Q + (int64_t)q * ld, q < n, s, h);
+        rel.expand<false>(win, hh, scale);                    // published by the first barrier of the loop
+        const DirectTileLoader ldr(ld);
+        const float sl2 = scale * LOG2E;
+        constexpr int PER_TILE = 2 * DirectTileLoader::LOADS + (DROP ? 1 : 0);
+        static_assert(2 * DirectTileLoader::LOADS == 4, "the waits below are written for four (five) transfers per tile");
+        const int n_kt = (S + TILE - 1) / TILE;
+        const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * n_kt * 2 + h : nullptr;
+        auto issue_tile = [&](int kv0, int bufi) {
+            ldr.issue(K + (int64_t)kv0 * ld, n - kv0, Ks3[bufi]);
+            ldr.issue(V + (int64_t)kv0 * ld, n - kv0, Vs3[bufi]);
+            if constexpr (DROP) issue_word(keep_row + (kv0 / TILE) * 2, &keep_s[bufi][0]);
+        };
+        issue_tile(0, 0);
+        if (TILE < kv_end) issue_tile(TILE, 1);
+        // consumed before the loop, so that the wait for these loads is not one for all transfers in every iteration
+#pragma unroll
+        for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(qf[s].v));
+        int buf = 0;
+        for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
+            if (kv0 + TILE < kv_end) __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | PER_TILE);   // vmcnt: only the next tile may be outstanding
+            else __builtin_amdgcn_s_waitcnt(0x0F70);                                           // vmcnt(0)
+            __syncthreads();
+            if (kv0 + 2 * TILE < kv_end) issue_tile(kv0 + 2 * TILE, buf == 0 ? 2 : buf - 1);
+            const char *Ks = Ks3[buf], *Vs = Vs3[buf];
+            uint32_t keep = 0xffffffffu;
+            if constexpr (DROP) keep = keep_s[buf][threadIdx.x];
+            const float *w = win + rel.at<64>(kv0 - qw, c, h);
+            f32x16 st[2] = {bias_tile(w), bias_tile(w + 32)};
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) st[t] = mma(frag_rowk(Ks, t * 32 + c, s, h), qf[s], st[t]);
+            if (kv0 + TILE > n || (CAUSAL && kv0 + TILE - 1 > qw)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int kv = kv0 + t * 32 + acc_row(r, h);
+                        if (kv >= n || (CAUSAL && kv > q)) st[t][r] = -INFINITY;
+                    }
+            }
+            float mx = st[0][0];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[t][r]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float m_new = fmaxf(m, mx * sl2);
+            const float msub = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = __builtin_amdgcn_exp2f(m - msub);
+            float psum = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(st[t][r], sl2, -msub));
+                    st[t][r] = p;
+                    psum += p;
+                }
+            m = m_new;
+            lsum = lsum * alpha + psum;
+            if constexpr (DROP) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) st[t][r] = (keep & (1u << (t * 16 + r))) ? st[t][r] : 0.f;
+            }
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ot[u][r] *= alpha;
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const frag_t pb = acc_to_b(st[s >> 1], s & 1);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) ot[u] = mma(tr.frag(Vs, u * 32, s), pb, ot[u]);
+            }
+            buf = buf == NST - 1 ? 0 : buf + 1;
+        }
+    }
+    const float l = lsum + __shfl_xor(lsum, 32, 64);
+    const bool seen = q < n && l > 0.f;                       // a padded query, or one that sees nothing: zeros, lse = -inf
+    const float inv = seen ? (DROP ? keep_scale : 1.f) / l : 0.f;
+    if (q < S) {
+        bf16_t *orow = out + ((int64_t)b * S + q) * E + hh * HD;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                bf16x4 o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (bf16_t)(l != l ? l : (seen ? ot[u][g * 4 + e] * inv : 0.f));
+                *(bf16x4 *)(orow + u * 32 + g * 8 + h * 4) = o;
+            }
+        if (h == 0) lse[((int64_t)b * H + hh) * S + q] = q < n ? m * LN2 + logf(l) : -INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// dQ and the bias gradient: lanes own query columns, kv tiles are streamed
+// ---------------------------------------------------------------------------------------------
+template <bool CAUSAL, bool DROP>
+__global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *out,
+                                                                  const bf16_t *dout, const float *lse, float *delta,
+                                                                  bf16_t *dqkv, float *part, const int32_t *lengths, int S,
+                                                                  int H, float scale, const uint32_t *keep_rows,
+                                                                  float keep_scale) {
+    __shared__ __attribute__((aligned(16))) char Ks[TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char Vs[TILE_BYTES];
+    extern __shared__ float win[];                            // the bias window, then the eight windows of ds sums
+    const TransposedReader tr;
+    const int W = rel.window();
+    const int E = H * HD, ld = 3 * E;
+    const int blk = BlockOrder<CAUSAL>::row_block(true), bh = BlockOrder<CAUSAL>::batch_head();
+    const int b = bh / H, hh = bh % H;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int n = row_length(lengths, b, S);
+    const int qw = blk * 128 + wave * 32, q = qw + c;
+    const bool qok = q < n;
+    const bf16_t *Q = qkv + (int64_t)b * S * ld + hh * HD;
+    const bf16_t *K = Q + E, *V = Q + 2 * E;
+    const bf16_t *dO = dout + (int64_t)b * S * E + hh * HD;
+    const int q_blk_end = blk * 128 + 128;
+    const int kv_end = blk * 128 >= n ? 0 : ((CAUSAL && q_blk_end < n) ? q_blk_end : n);
+    float *sums = win + W, *own = sums + (wave * 2 + h) * W;
+    for (int i = threadIdx.x; i < 8 * W; i += AT_THREADS) sums[i] = 0.f;
+    f32x16 dqt[2] = {zero16(), zero16()};
+    if (kv_end > 0) {
+        rel.expand<false>(win, hh, scale);                    // both published by the loop's first barrier
+        frag_t qf[4], dof[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            qf[s] = load_row_frag(Q + (int64_t)q * ld, qok, s, h);
+            dof[s] = load_row_frag(dO + (int64_t)q * E, qok, s, h);
+        }
+        const float lse_q = qok ? lse[((int64_t)b * H + hh) * S + q] : -INFINITY;
+        float delta_q = 0.f;
+        {
+            const bf16_t *O = out + (int64_t)b * S * E + hh * HD;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const frag_t of = load_row_frag(O + (int64_t)q * E, qok, s, h);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta_q += (float)of.v[e] * (float)dof[s].v[e];
+            }
+            delta_q += __shfl_xor(delta_q, 32, 64);
+            if (qok && h == 0) delta[((int64_t)b * H + hh) * S + q] = delta_q;
+        }
+        PairLoader lk(ld), lv(ld);
+        // ds is kept without its factor `scale`; a query that sees nothing (lse = -inf) has p = 0
+        const float sl2 = scale * LOG2E, nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
+        lk.load(K, n);
+        lv.load(V, n);
+        const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * ((S + TILE - 1) / TILE) * 2 + h : nullptr;
+        uint32_t keep = 0xffffffffu, keep_next = 0xffffffffu;
+        if constexpr (DROP) keep_next = keep_row[0];
+        for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
+            __syncthreads();
+            lk.store_rows(Ks);
+            lv.store_rows(Vs);
+            if constexpr (DROP) keep = keep_next;
+            __syncthreads();
+            if (kv0 + TILE < kv_end) {
+                const int nx = kv0 + TILE;
+                lk.load(K + (int64_t)nx * ld, n - nx);
+                lv.load(V + (int64_t)nx * ld, n - nx);
+                if constexpr (DROP) keep_next = keep_row[(nx / TILE) * 2];
+            }
+            if (qw >= n) continue;                            // a wave without queries only moves tiles and meets barriers
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (t == 1 && kv0 + 32 >= n) break;
+                const int at = rel.at<32>(kv0 + t * 32 - qw, c, h);
+                f32x16 st = bias_tile(win + at), dp = zero16();
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    st = mma(frag_rowk(Ks, t * 32 + c, s, h), qf[s], st);
+                    dp = mma(frag_rowk(Vs, t * 32 + c, s, h), dof[s], dp);
+                }
+                if constexpr (DROP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f;
+                }
+                if (kv0 + t * 32 + 32 > n || (CAUSAL && kv0 + t * 32 + 31 > qw)) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int kv = kv0 + t * 32 + acc_row(r, h);
+                        if (kv >= n || (CAUSAL && kv > q)) st[r] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl)) * (dp[r] - delta_q);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    __hip_atomic_fetch_add(own + at - 4 * h + acc_row(r, h), dp[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+#pragma unroll
+                for (int sp = 0; sp < 2; ++sp) {
+                    const frag_t db = acc_to_b(dp, sp);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) dqt[u] = mma(tr.frag(Ks, u * 32, t * 2 + sp), db, dqt[u]);
+                }
+            }
+        }
+    }
+    if (q < S) {
+        bf16_t *drow = dqkv + ((int64_t)b * S + q) * ld + hh * HD;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                bf16x4 o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (bf16_t)(qok ? dqt[u][g * 4 + e] * scale : 0.f);
+                *(bf16x4 *)(drow + u * 32 + g * 8 + h * 4) = o;
+            }
+    }
+    __syncthreads();
+    float *mine = part + ((int64_t)bh * ((S + 127) / 128) + blk) * W;
+    for (int i = threadIdx.x; i < W; i += AT_THREADS) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += sums[k * W + i];
+        mine[i] = v;
+    }
+}
+
+// dT[u, h] (+)= the blocks' windows [b * H][row blocks][W], added over b and row block in order, then over the relative
+// positions of bucket u in order.  One block per head: the windows are short next to the scores they come from.
+__global__ __launch_bounds__(1024) void relbias_dtable_kernel(const RelArgs rel, const float *part, float *dtable, int64_t ldd,
+                                                            int n_buckets, int b, int H, int row_blocks, int accumulate) {
+    extern __shared__ float tot[];
+    const int W = rel.window(), h = blockIdx.x;
+    for (int i = threadIdx.x; i < W; i += 1024) {
+        float v = 0.f;
+        for (int z = 0; z < b; ++z) {
+            const float *p = part + ((int64_t)z * H + h) * row_blocks * W + i;
+            for (int k = 0; k < row_blocks; ++k) v += p[(int64_t)k * W];
+        }
+        tot[i] = v;
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < n_buckets; u += 1024) {
+        float v = 0.f;
+        for (int i = 0; i < W; ++i) {
+            int r = i - rel.R - MARGIN;
+            r = r < -rel.R ? -rel.R : (r > rel.R ? rel.R : r);
+            if (rel.bucket(r) == u) v += tot[i];
+        }
+        float *d = dtable + (int64_t)u * ldd + h;
+        *d = accumulate ? *d + v : v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// dK, dV: lanes own kv columns, query tiles are streamed
+// ---------------------------------------------------------------------------------------------
+template <bool CAUSAL, bool DROP>
+__global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *dout,
+                                                                   const float *lse, const float *delta, bf16_t *dqkv,
+                                                                   const int32_t *lengths, int S, int H, float scale,
+                                                                   const uint32_t *keep_cols, float keep_scale) {
+    __shared__ __attribute__((aligned(16))) char Qs[TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char dOs[TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) float lse_s[TILE], delta_s[TILE];
+    extern __shared__ float win[];
+    const TransposedReader tr;
+    const int E = H * HD, ld = 3 * E;
+    const int blk = BlockOrder<CAUSAL>::row_block(false), bh = BlockOrder<CAUSAL>::batch_head();
+    const int b = bh / H, hh = bh % H;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int n = row_length(lengths, b, S);
+    const int kvw = blk * 128 + wave * 32, kv = kvw + c;
+    const bool kok = kv < n;
+    const bf16_t *Q = qkv + (int64_t)b * S * ld + hh * HD;
+    const bf16_t *K = Q + E, *V = Q + 2 * E;
+    const bf16_t *dO = dout + (int64_t)b * S * E + hh * HD;
+    const float *lse_b = lse + ((int64_t)b * H + hh) * S, *delta_b = delta + ((int64_t)b * H + hh) * S;
+    f32x16 dvt[2] = {zero16(), zero16()}, dkt[2] = {zero16(), zero16()};
+    if (blk * 128 < n) {
+        rel.expand<true>(win, hh, scale);
+        frag_t kf[4], vf[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            kf[s] = load_row_frag(K + (int64_t)kv * ld, kok, s, h);
+            vf[s] = load_row_frag(V + (int64_t)kv * ld, kok, s, h);
+        }
+        PairLoader lq(ld), ldo(E);
+        const float sl2 = scale * LOG2E;
+        const int q_begin = CAUSAL ? blk * 128 : 0;           // causal: earlier queries see none of the block's keys
+        lq.load(Q + (int64_t)q_begin * ld, n - q_begin);
+        ldo.load(dO + (int64_t)q_begin * E, n - q_begin);
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 *keep_col = DROP ? (const u32x2 *)(keep_cols + ((int64_t)bh * S + (kv < S ? kv : S - 1)) * (2 * ((S + TILE - 1) / TILE))) : nullptr;
+        u32x2 keep2 = {0xffffffffu, 0xffffffffu}, keep2_next = keep2;
+        if constexpr (DROP) keep2_next = keep_col[q_begin / TILE];
+        for (int q0 = q_begin; q0 < n; q0 += TILE) {
+            __syncthreads();
+            lq.store_rows(Qs);
+            ldo.store_rows(dOs);
+            if constexpr (DROP) keep2 = keep2_next;
+            if (threadIdx.x < TILE) {
+                const int qq = q0 + threadIdx.x;
+                const float l = qq < n ? lse_b[qq] : -INFINITY;
+                lse_s[threadIdx.x] = l == -INFINITY ? INFINITY : l * LOG2E;        // a query that sees nothing: p = 0
+                delta_s[threadIdx.x] = qq < n ? delta_b[qq] : 0.f;
+            }
+            __syncthreads();
+            if (q0 + TILE < n) {
+                const int nx = q0 + TILE;
+                lq.load(Q + (int64_t)nx * ld, n - nx);
+                ldo.load(dO + (int64_t)nx * E, n - nx);
+                if constexpr (DROP) keep2_next = keep_col[nx / TILE];
+            }
+            if (kvw >= n) continue;                           // a wave without keys only moves tiles and meets barriers
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                if (t == 1 && q0 + 32 >= n) break;
+                f32x16 sc = bias_tile(win + rel.at<32>(q0 + t * 32 - kvw, c, h)), dp = zero16();
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    sc = mma(frag_rowk(Qs, t * 32 + c, s, h), kf[s], sc);
+                    dp = mma(frag_rowk(dOs, t * 32 + c, s, h), vf[s], dp);
+                }
+                const uint32_t keep = t ? keep2.y : keep2.x;
+                if constexpr (DROP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << acc_row(r, h))) ? dp[r] * keep_scale : 0.f;
+                }
+                if (CAUSAL && kvw + 31 > q0 + t * 32) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (kv > q0 + t * 32 + acc_row(r, h)) sc[r] = -INFINITY;
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int ql = t * 32 + g * 8 + h * 4;
+                    const f32x4 l4 = *(const f32x4 *)(lse_s + ql), d4 = *(const f32x4 *)(delta_s + ql);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = g * 4 + e;
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, -l4[e]));
+                        sc[r] = p;
+                        dp[r] = p * (dp[r] - d4[e]);
+                    }
+                }
+                if constexpr (DROP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[r] = (keep & (1u << acc_row(r, h))) ? sc[r] * keep_scale : 0.f;
+                }
+#pragma unroll
+                for (int sp = 0; sp < 2; ++sp) {
+                    const frag_t pb = acc_to_b(sc, sp), db = acc_to_b(dp, sp);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        dvt[u] = mma(tr.frag(dOs, u * 32, t * 2 + sp), pb, dvt[u]);
+                        dkt[u] = mma(tr.frag(Qs, u * 32, t * 2 + sp), db, dkt[u]);
+                    }
+                }
+            }
+        }
+    }
+    if (kv < S) {
+        bf16_t *drow = dqkv + ((int64_t)b * S + kv) * ld + hh * HD;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                bf16x4 ok_, ov;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ok_[e] = (bf16_t)(kok ? dkt[u][g * 4 + e] * scale : 0.f);
+                    ov[e] = (bf16_t)(kok ? dvt[u][g * 4 + e] : 0.f);
+                }
+                *(bf16x4 *)(drow + E + u * 32 + g * 8 + h * 4) = ok_;
+                *(bf16x4 *)(drow + 2 * E + u * 32 + g * 8 + h * 4) = ov;
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+int window_of(int R) { return 2 * R + 1 + 2 * MARGIN; }
+
+int check_rel(const char *name, const hapmi_relbias *r, int64_t H, RelArgs *a) {
+    HAPMI_REQUIRE(r && r->starts_host, HAPMI_EINVAL, "%s: null bias description", name);
+    const int sides = r->bidirectional ? 2 : 1;
+    HAPMI_REQUIRE(r->n_buckets >= 2 && r->n_buckets % sides == 0, HAPMI_EINVAL, "%s: %d buckets: at least 2, and even for two sides", name,
+                  r->n_buckets);
+    a->side = r->n_buckets / sides;
+    HAPMI_REQUIRE(a->side <= REL_MAX_SIDE, HAPMI_ELIMIT, "%s: %d buckets on a side, at most %d", name, a->side, REL_MAX_SIDE);
+    HAPMI_REQUIRE(r->starts_host[0] == 0, HAPMI_EINVAL, "%s: the first bucket must start at distance 0", name);
+    for (int i = 0; i < a->side; ++i) {
+        a->starts[i] = r->starts_host[i];
+        HAPMI_REQUIRE(i == 0 || a->starts[i] >= a->starts[i - 1], HAPMI_EINVAL, "%s: the buckets' first distances must not fall", name);
+    }
+    const int last = a->starts[a->side - 1];
+    HAPMI_REQUIRE(last <= REL_MAX_REACH, HAPMI_ELIMIT, "%s: the last bucket starts at distance %d, at most %d", name, last, REL_MAX_REACH);
+    a->bidir = r->bidirectional ? 1 : 0;
+    a->R = last < 1 ? 1 : last;
+    a->table = r->table;
+    a->ld = r->ld;
+    HAPMI_REQUIRE(r->ld >= H, HAPMI_EINVAL, "%s: table rows of %lld for %lld heads", name, (long long)r->ld, (long long)H);
+    return HAPMI_OK;
+}
+
+int check_shape(const char *name, int64_t b, int64_t S, int64_t H, float scale, float p) {
+    HAPMI_REQUIRE(b >= 0 && S >= 1 && H >= 1, HAPMI_EINVAL, "%s: bad shape", name);
+    HAPMI_REQUIRE(S < (1ll << 24) && H <= 4096 && b <= 65535 / H, HAPMI_ELIMIT, "%s: b * H above 65535, H above 4096 or S too long", name);
+    HAPMI_REQUIRE(scale > 0.f && scale < INFINITY, HAPMI_EINVAL, "%s: scale = %g must be positive", name, (double)scale);
+    HAPMI_REQUIRE(p >= 0.f && p < 1.f, HAPMI_EINVAL, "%s: p = %g must lie in [0, 1)", name, (double)p);
+    return HAPMI_OK;
+}
+
+bool aligned(const void *p, uintptr_t n) { return (uintptr_t)p % n == 0; }
+
+// more than 64 KiB of LDS a block has to be asked for once per kernel and device; asking again is harmless
+template <typename F> int allow_lds(const char *name, F kernel, size_t bytes) {
+    const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    HAPMI_REQUIRE(e == hipSuccess, HAPMI_ELAUNCH, "%s: %s", name, hipGetErrorString(e));
+    return HAPMI_OK;
+}
+
+}  // namespace
+
+extern "C" int hapmi_attention_relbias_fwd(const void *qkv, const hapmi_relbias *bias_host, int causal, const int32_t *lengths, void *out,
+                                           float *lse, int64_t b, int64_t S, int64_t H, float scale, const uint32_t *keep_rows,
+                                           float p, hapmi_stream_t stream) {
+    const char *name = "attention_relbias_fwd";
+    RelArgs a;
+    int rc = check_shape(name, b, S, H, scale, p);
+    if (!rc) rc = check_rel(name, bias_host, H, &a);
+    if (rc) return rc;
+    if (b == 0) return HAPMI_OK;
+    HAPMI_REQUIRE(qkv && out && lse && a.table, HAPMI_EINVAL, "%s: null pointer", name);
+    HAPMI_REQUIRE(aligned(qkv, 16) && aligned(out, 16) && aligned(keep_rows, 8) && aligned(lse, 4) && aligned(a.table, 4) && aligned(lengths, 4),
+                  HAPMI_EALIGN, "%s: qkv and out must be 16-byte aligned (keep words: 8)", name);
+    const float ks = keep_rows ? 1.0f / (1.0f - p) : 1.0f;
+    const size_t lds = (size_t)window_of(a.R) * 4;
+    dim3 grid((unsigned)hapmi_cdiv(S, 128), (unsigned)(b * H)), block(AT_THREADS);
+    auto go = [&](auto kernel) -> int {
+        hipLaunchKernelGGL(kernel, grid, block, lds, (hipStream_t)stream, a, (const bf16_t *)qkv, (bf16_t *)out, lse, lengths, (int)S,
+                           (int)H, scale, keep_rows, ks);
+        HAPMI_CHECK_LAUNCH(name);
+        return HAPMI_OK;
+    };
+    if (causal) return keep_rows ? go(relbias_fwd_kernel<true, true>) : go(relbias_fwd_kernel<true, false>);
+    return keep_rows ? go(relbias_fwd_kernel<false, true>) : go(relbias_fwd_kernel<false, false>);
+}
+
+extern "C" int hapmi_attention_relbias_workspace_elems(const hapmi_relbias *bias_host, int64_t b, int64_t S, int64_t H, int64_t *elems_host) {
+    const char *name = "attention_relbias_workspace_elems";
+    RelArgs a;
+    int rc = check_shape(name, b, S, H, 1.f, 0.f);
+    if (!rc) rc = check_rel(name, bias_host, H, &a);
+    if (rc) return rc;
+    HAPMI_REQUIRE(elems_host, HAPMI_EINVAL, "%s: null pointer", name);
+    *elems_host = b * H * hapmi_cdiv(S, 128) * window_of(a.R);
+    return HAPMI_OK;
+}
+
+extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias *bias_host, int causal, const int32_t *lengths,
+                                           const void *out, const void *dout, const float *lse, void *dqkv, float *dtable,
+                                           int64_t ld_dtable, int accumulate, float *delta_ws, float *workspace,
+                                           int64_t workspace_elems, int64_t b, int64_t S, int64_t H, float scale,
+                                           const uint32_t *keep_rows, const uint32_t *keep_cols, float p, hapmi_stream_t stream) {
+    const char *name = "attention_relbias_bwd";
+    RelArgs a;
+    int rc = check_shape(name, b, S, H, scale, p);
+    if (!rc) rc = check_rel(name, bias_host, H, &a);
+    if (rc) return rc;
+    HAPMI_REQUIRE(b >= 1, HAPMI_EINVAL, "%s: empty batch (the table's gradient would stay unwritten)", name);
+    HAPMI_REQUIRE(qkv && out && dout && lse && dqkv && dtable && delta_ws && workspace && a.table, HAPMI_EINVAL, "%s: null pointer", name);
+    HAPMI_REQUIRE(aligned(qkv, 16) && aligned(out, 16) && aligned(dout, 16) && aligned(dqkv, 16) && aligned(keep_rows, 8) && aligned(keep_cols, 8) &&
+                      aligned(lse, 4) && aligned(a.table, 4) && aligned(dtable, 4) && aligned(delta_ws, 4) && aligned(workspace, 4) &&
+                      aligned(lengths, 4),
+                  HAPMI_EALIGN, "%s: bf16 tensors must be 16-byte aligned (keep words: 8)", name);
+    HAPMI_REQUIRE((keep_rows != nullptr) == (keep_cols != nullptr), HAPMI_EINVAL, "%s: keep_rows and keep_cols come together", name);
+    HAPMI_REQUIRE(ld_dtable >= H, HAPMI_EINVAL, "%s: gradient rows of %lld for %lld heads", name, (long long)ld_dtable, (long long)H);
+    const int W = window_of(a.R);
+    const int64_t row_blocks = hapmi_cdiv(S, 128);
+    HAPMI_REQUIRE(workspace_elems >= b * H * row_blocks * W, HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name,
+                  (long long)workspace_elems, (long long)(b * H * row_blocks * W));
+    const bool drop = keep_rows != nullptr;
+    const float ks = drop ? 1.0f / (1.0f - p) : 1.0f;
+    hipStream_t st = (hipStream_t)stream;
+    dim3 grid((unsigned)row_blocks, (unsigned)(b * H)), block(AT_THREADS);
+    auto dq = [&](auto kernel) -> int {
+        const size_t lds = (size_t)W * 4 * 9;
+        rc = allow_lds(name, kernel, lds);
+        if (rc) return rc;
+        hipLaunchKernelGGL(kernel, grid, block, lds, st, a, (const bf16_t *)qkv, (const bf16_t *)out, (const bf16_t *)dout, lse, delta_ws,
+                           (bf16_t *)dqkv, workspace, lengths, (int)S, (int)H, scale, keep_rows, ks);
+        HAPMI_CHECK_LAUNCH(name);
+        return HAPMI_OK;
+    };
+    auto dkv = [&](auto kernel) -> int {
+        hipLaunchKernelGGL(kernel, grid, block, (size_t)W * 4, st, a, (const bf16_t *)qkv, (const bf16_t *)dout, lse, (const float *)delta_ws,
+                           (bf16_t *)dqkv, lengths, (int)S, (int)H, scale, keep_cols, ks);
+        HAPMI_CHECK_LAUNCH(name);
+        return HAPMI_OK;
+    };
+    if (causal) rc = drop ? dq(relbias_bwd_dq_kernel<true, true>) : dq(relbias_bwd_dq_kernel<true, false>);
+    else rc = drop ? dq(relbias_bwd_dq_kernel<false, true>) : dq(relbias_bwd_dq_kernel<false, false>);
+    if (rc) return rc;
+    hipLaunchKernelGGL(relbias_dtable_kernel, dim3((unsigned)H), dim3(1024), (size_t)W * 4, st, a, (const float *)workspace, dtable, ld_dtable,
+                       bias_host->n_buckets, (int)b, (int)H, (int)row_blocks, accumulate);
+    HAPMI_CHECK_LAUNCH(name);
+    if (causal) return drop ? dkv(relbias_bwd_dkv_kernel<true, true>) : dkv(relbias_bwd_dkv_kernel<true, false>);
+    return drop ? dkv(relbias_bwd_dkv_kernel<false, true>) : dkv(relbias_bwd_dkv_kernel<false, false>);
+}

@@ -1,0 +1,234 @@
+// Balance loss of a router with its per-expert counts, and its gradient, on the records of the top-2 / switch gates.
+//
+//   n_b = number of real tokens of row b, G = number of rows with n_b > 0, k = choices counted per token (1 or 2)
+//   c_be = how many of the row's choices name expert e,  P_be = sum of the row's probabilities of e
+//   loss = coef E / G * sum_b 1 / (k n_b^2) * sum_e c_be P_be         (1 * coef for a perfectly even routing)
+//   dlogits_bse = p_bse (w_be - sum_e' p_bse' w_be'),  w_be = coef E c_be / (G k n_b^2)       (c is a count: no gradient)
+//
+// The gate's own gradient (softmax backward of the kept choices' gate gradients) has the same form, so one pass over the
+// probabilities serves both.  Memory bound at large sizes and launch bound at small ones: forward is one pass and one
+// small joining launch, backward one launch.
+#include "common.h"
+
+namespace {
+
+constexpr int BAL_THREADS = 256;
+constexpr int BAL_MAX_E = 64;
+constexpr int BAL_BLOCKS = 512;                     // a row is cut into slabs until about this many blocks run
+
+__device__ __forceinline__ int bal_length(const int32_t *lengths, int b, int S) {
+    if (!lengths) return S;
+    const int n = lengths[b];
+    return n < 0 ? 0 : (n > S ? S : n);
+}
+
+// number of rows with tokens, by the whole block (BAL_THREADS or more threads, `red` 16 floats of LDS)
+__device__ __forceinline__ float bal_rows(const int32_t *lengths, int B, int S, float *red) {
+    if (!lengths) return (float)B;
+    float v = 0.f;
+    for (int i = threadIdx.x; i < B; i += blockDim.x) v += bal_length(lengths, i, S) > 0 ? 1.f : 0.f;
+    return block_sum(v, red);                       // whole numbers below 2^24: exact in any order
+}
+
+// one slab of one row: counts, kept counts and probability sums of every expert
+template <int V>
+__global__ __launch_bounds__(BAL_THREADS) void balance_count_kernel(const float *probs, const int32_t *index, const int32_t *slot,
+                                                                  const int32_t *lengths, int32_t *counts, int32_t *kept, float *psum,
+                                                                  int S, int E, int choices, int slab) {
+    __shared__ int32_t cnt[2][BAL_MAX_E];
+    __shared__ float red[BAL_THREADS * V];
+    const int b = blockIdx.y, n = bal_length(lengths, b, S);
+    const int s0 = blockIdx.x * slab, s1 = s0 + slab < n ? s0 + slab : n;
+    for (int i = threadIdx.x; i < 2 * BAL_MAX_E; i += BAL_THREADS) cnt[i / BAL_MAX_E][i % BAL_MAX_E] = 0;
+    __syncthreads();
+    for (int s = s0 + (int)threadIdx.x; s < s1; s += BAL_THREADS) {
+        const int64_t rec = ((int64_t)b * S + s) * 2;
+        for (int k = 0; k < choices; ++k) {
+            const int e = index[rec + k];
+            if (e >= 0 && e < E) {                  // whole numbers: the order of these additions does not show
+                atomicAdd(&cnt[0][e], 1);
+                if (slot[rec + k] > 0) atomicAdd(&cnt[1][e], 1);
+            }
+        }
+    }
+    const int cols = E / V, per = BAL_THREADS / cols, c = threadIdx.x % cols, r = threadIdx.x / cols;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    if (r < per) {
+        const float *p = probs + (int64_t)b * S * E + c * V;
+#pragma unroll 4
+        for (int s = s0 + r; s < s1; s += per) {
+            if (V == 4) {
+                const f32x4 x = *(const f32x4 *)(p + (int64_t)s * E);
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] += x[i];
+            } else {
+                acc[0] += p[(int64_t)s * E];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = acc[i];
+    __syncthreads();
+    if ((int)threadIdx.x < E) {
+        float v = 0.f;
+        for (int i = 0; i < per; ++i) v += red[i * E + threadIdx.x];
+        const int64_t at = ((int64_t)b * gridDim.x + blockIdx.x) * E + threadIdx.x;
+        counts[at] = cnt[0][threadIdx.x];
+        kept[at] = cnt[1][threadIdx.x];
+        psum[at] = v;
+    }
+}
+
+// joins the slabs of every row (slabs == 1: counts, kept, psum are the first kernel's own outputs) and adds up the loss
+__global__ __launch_bounds__(1024) void balance_join_kernel(const int32_t *lengths, const int32_t *pcounts, const int32_t *pkept,
+                                                          const float *ppsum, int32_t *counts, int32_t *kept, float *psum, float *loss,
+                                                          int B, int S, int E, int slabs, float coef, int choices) {
+    __shared__ float red[16];
+    const float G = bal_rows(lengths, B, S, red);
+    float v = 0.f;
+    for (int64_t i = threadIdx.x; i < (int64_t)B * E; i += 1024) {
+        const int b = (int)(i / E), e = (int)(i - (int64_t)b * E);
+        int32_t c = 0, k = 0;
+        float p = 0.f;
+        for (int z = 0; z < slabs; ++z) {
+            const int64_t at = ((int64_t)b * slabs + z) * E + e;
+            c += pcounts[at];
+            k += pkept[at];
+            p += ppsum[at];
+        }
+        if (slabs > 1) {
+            counts[i] = c;
+            kept[i] = k;
+            psum[i] = p;
+        }
+        const float n = (float)bal_length(lengths, b, S);
+        if (n > 0.f) v += (float)c / n * (p / n);
+    }
+    v = block_sum(v, red);
+    if (threadIdx.x == 0) loss[0] = G > 0.f ? coef * (float)E / (G * (float)choices) * v : 0.f;
+}
+
+// a group of lanes per token, V experts a lane
+template <int V>
+__global__ __launch_bounds__(BAL_THREADS) void balance_bwd_kernel(const float *probs, const int32_t *index, const int32_t *slot,
+                                                                const float *dgate, const int32_t *counts, const int32_t *lengths,
+                                                                float *dlogits, int B, int S, int E, float coef, int choices, int slab,
+                                                                int group_log2) {
+    __shared__ float red[16];
+    const int b = blockIdx.y, n = bal_length(lengths, b, S);
+    const float G = bal_rows(lengths, B, S, red);
+    const int j = threadIdx.x & ((1 << group_log2) - 1), e0 = j * V;
+    float w[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        w[i] = n > 0 && e0 + i < E ? coef * (float)E / (G * (float)choices) * ((float)counts[(int64_t)b * E + e0 + i] / (float)n / (float)n) : 0.f;
+    const int s_end = (int)(blockIdx.x + 1) * slab < S ? (int)(blockIdx.x + 1) * slab : S;
+    for (int s = blockIdx.x * slab + (int)(threadIdx.x >> group_log2); s < s_end; s += BAL_THREADS >> group_log2) {
+        const int64_t tok = (int64_t)b * S + s;
+        float p[V], g[V], dot = 0.f;
+        if (V == 4 && e0 < E) {
+            const f32x4 x = *(const f32x4 *)(probs + tok * E + e0);
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[i] = x[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[i] = e0 + i < E ? probs[tok * E + e0 + i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = s < n ? w[i] : 0.f;
+        if (dgate) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int e = index[tok * 2 + k];
+                const float d = slot[tok * 2 + k] > 0 ? dgate[tok * 2 + k] : 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] += e == e0 + i ? d : 0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) dot += p[i] * g[i];
+        for (int o = 0; o < group_log2; ++o) dot += __shfl_xor(dot, 1 << o, 64);
+        if (V == 4 && e0 < E) {
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = p[i] * (g[i] - dot);
+            *(f32x4 *)(dlogits + tok * E + e0) = x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (e0 + i < E) dlogits[tok * E + e0 + i] = p[i] * (g[i] - dot);
+        }
+    }
+}
+
+int bal_check(const char *name, int64_t B, int64_t S, int64_t E, int choices) {
+    HAPMI_REQUIRE(B >= 0 && S >= 1 && E >= 1 && (choices == 1 || choices == 2), HAPMI_EINVAL, "%s: bad argument", name);
+    HAPMI_REQUIRE(E <= BAL_MAX_E && B <= 65535 && S < (1ll << 24), HAPMI_ELIMIT, "%s: at most %d experts, 65535 rows and 2^24 - 1 tokens a row", name, BAL_MAX_E);
+    return HAPMI_OK;
+}
+
+// tokens a block takes: about 16 KiB of probabilities at least, whole rows once there are BAL_BLOCKS of them
+int64_t bal_slab(int64_t B, int64_t S, int64_t E) {
+    const int64_t least = hapmi_cdiv(4096, E);
+    int64_t slabs = hapmi_cdiv(BAL_BLOCKS, B);
+    if (slabs > hapmi_cdiv(S, least)) slabs = hapmi_cdiv(S, least);
+    return hapmi_cdiv(S, slabs);
+}
+
+}  // namespace
+
+extern "C" int hapmi_balance_workspace_elems(int64_t B, int64_t S, int64_t E, int64_t *elems_host) {
+    const int rc = bal_check("balance_workspace_elems", B, S, E, 1);
+    if (rc) return rc;
+    HAPMI_REQUIRE(elems_host, HAPMI_EINVAL, "balance_workspace_elems: null pointer");
+    const int64_t slabs = B ? hapmi_cdiv(S, bal_slab(B, S, E)) : 1;
+    *elems_host = slabs > 1 ? 3 * B * slabs * E : 0;
+    return HAPMI_OK;
+}
+
+extern "C" int hapmi_balance_loss_fwd(const float *probs, const int32_t *index, const int32_t *slot, const int32_t *lengths, float *loss,
+                                      int32_t *counts, int32_t *kept, float *prob_sum, int64_t B, int64_t S, int64_t E, float coef, int choices,
+                                      float *workspace, int64_t workspace_elems, hapmi_stream_t stream) {
+    const char *name = "balance_loss_fwd";
+    const int rc = bal_check(name, B, S, E, choices);
+    if (rc) return rc;
+    HAPMI_REQUIRE(B >= 1, HAPMI_EINVAL, "%s: empty batch (the loss would stay unwritten)", name);
+    HAPMI_REQUIRE(probs && index && slot && loss && counts && kept && prob_sum, HAPMI_EINVAL, "%s: null pointer", name);
+    HAPMI_REQUIRE((uintptr_t)probs % 16 == 0, HAPMI_EALIGN, "%s: probs must be 16-byte aligned", name);
+    const int64_t slab = bal_slab(B, S, E), slabs = hapmi_cdiv(S, slab), n = B * slabs * E;
+    HAPMI_REQUIRE(slabs == 1 || (workspace && workspace_elems >= 3 * n), HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name,
+                  (long long)(workspace ? workspace_elems : 0), (long long)(3 * n));
+    int32_t *pc = slabs > 1 ? (int32_t *)workspace : counts, *pk = slabs > 1 ? (int32_t *)workspace + n : kept;
+    float *pp = slabs > 1 ? workspace + 2 * n : prob_sum;
+    const dim3 grid((unsigned)slabs, (unsigned)B), block(BAL_THREADS);
+    hipStream_t st = (hipStream_t)stream;
+    if (E % 4 == 0) hipLaunchKernelGGL((balance_count_kernel<4>), grid, block, 0, st, probs, index, slot, lengths, pc, pk, pp, (int)S, (int)E, choices, (int)slab);
+    else hipLaunchKernelGGL((balance_count_kernel<1>), grid, block, 0, st, probs, index, slot, lengths, pc, pk, pp, (int)S, (int)E, choices, (int)slab);
+    HAPMI_CHECK_LAUNCH(name);
+    hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(1024), 0, st, lengths, (const int32_t *)pc, (const int32_t *)pk, (const float *)pp, counts, kept, prob_sum,
+                       loss, (int)B, (int)S, (int)E, (int)slabs, coef, choices);
+    HAPMI_CHECK_LAUNCH(name);
+    return HAPMI_OK;
+}
+
+extern "C" int hapmi_balance_loss_bwd(const float *probs, const int32_t *index, const int32_t *slot, const float *dgate, const int32_t *counts,
+                                      const int32_t *lengths, float *dlogits, int64_t B, int64_t S, int64_t E, float coef, int choices,
+                                      hapmi_stream_t stream) {
+    const char *name = "balance_loss_bwd";
+    const int rc = bal_check(name, B, S, E, choices);
+    if (rc) return rc;
+    if (B == 0) return HAPMI_OK;
+    HAPMI_REQUIRE(probs && counts && dlogits && (!dgate || (index && slot)), HAPMI_EINVAL, "%s: null pointer", name);
+    HAPMI_REQUIRE((uintptr_t)probs % 16 == 0 && (uintptr_t)dlogits % 16 == 0, HAPMI_EALIGN, "%s: probs and dlogits must be 16-byte aligned", name);
+    const int V = E % 4 == 0 ? 4 : 1;
+    int group_log2 = 0;
+    while ((V << group_log2) < E) ++group_log2;
+    const int64_t slab = bal_slab(B, S, E);
+    const dim3 grid((unsigned)hapmi_cdiv(S, slab), (unsigned)B), block(BAL_THREADS);
+    if (V == 4) hipLaunchKernelGGL((balance_bwd_kernel<4>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, (int)slab, group_log2);
+    else hipLaunchKernelGGL((balance_bwd_kernel<1>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, (int)slab, group_log2);
+    HAPMI_CHECK_LAUNCH(name);
+    return HAPMI_OK;
+}

@@ -7,6 +7,7 @@ are refused: there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import List, Optional, Sequence
 
@@ -773,6 +774,84 @@ def layernorm_bwd(dy, y, rstd, dx_add, dx, dx_drop=None, drop=None):
                                             dtype_code(y), _stream()))
 
 
+def rotary_table(n_positions: int, rot: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """Cosines and sines of the rotation angles position * base ** (-2 i / rot), float32 [n_positions, rot / 2, 2]: the
+    angles and their functions in float64 (a far position's angle has lost its fraction in float32), rounded once."""
+    if n_positions < 1 or rot < 2 or rot % 2 or not base > 0:
+        raise ValueError("rotary_table: at least one position, an even number of rotated dimensions and a positive base expected")
+    freq = float(base) ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
+    angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.stack([angle.cos(), angle.sin()], -1).float().contiguous()
+
+
+def _qk_norm_args(what, qkv, b, S, H, q_gain, k_gain, rotary, positions):
+    """(head dimension, table positions, rotated dimensions) after the checks that both directions share."""
+    dtype_code(qkv)
+    if b < 0 or S < 1 or H < 1 or qkv.dim() != 3 or qkv.shape[0] != b or qkv.shape[1] != S or qkv.shape[2] % (3 * H):
+        raise ValueError(f"{what}: a packed projection [b, S, 3 * H * head_dim] expected")
+    D = qkv.shape[2] // (3 * H)
+    for g in (q_gain, k_gain):
+        if g is not None and (g.dtype != torch.float32 or g.numel() != D or not g.is_contiguous()):
+            raise TypeError(f"{what}: gains must be {D} contiguous float32")
+    if rotary is not None and (rotary.dtype != torch.float32 or rotary.dim() != 3 or rotary.shape[2] != 2 or not rotary.is_contiguous()):
+        raise TypeError(f"{what}: the angle table must be a contiguous float32 [positions, rot / 2, 2] tensor")
+    if positions is not None and (positions.dtype != torch.int32 or positions.numel() != b * S or not positions.is_contiguous()):
+        raise TypeError(f"{what}: positions must be b * S contiguous int32")
+    return D, (rotary.shape[0] if rotary is not None else 0), (2 * rotary.shape[1] if rotary is not None else 0)
+
+
+def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None, positions=None, interleaved=False, eps=1e-6):
+    """Queries and keys of the packed projection ``qkv`` [b, S, 3 * H * head_dim] normalised per head (root mean square,
+    float32 gains [head_dim]) and rotated by position (``rotary`` from ``rotary_table``; its first 2 * shape[1] dimensions;
+    None: norm only), values copied; ``out`` may be ``qkv`` itself (in place).  ``positions``: int32 [b, S] (None: the index
+    inside the sequence); one outside the table gives NaN.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
+    what = "qk_norm_rotary_fwd"
+    _here(what, qkv, out, q_gain, k_gain, rotary, positions)
+    D, n_pos, rot = _qk_norm_args(what, qkv, b, S, H, q_gain, k_gain, rotary, positions)
+    if out.dtype != qkv.dtype:
+        raise TypeError(f"{what}: dtype mismatch")
+    _need(qkv, qkv.numel(), f"{what} qkv")
+    _need(out, qkv.numel(), f"{what} out")
+    if out.data_ptr() != qkv.data_ptr():
+        _no_overlap(what, (out, qkv))
+    _no_overlap(what, *[(out, t) for t in (q_gain, k_gain, rotary, positions)])
+    check(lib().hapmi_qk_norm_rotary_fwd(_ptr(qkv), _ptr(out), _ptr(q_gain), _ptr(k_gain), _ptr(rotary), n_pos, rot, int(interleaved),
+                                         _ptr(positions), b, S, H, D, ctypes.c_float(eps), dtype_code(qkv), _stream()))
+
+
+def qk_norm_rotary_workspace_elems(D: int) -> int:
+    """Float32 elements of the scratch buffer that ``qk_norm_rotary_bwd`` needs for the gains' gradients."""
+    need = ctypes.c_int64()
+    check(_lib._load().hapmi_qk_norm_rotary_workspace_elems(D, ctypes.byref(need)))
+    return need.value
+
+
+def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_gain=None, dk_gain=None, rotary=None,
+                       positions=None, interleaved=False, eps=1e-6, accumulate=False, workspace=None):
+    """Backward of ``qk_norm_rotary_fwd``: ``dqkv`` from ``dout`` (``dqkv`` may be ``dout``: in place) and forward's input
+    ``qkv``; ``dq_gain`` / ``dk_gain`` float32 [head_dim] (None: not wanted; ``accumulate``: added to)."""
+    what = "qk_norm_rotary_bwd"
+    _here(what, dout, qkv, dqkv, q_gain, k_gain, dq_gain, dk_gain, rotary, positions, workspace)
+    D, n_pos, rot = _qk_norm_args(what, qkv, b, S, H, q_gain, k_gain, rotary, positions)
+    if dout.dtype != qkv.dtype or dqkv.dtype != qkv.dtype:
+        raise TypeError(f"{what}: dtype mismatch")
+    for t in (qkv, dout, dqkv):
+        _need(t, qkv.numel(), what)
+    for g in (dq_gain, dk_gain):
+        if g is not None and (g.dtype != torch.float32 or g.numel() != D or not g.is_contiguous()):
+            raise TypeError(f"{what}: gain gradients must be {D} contiguous float32")
+    if dqkv.data_ptr() != dout.data_ptr():
+        _no_overlap(what, (dqkv, dout))
+    _no_overlap(what, *[(w, t) for w in (dqkv, dq_gain, dk_gain) for t in (qkv, q_gain, k_gain, rotary, positions)], (dq_gain, dk_gain),
+                (dqkv, dq_gain), (dqkv, dk_gain))
+    ws, ws_elems = None, 0
+    if dq_gain is not None or dk_gain is not None:
+        ws, ws_elems = _scratch(what, workspace, qk_norm_rotary_workspace_elems(D), qkv.device)
+    check(lib().hapmi_qk_norm_rotary_bwd(_ptr(dout), _ptr(qkv), _ptr(dqkv), _ptr(q_gain), _ptr(k_gain), _ptr(dq_gain), _ptr(dk_gain),
+                                         int(accumulate), _ptr(rotary), n_pos, rot, int(interleaved), _ptr(positions), b, S, H, D,
+                                         ctypes.c_float(eps), dtype_code(qkv), ws, ws_elems, _stream()))
+
+
 def softmax_fwd(x, mask, p, rows, width, ld, mask_rows=1):
     _dev(x, mask, p)
     _need(x, _span(rows, width, ld), "softmax_fwd x")
@@ -861,6 +940,152 @@ def attention_bwd(qkv, out, dout, lse, mask, dqkv, delta_ws, b, S, H, scale, cau
     check(lib().hapmi_attention_bwd_dropout(_ptr(qkv), _ptr(out), _ptr(dout), _ptr(lse), _ptr(mask), int(causal),
                                             _ptr(dqkv), _ptr(delta_ws), b, S, H, ctypes.c_float(scale),
                                             _ptr(keep_rows), _ptr(keep_cols), ctypes.c_float(p), _stream()))
+
+
+def _here(what, *tensors):
+    """The kernels run on the current device's current stream: every operand has to live there."""
+    _dev(*tensors)
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise _lib.HapmiError(f"{what}: a tensor on {t.device} while cuda:{cur} is the current device")
+
+
+@functools.lru_cache(maxsize=None)
+def relative_bucket_starts(n_buckets: int, max_distance: int, bidirectional: bool = True):
+    """First distance of every bucket of one side of a relative position bias with ``n_buckets`` buckets (two sides share
+    them when ``bidirectional``): the first half of a side's buckets hold one distance each, the others grow
+    geometrically, the last one ends the growth towards ``max_distance`` and holds everything beyond.  With e = half of
+    the side's buckets and w the rest, bucket e + j starts at the smallest distance d >= e * (max_distance / e) ** (j / w);
+    the comparison is made in whole numbers, so a distance on a border is in the farther bucket."""
+    n_buckets, max_distance = int(n_buckets), int(max_distance)
+    if n_buckets < 2 or (bidirectional and n_buckets % 2):
+        raise ValueError(f"relative_bucket_starts: {n_buckets} buckets: at least 2, and an even number for two sides")
+    side = n_buckets // 2 if bidirectional else n_buckets
+    if side > _lib.RELBIAS_MAX_SIDE:
+        raise ValueError(f"relative_bucket_starts: {side} buckets on a side, at most {_lib.RELBIAS_MAX_SIDE}")
+    if side == 1:
+        return (0,)
+    near = side // 2
+    wide = side - near
+    if max_distance <= near or max_distance > _lib.RELBIAS_MAX_DISTANCE:
+        raise ValueError(f"relative_bucket_starts: max_distance {max_distance} must lie in ({near}, {_lib.RELBIAS_MAX_DISTANCE}]")
+    starts, d = list(range(near + 1)), near
+    for j in range(1, wide):
+        bound = max_distance ** j * near ** (wide - j)
+        while d ** wide < bound:
+            d += 1
+        starts.append(d)
+    if starts[-1] > _lib.RELBIAS_MAX_REACH:
+        raise ValueError(f"relative_bucket_starts: the last bucket starts at distance {starts[-1]}, at most "
+                         f"{_lib.RELBIAS_MAX_REACH} is handled")
+    return tuple(starts)
+
+
+@functools.lru_cache(maxsize=None)
+def _bucket_array(n_buckets, max_distance, bidirectional):
+    starts = relative_bucket_starts(n_buckets, max_distance, bidirectional)
+    return (ctypes.c_int32 * len(starts))(*starts)
+
+
+def _relbias(what, table, H, max_distance, bidirectional, causal):
+    if table.dim() != 2 or table.shape[1] != H or table.dtype != torch.float32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{what}: the table must be a float32 [buckets, {H}] tensor with unit column stride")
+    bidirectional = (not causal) if bidirectional is None else bool(bidirectional)
+    arr = _bucket_array(int(table.shape[0]), int(max_distance), bidirectional)
+    a = _lib.RelBias()
+    a.table = table.data_ptr()
+    a.ld = max(table.stride(0), H)
+    a.n_buckets, a.bidirectional = table.shape[0], int(bidirectional)
+    a.starts_host = ctypes.addressof(arr)
+    a._keep = arr
+    return a
+
+
+def _check_lengths(what, lengths, b):
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.numel() != b or not lengths.is_contiguous()):
+        raise TypeError(f"{what}: lengths must be {b} contiguous int32")
+
+
+def _no_overlap(what, *pairs):
+    """Every pair (written, other) must lie in separate memory."""
+    end = lambda t: t.data_ptr() + (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
+    for w, o in pairs:
+        if w is not None and o is not None and w.numel() and o.numel() and w.data_ptr() < end(o) and o.data_ptr() < end(w):
+            raise ValueError(f"{what}: an output shares memory with another operand")
+
+
+def _scratch(what, workspace, elems: int, device):
+    """Pointer to float32 scratch of ``elems`` elements: the caller's, or one of this call's own (which the pointer object
+    keeps, so that a recorded launch list replays with memory that is still there)."""
+    if workspace is None:
+        workspace = torch.empty(elems, dtype=torch.float32, device=device)
+    if workspace.dtype != torch.float32:
+        raise TypeError(f"{what}: float32 workspace expected")
+    _need(workspace, elems, f"{what} workspace")
+    ptr = _ptr(workspace)
+    ptr._keep = workspace
+    return ptr, workspace.numel()
+
+
+def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128, bidirectional=None, causal=False,
+                          lengths=None, keep_rows=None, p=0.0):
+    """``attention_fwd`` with a learned relative position bias: scores scale * q_i k_j + table[bucket(j - i), head],
+    ``table`` float32 [buckets, H] (rows may be strided: the columns of a device's heads).  Buckets as
+    ``relative_bucket_starts(buckets, max_distance, bidirectional)`` cuts the distances; ``bidirectional`` None: two sides
+    unless ``causal``.  ``lengths`` (int32 [b]): the sequences of a padded batch; rows behind a sequence's end get zeros and
+    lse = -inf, its keys there are not read.  ``keep_rows`` / ``p``: dropout of the probabilities."""
+    what = "attention_relbias_fwd"
+    _here(what, qkv, table, out, lse, lengths, keep_rows)
+    _check_attn(qkv, out, lse, None, b, S, H)
+    _check_lengths(what, lengths, b)
+    _no_overlap(what, (out, qkv), (lse, qkv), (lse, out), (lse, table), (out, table))
+    rel = _relbias(what, table, H, max_distance, bidirectional, causal)
+    if keep_rows is not None:
+        _check_keep(keep_rows, b, S, H, "keep_rows")
+    check(lib().hapmi_attention_relbias_fwd(_ptr(qkv), ctypes.byref(rel), int(causal), _ptr(lengths), _ptr(out), _ptr(lse),
+                                            b, S, H, ctypes.c_float(scale), _ptr(keep_rows), ctypes.c_float(p), _stream()))
+
+
+def attention_relbias_workspace_elems(table, b, S, H, max_distance=128, bidirectional=None, causal=False) -> int:
+    """Float32 elements of the scratch buffer that ``attention_relbias_bwd`` needs."""
+    rel = _relbias("attention_relbias_workspace_elems", table, H, max_distance, bidirectional, causal)
+    need = ctypes.c_int64()
+    check(_lib._load().hapmi_attention_relbias_workspace_elems(ctypes.byref(rel), b, S, H, ctypes.byref(need)))
+    return need.value
+
+
+def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b, S, H, scale, max_distance=128,
+                          bidirectional=None, causal=False, lengths=None, keep_rows=None, keep_cols=None, p=0.0,
+                          accumulate=False, workspace=None):
+    """Backward of ``attention_relbias_fwd``: ``dqkv`` completely and ``dtable`` (float32 [buckets, H], rows may be strided;
+    ``accumulate``: added to, for a table that several layers share).  ``out`` and ``lse`` as forward left them.
+    ``workspace``: float32 scratch of ``attention_relbias_workspace_elems`` (None: taken from torch's allocator)."""
+    what = "attention_relbias_bwd"
+    _here(what, qkv, table, out, dout, lse, dqkv, dtable, delta_ws, lengths, keep_rows, keep_cols, workspace)
+    _check_attn(qkv, out, lse, None, b, S, H)
+    _check_lengths(what, lengths, b)
+    _need(dout, b * S * H * 64, "attention dout")
+    _need(dqkv, b * S * 3 * H * 64, "attention dqkv")
+    _need(delta_ws, b * H * S, "attention delta")
+    if dout.dtype != torch.bfloat16 or dqkv.dtype != torch.bfloat16 or delta_ws.dtype != torch.float32:
+        raise TypeError(f"{what}: dtype mismatch")
+    rel = _relbias(what, table, H, max_distance, bidirectional, causal)
+    if dtable.shape != table.shape or dtable.dtype != torch.float32 or (H > 1 and dtable.stride(1) != 1):
+        raise ValueError(f"{what}: dtable must be float32 of the table's shape with unit column stride")
+    _no_overlap(what, *[(w, o) for w in (dqkv, delta_ws) for o in (qkv, out, dout, lse, table)], (dqkv, delta_ws))
+    if (keep_rows is None) != (keep_cols is None):
+        raise ValueError(f"{what}: keep_rows and keep_cols come together")
+    if keep_rows is not None:
+        _check_keep(keep_rows, b, S, H, "keep_rows")
+        _check_keep(keep_cols, b, S, H, "keep_cols")
+    need = ctypes.c_int64()
+    check(_lib._load().hapmi_attention_relbias_workspace_elems(ctypes.byref(rel), b, S, H, ctypes.byref(need)))
+    ws, ws_elems = _scratch(what, workspace, need.value, qkv.device)
+    check(lib().hapmi_attention_relbias_bwd(
+        _ptr(qkv), ctypes.byref(rel), int(causal), _ptr(lengths), _ptr(out), _ptr(dout), _ptr(lse), _ptr(dqkv), _ptr(dtable),
+        max(dtable.stride(0), H), int(accumulate), _ptr(delta_ws), ws, ws_elems, b, S, H,
+        ctypes.c_float(scale), _ptr(keep_rows), _ptr(keep_cols), ctypes.c_float(p), _stream()))
 
 
 def head_parallel_attention(x, w_in, b_in, w_out, num_heads, mask=None):
@@ -1226,6 +1451,60 @@ def top2_gate_bwd(r, dgate, dlogits):
         raise TypeError("top2_gate_bwd: float32 expected")
     check(lib().hapmi_top2_gate_bwd(_ptr(r["probs"]), _ptr(r["index"]), _ptr(r["slot"]), _ptr(dgate), _ptr(dlogits),
                                     B, S, E, _stream()))
+
+
+def _check_balance(what, r, E, lengths, B, S):
+    _check_routing(r, B, S, E)
+    _here(what, *r.values(), lengths)
+    if r["probs"].dtype != torch.float32:
+        raise TypeError(f"{what}: float32 probabilities expected")
+    _check_lengths(what, lengths, B)
+
+
+def _check_counts(what, t, B, E, dtype):
+    if t.dtype != dtype or t.numel() != B * E or not t.is_contiguous():
+        raise TypeError(f"{what}: counts are contiguous int32 [B, E], probability sums float32 [B, E]")
+
+
+def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, lengths=None, workspace=None):
+    """Balance loss of the routing records ``r`` (``top2_gate`` / ``switch_gate``) into ``loss`` (float32 [1]) and what it is
+    made of: ``counts`` (int32 [B, E]: choices of every expert before capacity; ``choices`` = 1: first choices, 2: both),
+    ``kept`` (int32 [B, E]: those that got a slot), ``prob_sum`` (float32 [B, E]).
+    loss = coef * E * mean over the rows of sum_e counts / (choices * n) * prob_sum / n, n the row's tokens: all S, or
+    ``lengths`` (int32 [B]) of a padded batch (empty rows do not enter the mean).  Perfectly even routing gives coef."""
+    what = "balance_loss_fwd"
+    B, S, E = r["probs"].shape
+    _check_balance(what, r, E, lengths, B, S)
+    _here(what, loss, counts, kept, prob_sum, workspace)
+    if loss.dtype != torch.float32 or loss.numel() != 1:
+        raise TypeError(f"{what}: the loss is one float32")
+    _check_counts(what, counts, B, E, torch.int32)
+    _check_counts(what, kept, B, E, torch.int32)
+    _check_counts(what, prob_sum, B, E, torch.float32)
+    outs = (loss, counts, kept, prob_sum)
+    _no_overlap(what, *[(w, t) for w in outs for t in (*r.values(), lengths)], *[(a, c) for i, a in enumerate(outs) for c in outs[:i]])
+    need = ctypes.c_int64()
+    check(_lib._load().hapmi_balance_workspace_elems(B, S, E, ctypes.byref(need)))
+    ws, ws_elems = _scratch(what, workspace, need.value, loss.device) if need.value else (None, 0)
+    check(lib().hapmi_balance_loss_fwd(_ptr(r["probs"]), _ptr(r["index"]), _ptr(r["slot"]), _ptr(lengths), _ptr(loss), _ptr(counts), _ptr(kept),
+                                       _ptr(prob_sum), B, S, E, ctypes.c_float(coef), int(choices), ws, ws_elems, _stream()))
+
+
+def balance_loss_bwd(r, counts, dlogits, choices=2, coef=0.01, grad=1.0, dgate=None, lengths=None):
+    """Gradient of ``grad`` times the balance loss with respect to the router's logits, from forward's ``counts``; with
+    ``dgate`` (float32 [B, S, 2]) ``dlogits`` also holds what ``top2_gate_bwd`` gives for it, in the same pass."""
+    what = "balance_loss_bwd"
+    B, S, E = r["probs"].shape
+    _check_balance(what, r, E, lengths, B, S)
+    _here(what, counts, dlogits, dgate)
+    _check_counts(what, counts, B, E, torch.int32)
+    _need(dlogits, B * S * E, f"{what} dlogits")
+    _need(dgate, B * S * 2, f"{what} dgate")
+    if dlogits.dtype != torch.float32 or (dgate is not None and dgate.dtype != torch.float32):
+        raise TypeError(f"{what}: float32 expected")
+    _no_overlap(what, *[(dlogits, t) for t in (*r.values(), counts, dgate, lengths)])
+    check(lib().hapmi_balance_loss_bwd(_ptr(r["probs"]), _ptr(r["index"]), _ptr(r["slot"]), _ptr(dgate), _ptr(counts), _ptr(lengths), _ptr(dlogits),
+                                       B, S, E, ctypes.c_float(float(coef) * float(grad)), int(choices), _stream()))
 
 
 def top2_densify(r, E, C):

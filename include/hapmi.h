@@ -274,6 +274,28 @@ int hapmi_layernorm_bwd_dropout(const void *dy, const void *y, const float *rstd
                                 void *dx_drop, int64_t rows, int64_t width, float p, const int64_t *rng_state_dev,
                                 int64_t stream_id, int dtype, hapmi_stream_t stream);
 
+/* Norm of queries and keys per head and the rotation by position in one pass over a packed projection qkv[b, S, 3*H*D]
+ * (queries, keys, values of H heads), as it lies in front of hapmi_attention_fwd / hapmi_attention_relbias_fwd.  No
+ * counterpart in the reference (its models neither normalise nor rotate: models.py:79-81, torch's
+ * nn.TransformerEncoderLayer).  For every token and head: u = x / sqrt(mean(x^2) + eps), n = gain * u, and the first `rot`
+ * dimensions of n turned in pairs by the position's angles; values are copied (out == qkv: in place, they stay).
+ *   q_gain, k_gain  float32[D], shared by the heads, or NULL (ones)
+ *   angles          float32[n_pos][rot / 2][2] = cosine, sine; NULL with rot = 0: norm only
+ *   interleaved     pairs (2 i, 2 i + 1) instead of (i, i + rot / 2)
+ *   positions       int32[b * S] on the device, or NULL: the index inside the sequence.  A position outside
+ *                   [0, n_pos) gives NaN in the token's queries and keys
+ * D at most 256 and a multiple of 8 (bf16) / 4 (float32); rot a multiple of twice that (interleaved: of that).
+ * Backward: dqkv (== dout: in place) from dout and forward's input; dq_gain / dk_gain float32[D] or NULL, overwritten or
+ * (accumulate) added to; they need float32 workspace of hapmi_qk_norm_rotary_workspace_elems(D).  No atomics. */
+int hapmi_qk_norm_rotary_fwd(const void *qkv, void *out, const float *q_gain, const float *k_gain, const float *angles, int64_t n_pos,
+                             int64_t rot, int interleaved, const int32_t *positions, int64_t b, int64_t S, int64_t H, int64_t D,
+                             float eps, int dtype, hapmi_stream_t stream);
+int hapmi_qk_norm_rotary_workspace_elems(int64_t D, int64_t *elems_host);
+int hapmi_qk_norm_rotary_bwd(const void *dout, const void *qkv, void *dqkv, const float *q_gain, const float *k_gain, float *dq_gain,
+                             float *dk_gain, int accumulate, const float *angles, int64_t n_pos, int64_t rot, int interleaved,
+                             const int32_t *positions, int64_t b, int64_t S, int64_t H, int64_t D, float eps, int dtype,
+                             float *workspace, int64_t workspace_elems, hapmi_stream_t stream);
+
 /* softmax over the last dimension of [rows, width] (row stride ld elements, the same for
  * input and output) with an optional additive float32 mask[mask_rows, width] (contiguous;
  * row r uses mask row r % mask_rows), in place allowed:
@@ -317,6 +339,44 @@ int hapmi_attention_bwd_dropout(const void *qkv, const void *out, const void *do
                                 const float *mask, int causal, void *dqkv, float *delta_ws, int64_t b, int64_t S,
                                 int64_t H, float scale, const uint32_t *keep_rows, const uint32_t *keep_cols, float p,
                                 hapmi_stream_t stream);
+
+/* The same attention with a learned relative position bias: s_ij = scale <q_i, k_j> + table[bucket(j - i), h], h being the
+ * head (column of the table), and the table's gradient.  No counterpart in the reference, whose models add their
+ * positions to the input (models.py:79-81, 167, 504-509).
+ *   table          float32 [n_buckets][ld], ld >= H; an entry at or below -1e30 hides the pairs of its bucket
+ *   starts_host    the first distance of every bucket of one side: n_buckets / 2 (bidirectional) or n_buckets numbers,
+ *                  starts[0] = 0, never falling; bucket k of a side holds the distances starts[k] .. starts[k + 1] - 1, the
+ *                  last one all from its start on (a bucket whose start equals the next one's is never used).
+ *                  Bidirectional: distance |j - i|, keys behind the query (j > i) use the second half of the table.
+ *                  Otherwise: distance max(i - j, 0).
+ * At most HAPMI_RELBIAS_MAX_SIDE buckets a side, the last one starting at distance HAPMI_RELBIAS_MAX_REACH at most
+ * (the window of distances is held in LDS). */
+#define HAPMI_RELBIAS_MAX_SIDE 64
+#define HAPMI_RELBIAS_MAX_REACH 1024
+typedef struct {
+    const float *table;
+    int64_t ld;
+    int n_buckets;
+    int bidirectional;
+    const int32_t *starts_host;
+} hapmi_relbias;
+/* causal != 0: key j is visible to query i iff j <= i.  lengths: int32[b] on the device or NULL: the sequences of a padded
+ * batch; of sample z the first lengths[z] (clamped to 0 .. S) positions exist, later keys are not read and later rows get
+ * zeros (out, dqkv) and -inf (lse).  A query that sees nothing gets the same.  keep_rows / keep_cols / p: dropout of the
+ * probabilities as in hapmi_attention_fwd_dropout (NULL = none).  scale > 0.
+ * Backward takes out and lse as forward left them, writes dqkv completely and dtable[n_buckets][ld_dtable]'s columns
+ * 0 .. H - 1 (accumulate != 0: adds to them; b >= 1); delta_ws is float32 scratch of b*H*S elements, workspace float32 scratch
+ * of the number of elements that hapmi_attention_relbias_workspace_elems reports.  No atomics between waves: the same call
+ * gives the same bits. */
+int hapmi_attention_relbias_fwd(const void *qkv, const hapmi_relbias *bias_host, int causal, const int32_t *lengths, void *out,
+                                float *lse, int64_t b, int64_t S, int64_t H, float scale, const uint32_t *keep_rows,
+                                float p, hapmi_stream_t stream);
+int hapmi_attention_relbias_workspace_elems(const hapmi_relbias *bias_host, int64_t b, int64_t S, int64_t H, int64_t *elems_host);
+int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias *bias_host, int causal, const int32_t *lengths,
+                                const void *out, const void *dout, const float *lse, void *dqkv, float *dtable,
+                                int64_t ld_dtable, int accumulate, float *delta_ws, float *workspace,
+                                int64_t workspace_elems, int64_t b, int64_t S, int64_t H, float scale,
+                                const uint32_t *keep_rows, const uint32_t *keep_cols, float p, hapmi_stream_t stream);
 
 /* torch.log_softmax + F.nll_loss(reduction='sum', ignore_index) (hap.rs:1829, 1881) and their
  * backward in one pass: row_loss[rows] float32, dlogits = (softmax - onehot) * grad_scale for
@@ -400,6 +460,22 @@ int hapmi_switch_gate(const float *logits, float *probs, int32_t *index, int32_t
 /* dlogits = softmax backward of the two kept gate gradients */
 int hapmi_top2_gate_bwd(const float *probs, const int32_t *index, const int32_t *slot, const float *dgate,
                         float *dlogits, int64_t B, int64_t S, int64_t E, hapmi_stream_t stream);
+/* Balance loss of the router on the records of either gate, the counts that it is made of, and its gradient.  No counterpart
+ * in the reference (models.py:452-502 has no auxiliary loss).  Of row b the first n_b = lengths[b] tokens count (lengths NULL:
+ * all S; int32[B] on the device); choices = 1 counts every token's first choice, 2 both:
+ *   counts[b, e] = choices of expert e (before capacity), kept[b, e] = those of them that got a slot,
+ *   prob_sum[b, e] = sum of the probabilities,
+ *   loss[0] = coef * E / (rows with tokens) * sum_b sum_e counts[b, e] / (choices * n_b) * prob_sum[b, e] / n_b.
+ * Backward: dlogits = softmax backward of coef's loss through prob_sum (counts carry no gradient), 0 for tokens that do not
+ * count; with dgate also the result of hapmi_top2_gate_bwd, in the same pass.  coef there = coef of the loss times the
+ * gradient that reaches it.  E <= 64.  workspace: hapmi_balance_workspace_elems floats (0: may be NULL). */
+int hapmi_balance_workspace_elems(int64_t B, int64_t S, int64_t E, int64_t *elems_host);
+int hapmi_balance_loss_fwd(const float *probs, const int32_t *index, const int32_t *slot, const int32_t *lengths, float *loss,
+                           int32_t *counts, int32_t *kept, float *prob_sum, int64_t B, int64_t S, int64_t E, float coef, int choices,
+                           float *workspace, int64_t workspace_elems, hapmi_stream_t stream);
+int hapmi_balance_loss_bwd(const float *probs, const int32_t *index, const int32_t *slot, const float *dgate, const int32_t *counts,
+                           const int32_t *lengths, float *dlogits, int64_t B, int64_t S, int64_t E, float coef, int choices,
+                           hapmi_stream_t stream);
 /* dense [B, S, E, C] tensors exactly as models.py:495-500 lays them out */
 int hapmi_top2_densify(const int32_t *index, const int32_t *slot, const float *gate, float *dispatch,
                        float *combine, int64_t B, int64_t S, int64_t E, int64_t C, hapmi_stream_t stream);

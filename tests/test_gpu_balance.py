@@ -1,0 +1,145 @@
+"""Balance loss, per-expert counts and the router's gradient on the GPU against the float64 formulas.
+
+Tolerances: probability sums add up to n values in [0, 1] in float32, at most n * 2^-24 of the sum; the loss is a sum of
+B * E such products, 16 more roundings; a gradient element is a handful of float32 operations on one token's values: 32 * 2^-24
+of the sum of its |terms|."""
+import pytest
+import torch
+
+from hap_amd import ops
+from oracle import layer_ops as L
+
+pytestmark = pytest.mark.gpu
+E24 = 2.0 ** -24
+
+
+def routing(cuda, seed, B, S, E, switch=False, capacity=None):
+    g = torch.Generator().manual_seed(seed)
+    logits = torch.randn(B, S, E, generator=g) + torch.randn(1, 1, E, generator=g)
+    gate = ops.switch_gate if switch else ops.top2_gate
+    r = gate(logits.to(cuda), capacity or max(2, 2 * S // E))
+    return r, torch.randn(B, S, 2, generator=g)
+
+
+def outputs(cuda, B, S, E):
+    nan = lambda *s: torch.full(s, float("nan"), device=cuda)  # noqa: E731
+    whole = lambda: torch.full((B, E), -77, dtype=torch.int32, device=cuda)  # noqa: E731
+    return nan(1), whole(), whole(), nan(B, E), nan(B, S, E)
+
+
+CASES = [(1, 1, 2, 1, None, False), (2, 7, 4, 2, None, False), (3, 64, 5, 1, None, True), (4, 33, 16, 2, [33, 0, 1, 20], False), (2, 512, 64, 2, None, False),
+         (1, 3000, 63, 2, [2999], False), (16, 512, 16, 1, None, False), (600, 5, 8, 2, None, False), (3, 900, 24, 1, [0, 0, 0], True), (1, 4097, 3, 2, None, False),
+         (5, 300, 61, 2, [300, 299, -4, 1000, 1], False)]
+
+
+@pytest.mark.parametrize("B,S,E,choices,lengths,switch", CASES)
+def test_loss_counts_and_gradient(cuda, B, S, E, choices, lengths, switch):
+    r, dgate = routing(cuda, B + S + E, B, S, E, switch)
+    loss, counts, kept, sums, d = outputs(cuda, B, S, E)
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    ops.balance_loss_fwd(r, loss, counts, kept, sums, choices=choices, coef=0.02, lengths=ln)
+    cpu = {k: v.cpu() for k, v in r.items()}
+    real = None if lengths is None else torch.tensor(lengths).clamp(0, S)
+    wl, wc, wk, ws, wd = L.balance(cpu["probs"], cpu["index"], cpu["slot"], choices, 0.02, real)
+    assert torch.equal(counts.cpu(), wc) and torch.equal(kept.cpu(), wk)
+    assert ((sums.double().cpu() - ws).abs() <= S * E24 * ws).all()
+    assert abs(loss.item() - wl.item()) <= (S + 16) * E24 * wl.item()
+    ops.balance_loss_bwd(r, counts, d, choices=choices, coef=0.01, grad=2.0, lengths=ln)
+    p = cpu["probs"].double()
+    n = torch.full((B,), S) if real is None else real
+    w = 0.02 * E * wc.double() / ((n > 0).sum().clamp(min=1) * choices * n.clamp(min=1)[:, None].double() ** 2)
+    size = p * (w[:, None] + (p * w[:, None]).sum(-1, keepdim=True))
+    assert ((d.double().cpu() - wd).abs() <= 32 * E24 * size + 1e-30).all()
+    for b in range(B):
+        assert (d[b, int(n[b]):] == 0).all()
+    # with the gate's own gradient in the same pass
+    _, _, _, _, both = L.balance(cpu["probs"], cpu["index"], cpu["slot"], choices, 0.02, real, dgate)
+    ops.balance_loss_bwd(r, counts, d, choices=choices, coef=0.02, dgate=dgate.to(cuda), lengths=ln)
+    dp = torch.zeros(B, S, E, dtype=torch.float64).scatter_add_(2, cpu["index"].long(), dgate.double().abs() * (cpu["slot"] > 0))
+    size = size + p * (dp + (p * dp).sum(-1, keepdim=True))
+    assert ((d.double().cpu() - both).abs() <= 32 * E24 * size + 1e-30).all()
+
+
+def test_agrees_with_the_gate_backward_at_coefficient_zero(cuda):
+    r, dgate = routing(cuda, 3, 4, 100, 16)
+    loss, counts, kept, sums, d = outputs(cuda, 4, 100, 16)
+    ops.balance_loss_fwd(r, loss, counts, kept, sums, coef=0.0)
+    assert loss.item() == 0.0
+    g = dgate.to(cuda)
+    ops.balance_loss_bwd(r, counts, d, coef=0.0, dgate=g)
+    want = torch.empty_like(d)
+    ops.top2_gate_bwd(r, g, want)
+    torch.testing.assert_close(d, want, rtol=1e-5, atol=1e-6)
+
+
+def test_gradient_against_differences(cuda):
+    """Counts do not move, so the loss is smooth in the logits: central differences along random directions.  The loss (about
+    coef) carries 2^-24 * sqrt(B S) relative noise; over a step of 0.05 that is 1e-4 of the slope's scale."""
+    B, S, E = 2, 200, 8
+    g = torch.Generator().manual_seed(2)
+    logits, step = torch.randn(B, S, E, generator=g), torch.randn(B, S, E, generator=g)
+    r = ops.top2_gate(logits.to(cuda), 60)
+    loss, counts, kept, sums, d = outputs(cuda, B, S, E)
+    ops.balance_loss_fwd(r, loss, counts, kept, sums, coef=1.0)
+    ops.balance_loss_bwd(r, counts, d, coef=1.0)
+    vals = []
+    for sign in (1, -1):
+        moved = dict(r, probs=torch.softmax((logits + sign * 0.05 * step).to(cuda), -1).contiguous())
+        ops.balance_loss_fwd(moved, loss, counts, kept, sums, coef=1.0)
+        vals.append(loss.item())
+    want = (d.double().cpu() * step.double()).sum().item()
+    assert abs((vals[0] - vals[1]) / 0.1 - want) < 1e-2 * d.double().norm().item() * step.double().norm().item() ** 0.5
+
+
+def test_an_expert_index_outside_the_range_counts_nowhere(cuda):
+    r, _ = routing(cuda, 1, 1, 8, 4)
+    r["index"][0, 3] = torch.tensor([-1, 4], dtype=torch.int32, device=cuda)
+    loss, counts, kept, sums, _ = outputs(cuda, 1, 8, 4)
+    ops.balance_loss_fwd(r, loss, counts, kept, sums, choices=2)
+    assert counts.sum().item() == 14
+
+
+def test_same_bits_every_time_and_in_a_replayed_graph(cuda):
+    B, S, E = 3, 2000, 32
+    r, dgate = routing(cuda, 8, B, S, E)
+    loss, counts, kept, sums, d = outputs(cuda, B, S, E)
+    ln, dg = torch.tensor([2000, 700, 1], dtype=torch.int32, device=cuda), dgate.to(cuda)
+
+    def step():
+        ops.balance_loss_fwd(r, loss, counts, kept, sums, lengths=ln)
+        ops.balance_loss_bwd(r, counts, d, dgate=dg, lengths=ln)
+    step()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (loss, counts, kept, sums, d)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    assert all(torch.equal(t, w) for t, w in zip((loss, counts, kept, sums, d), want))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for i in range(4):
+        for t in (loss, counts, kept, sums, d):
+            t.fill_(3)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, w) for t, w in zip((loss, counts, kept, sums, d), want)), i
+        r["probs"].sum().item()
+
+
+def test_refused_calls(cuda):
+    r, dgate = routing(cuda, 1, 2, 8, 4)
+    loss, counts, kept, sums, d = outputs(cuda, 2, 8, 4)
+    f = lambda **kw: ops.balance_loss_fwd(**{**dict(r=r, loss=loss, counts=counts, kept=kept, prob_sum=sums), **kw})  # noqa: E731
+    f()
+    for kw, err in ((dict(counts=sums), TypeError), (dict(prob_sum=counts), TypeError), (dict(loss=sums), TypeError), (dict(kept=counts), ValueError),
+                    (dict(choices=3), ops._lib.HapmiError), (dict(lengths=torch.zeros(2, device=cuda)), TypeError),
+                    (dict(lengths=torch.zeros(3, dtype=torch.int32, device=cuda)), TypeError), (dict(r=dict(r, slot=r["slot"].long())), TypeError),
+                    (dict(r=dict(r, index=r["index"][:1])), ops._lib.HapmiError)):
+        with pytest.raises(err):
+            f(**kw)
+    with pytest.raises(ValueError):
+        ops.balance_loss_bwd(r, counts, r["probs"])
+    with pytest.raises(ops._lib.HapmiError):
+        ops.balance_loss_bwd(r, counts, d, dgate=dgate[:, :4].to(cuda).contiguous())

@@ -1,0 +1,153 @@
+"""Calls that the entry points of the relative position bias, the per-head norm with rotation and the balance loss refuse
+on the host, before any device is touched (the pointers below are never followed)."""
+import ctypes
+
+import pytest
+
+from hap_amd._lib import BF16, F32, HapmiError, RelBias, _load
+from hap_amd import ops
+
+P = 0x10000                                                   # 16-byte aligned, never dereferenced
+EINVAL, EALIGN, ELIMIT = -1, -2, -5
+
+
+def bias(starts=(0, 1, 2, 4), n=None, two=0, ld=8, table=P):
+    arr = (ctypes.c_int32 * len(starts))(*starts)
+    r = RelBias()
+    r.table, r.ld, r.n_buckets, r.bidirectional, r.starts_host = table, ld, n if n is not None else len(starts) * (2 if two else 1), two, ctypes.addressof(arr)
+    r._keep = arr
+    return r
+
+
+def refused(rc, code, text):
+    msg = _load().hapmi_last_error().decode()
+    assert rc == code and text in msg, (rc, msg)
+
+
+def rel_fwd(r=None, qkv=P, out=P, lse=P, b=2, S=16, H=4, scale=0.125, keep=None, p=0.0):
+    r = bias() if r is None else r
+    return _load().hapmi_attention_relbias_fwd(qkv, ctypes.byref(r), 0, None, out, lse, b, S, H, scale, keep, p, None)
+
+
+def rel_bwd(r=None, b=2, S=16, H=4, ws=P, elems=1 << 30, ldd=8, kr=None, kc=None, dtable=P, dqkv=P):
+    r = bias() if r is None else r
+    return _load().hapmi_attention_relbias_bwd(P, ctypes.byref(r), 0, None, P, P, P, dqkv, dtable, ldd, 0, P, ws, elems, b, S, H, 0.125, kr, kc, 0.0, None)
+
+
+def test_relative_bias_descriptions():
+    refused(rel_fwd(bias(n=1)), EINVAL, "at least 2")
+    refused(rel_fwd(bias(n=7, two=1)), EINVAL, "even")
+    refused(rel_fwd(bias(starts=tuple(range(65)))), ELIMIT, "at most 64")
+    refused(rel_fwd(bias(starts=(1, 2, 3, 4))), EINVAL, "distance 0")
+    refused(rel_fwd(bias(starts=(0, 3, 2, 4))), EINVAL, "must not fall")
+    refused(rel_fwd(bias(starts=(0, 1, 2, 1025))), ELIMIT, "1025")
+    refused(rel_fwd(bias(ld=3)), EINVAL, "heads")
+    refused(rel_fwd(bias(table=None)), EINVAL, "null pointer")
+    r = bias()
+    r.starts_host = None
+    refused(rel_fwd(r), EINVAL, "null bias")
+    assert _load().hapmi_attention_relbias_fwd(P, None, 0, None, P, P, 2, 16, 4, 0.125, None, 0.0, None) == EINVAL
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(b=-1), EINVAL, "bad shape"), (dict(S=0), EINVAL, "bad shape"), (dict(H=0), EINVAL, "bad shape"),
+    (dict(S=1 << 24), ELIMIT, "too long"), (dict(b=20000, H=4), ELIMIT, "65535"), (dict(b=1 << 62, H=4), ELIMIT, "65535"),
+    (dict(scale=0.0), EINVAL, "positive"), (dict(scale=-1.0), EINVAL, "positive"), (dict(scale=float("nan")), EINVAL, "positive"),
+    (dict(scale=float("inf")), EINVAL, "positive"), (dict(p=1.0, keep=P), EINVAL, "[0, 1)"), (dict(p=-0.1, keep=P), EINVAL, "[0, 1)"),
+    (dict(qkv=None), EINVAL, "null"), (dict(out=None), EINVAL, "null"), (dict(lse=None), EINVAL, "null"),
+    (dict(qkv=P + 8), EALIGN, "16-byte"), (dict(out=P + 2), EALIGN, "16-byte"), (dict(keep=P + 4), EALIGN, "keep words"),
+    (dict(lse=P + 2), EALIGN, "aligned")])
+def test_relative_bias_forward(kw, code, text):
+    refused(rel_fwd(**kw), code, text)
+
+
+def test_relative_bias_forward_of_an_empty_batch_does_nothing():
+    assert rel_fwd(b=0) == 0
+
+
+def test_relative_bias_backward():
+    need = ctypes.c_int64()
+    r = bias()
+    assert _load().hapmi_attention_relbias_workspace_elems(ctypes.byref(r), 2, 300, 4, ctypes.byref(need)) == 0
+    assert need.value > 0 and need.value % (2 * 4 * 3) == 0
+    refused(rel_bwd(S=300, elems=need.value - 1), ELIMIT, "workspace")
+    refused(rel_bwd(ws=None), EINVAL, "null")
+    refused(rel_bwd(dtable=None), EINVAL, "null")
+    refused(rel_bwd(b=0), EINVAL, "empty batch")
+    refused(rel_bwd(ldd=3), EINVAL, "gradient rows")
+    refused(rel_bwd(kr=P), EINVAL, "come together")
+    refused(rel_bwd(kc=P), EINVAL, "come together")
+    refused(rel_bwd(dqkv=P + 4), EALIGN, "16-byte")
+    refused(_load().hapmi_attention_relbias_workspace_elems(ctypes.byref(r), 2, 300, 4, None), EINVAL, "null")
+
+
+def qn_fwd(qkv=P, out=P, qg=P, kg=P, ang=P, n_pos=64, rot=64, inter=0, pos=None, b=2, S=16, H=4, D=64, eps=1e-6, dt=BF16):
+    return _load().hapmi_qk_norm_rotary_fwd(qkv, out, qg, kg, ang, n_pos, rot, inter, pos, b, S, H, D, eps, dt, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(D=0), EINVAL, "bad"), (dict(D=60), EALIGN, "multiple of 8"), (dict(D=66, dt=F32), EALIGN, "multiple of 4"), (dict(D=264), ELIMIT, "256"),
+    (dict(rot=72), EALIGN, "rot"), (dict(rot=24), EALIGN, "rot"), (dict(rot=12, inter=1), EALIGN, "rot"), (dict(rot=0), EINVAL, "come together"),
+    (dict(ang=None), EINVAL, "come together"), (dict(n_pos=0, pos=P), EINVAL, "empty"), (dict(n_pos=15), EINVAL, "sequences of 16"),
+    (dict(eps=-1.0), EINVAL, "bad"), (dict(eps=float("nan")), EINVAL, "bad"), (dict(dt=7), EINVAL, "bad"), (dict(S=0), EINVAL, "bad"),
+    (dict(b=1 << 30, S=1 << 20, n_pos=1 << 21), ELIMIT, "2^40"), (dict(ang=P + 4), EALIGN, "16-byte"), (dict(pos=P + 2), EALIGN, "aligned"),
+    (dict(qkv=P + 8), EALIGN, "16-byte"), (dict(out=P + 8), EALIGN, "16-byte"), (dict(qkv=None), EINVAL, "null"), (dict(out=None), EINVAL, "null")])
+def test_norm_and_rotation_forward(kw, code, text):
+    refused(qn_fwd(**kw), code, text)
+
+
+def test_norm_and_rotation_backward():
+    L = _load()
+    need = ctypes.c_int64()
+    assert L.hapmi_qk_norm_rotary_workspace_elems(64, ctypes.byref(need)) == 0 and need.value >= 2 * 64
+    refused(L.hapmi_qk_norm_rotary_workspace_elems(257, ctypes.byref(need)), EINVAL, "bad")
+
+    def bwd(dout=P, dqg=P, ws=P, elems=1 << 40, b=2):
+        return L.hapmi_qk_norm_rotary_bwd(dout, P, P, P, P, dqg, None, 0, P, 64, 64, 0, None, b, 16, 4, 64, 1e-6, BF16, ws, elems, None)
+    refused(bwd(elems=2 * 64 - 1), ELIMIT, "workspace")
+    refused(bwd(ws=None), ELIMIT, "workspace")
+    refused(bwd(dout=None), EINVAL, "null")
+    refused(bwd(b=0), EINVAL, "empty batch")
+    refused(bwd(dqg=P + 2), EALIGN, "aligned")
+    assert qn_fwd(b=0) == 0
+
+
+def test_balance_loss():
+    L = _load()
+
+    def fwd(probs=P, B=4, S=8192, E=8, choices=1, ws=P, elems=1 << 40, loss=P):
+        return L.hapmi_balance_loss_fwd(probs, P, P, None, loss, P, P, P, B, S, E, 0.01, choices, ws, elems, None)
+
+    def bwd(probs=P, index=P, dgate=None, B=4, E=8, choices=1, dlogits=P):
+        return L.hapmi_balance_loss_bwd(probs, index, P, dgate, P, None, dlogits, B, 16, E, 0.01, choices, None)
+    for call in (fwd, bwd):
+        refused(call(E=65), ELIMIT, "64 experts")
+        refused(call(E=0), EINVAL, "bad")
+        refused(call(choices=3), EINVAL, "bad")
+        refused(call(choices=0), EINVAL, "bad")
+        refused(call(B=65536), ELIMIT, "65535 rows")
+        refused(call(probs=P + 4), EALIGN, "16-byte")
+        refused(call(probs=None), EINVAL, "null")
+    refused(fwd(B=0), EINVAL, "empty batch")
+    refused(fwd(S=1 << 24), ELIMIT, "tokens a row")
+    refused(fwd(ws=None), ELIMIT, "workspace")
+    refused(fwd(elems=10), ELIMIT, "workspace")
+    refused(bwd(dgate=P, index=None), EINVAL, "null")
+    refused(bwd(dlogits=P + 8), EALIGN, "16-byte")
+    assert bwd(B=0) == 0
+    need = ctypes.c_int64()
+    assert L.hapmi_balance_workspace_elems(60000, 16, 8, ctypes.byref(need)) == 0 and need.value == 0     # whole rows: none needed
+    refused(L.hapmi_balance_workspace_elems(4, 16, 8, None), EINVAL, "null")
+
+
+def test_cpu_tensors_are_refused():
+    import torch
+    t = torch.zeros(1, 4, 192, dtype=torch.bfloat16)
+    with pytest.raises(HapmiError, match="GPU tensors only"):
+        ops.qk_norm_rotary_fwd(t, t, 1, 4, 1)
+    with pytest.raises(HapmiError, match="GPU tensors only"):
+        ops.attention_relbias_fwd(t, torch.zeros(4, 1), t, t, 1, 4, 1, 0.125)
+    with pytest.raises(ValueError):
+        ops.rotary_table(0, 8)
+    with pytest.raises(ValueError):
+        ops.rotary_table(8, 7)
