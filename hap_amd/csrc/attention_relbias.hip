@@ -13,10 +13,14 @@
 // one key column in dK / dV; consecutive registers are consecutive keys / queries, so a lane's window reads are runs of
 // four consecutive words and the 32 columns of a half wave read 32 consecutive addresses).
 //
-// dT: ds_ij is summed along the diagonals j - i of a 32 x 32 score block by LDS float additions into a window-long array of
-// the wave AND lane half: within one instruction a half wave's 32 columns go to 32 different words, a wave's LDS operations
-// complete in order and nobody else adds to that array, so the result is the same bits every time.  The eight arrays are
-// added in order at the block's end, the blocks' windows and the buckets' ranges by a second kernel, in order.
+// dT: ds_ij is summed along the diagonals j - i of a 32 x 32 score block in registers: the 63 diagonals fit the 64 lanes, the
+// rows of the block are added one after the other to a vector that moves up by one lane between two rows (a DPP wave
+// shift that rides on the addition), so that lane l always holds the diagonal (row) - l.  A row's 32 columns have to lie in
+// lanes 0 .. 31 with zeros above: the swap of half waves delivers that for the two rows of an accumulator register at
+// once.  That is 4 vector instructions a register, and no atomics: LDS float additions of the 16 registers cost 180 cycles
+// each on this chip (the dQ kernel of [12, 512] x 16 heads took 274 us with them).  The vector is added to the wave's own
+// window in LDS; the block adds its four windows and sums the buckets' ranges, a second kernel adds the blocks, all in a
+// fixed order: the same bits every time.
 #include "common.h"
 #include "attention_tile.h"
 
@@ -42,6 +46,18 @@ struct RelArgs {
         for (int i = 1; i < side; ++i) k += d >= starts[i] ? 1 : 0;
         return k + (bidir && rel > 0 ? side : 0);
     }
+    // relative positions lo .. hi of the window that belong to bucket u (none: lo > hi)
+    __device__ __forceinline__ void range(int u, int &lo, int &hi) const {
+        int first = 0, next = R + MARGIN + 1;                 // distances of the bucket: first .. next - 1
+        const int k = bidir && u >= side ? u - side : u;
+        for (int i = 0; i < side; ++i) {                      // (starts[] is indexed by the loop only: scalar loads)
+            if (i == k) first = starts[i];
+            if (i == k + 1) next = starts[i];
+        }
+        if (bidir && u >= side) { lo = first < 1 ? 1 : first; hi = next - 1; }
+        else { lo = -(next - 1); hi = first == 0 ? (bidir || next < 1 ? 0 : R + MARGIN) : -first; }
+        if (first >= next) { lo = 1; hi = 0; }
+    }
     // the head's bias / scale over the window; REV: entry i belongs to relative position -(i - R - MARGIN)
     template <bool REV> __device__ __forceinline__ void expand(float *win, int head, float scale) const {
         for (int i = threadIdx.x; i < window(); i += AT_THREADS) {
@@ -66,6 +82,31 @@ __device__ __forceinline__ f32x16 bias_tile(const float *w) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[g * 4 + e] = w[g * 8 + e];
     return a;
+}
+
+// sums of a 32 x 32 block along its diagonals: lane l gets the sum over (row, column) with row - column = 31 - l
+__device__ __forceinline__ float diagonal_sums(const f32x16 &x) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    float y = 0.f;
+    auto step = [&](uint32_t row) {                           // one more row: up by one lane, zero into lane 0
+        const int up = __builtin_amdgcn_update_dpp(0, __float_as_int(y), 0x138, 0xf, 0xf, true);   // wave_shr:1
+        y = __int_as_float(up) + __uint_as_float(row);
+    };
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        u32x2 rows[4];                                        // .x: row 8 g + e, .y: row 8 g + 4 + e, in lanes 0 .. 31
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[g * 4 + e]), 0u, false, false);
+            rows[e].x = r[0];
+            rows[e].y = r[1];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) step(rows[e].x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) step(rows[e].y);
+    }
+    return y;
 }
 
 __device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) {
@@ -215,7 +256,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
                                                                   float keep_scale) {
     __shared__ __attribute__((aligned(16))) char Ks[TILE_BYTES];
     __shared__ __attribute__((aligned(16))) char Vs[TILE_BYTES];
-    extern __shared__ float win[];                            // the bias window, then the eight windows of ds sums
+    extern __shared__ float win[];                            // the bias window, then the four waves' windows of ds sums
     const TransposedReader tr;
     const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
@@ -230,8 +271,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
     const bf16_t *dO = dout + (int64_t)b * S * E + hh * HD;
     const int q_blk_end = blk * 128 + 128;
     const int kv_end = blk * 128 >= n ? 0 : ((CAUSAL && q_blk_end < n) ? q_blk_end : n);
-    float *sums = win + W, *own = sums + (wave * 2 + h) * W;
-    for (int i = threadIdx.x; i < 8 * W; i += AT_THREADS) sums[i] = 0.f;
+    float *sums = win + W, *own = sums + wave * W;
+    for (int i = threadIdx.x; i < 4 * W; i += AT_THREADS) sums[i] = 0.f;
     f32x16 dqt[2] = {zero16(), zero16()};
     if (kv_end > 0) {
         rel.expand<false>(win, hh, scale);                    // both published by the loop's first barrier
@@ -298,9 +339,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl)) * (dp[r] - delta_q);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    __hip_atomic_fetch_add(own + at - 4 * h + acc_row(r, h), dp[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
+                own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
 #pragma unroll
                 for (int sp = 0; sp < 2; ++sp) {
                     const frag_t db = acc_to_b(dp, sp);
@@ -322,38 +362,41 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
                 *(bf16x4 *)(drow + u * 32 + g * 8 + h * 4) = o;
             }
     }
+    // the block's bucket sums: window words over the four waves, then every bucket's range by a group of eight lanes
     __syncthreads();
-    float *mine = part + ((int64_t)bh * ((S + 127) / 128) + blk) * W;
-    for (int i = threadIdx.x; i < W; i += AT_THREADS) {
+    for (int i = threadIdx.x; i < W; i += AT_THREADS) win[i] = ((sums[i] + sums[W + i]) + sums[2 * W + i]) + sums[3 * W + i];
+    __syncthreads();
+    const int n_buckets = rel.side << rel.bidir;
+    float *mine = part + ((int64_t)bh * ((S + 127) / 128) + blk) * n_buckets;
+    for (int u = threadIdx.x >> 3; u < n_buckets; u += AT_THREADS / 8) {
+        int lo, hi;
+        rel.range(u, lo, hi);
         float v = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v += sums[k * W + i];
-        mine[i] = v;
+        for (int r = lo + (threadIdx.x & 7); r <= hi; r += 8) v += win[r + rel.R + MARGIN];
+        v += __shfl_xor(v, 1, 64);
+        v += __shfl_xor(v, 2, 64);
+        v += __shfl_xor(v, 4, 64);
+        if ((threadIdx.x & 7) == 0) mine[u] = v;
     }
 }
 
-// dT[u, h] (+)= the blocks' windows [b * H][row blocks][W], added over b and row block in order, then over the relative
-// positions of bucket u in order.  One block per head: the windows are short next to the scores they come from.
-__global__ __launch_bounds__(1024) void relbias_dtable_kernel(const RelArgs rel, const float *part, float *dtable, int64_t ldd,
-                                                            int n_buckets, int b, int H, int row_blocks, int accumulate) {
-    extern __shared__ float tot[];
-    const int W = rel.window(), h = blockIdx.x;
-    for (int i = threadIdx.x; i < W; i += 1024) {
+// dT[u, h] (+)= the blocks' sums part[b][H][row blocks][buckets], in order.  One block per head; 1024 / buckets threads share
+// a bucket, each over a run of blocks, their sums added in order.
+__global__ __launch_bounds__(1024) void relbias_dtable_kernel(const float *part, float *dtable, int64_t ldd, int n_buckets, int b, int H,
+                                                            int row_blocks, int accumulate) {
+    __shared__ float red[1024];
+    const int h = blockIdx.x, u = threadIdx.x % n_buckets, run = threadIdx.x / n_buckets, runs = 1024 / n_buckets;
+    const int64_t items = (int64_t)b * row_blocks;
+    if (run < runs) {
         float v = 0.f;
-        for (int z = 0; z < b; ++z) {
-            const float *p = part + ((int64_t)z * H + h) * row_blocks * W + i;
-            for (int k = 0; k < row_blocks; ++k) v += p[(int64_t)k * W];
-        }
-        tot[i] = v;
+#pragma unroll 4
+        for (int64_t i = run; i < items; i += runs) v += part[(((i / row_blocks) * H + h) * row_blocks + i % row_blocks) * n_buckets + u];
+        red[threadIdx.x] = v;
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < n_buckets; u += 1024) {
+    if (run == 0) {
         float v = 0.f;
-        for (int i = 0; i < W; ++i) {
-            int r = i - rel.R - MARGIN;
-            r = r < -rel.R ? -rel.R : (r > rel.R ? rel.R : r);
-            if (rel.bucket(r) == u) v += tot[i];
-        }
+        for (int i = 0; i < runs; ++i) v += red[i * n_buckets + u];
         float *d = dtable + (int64_t)u * ldd + h;
         *d = accumulate ? *d + v : v;
     }
@@ -563,7 +606,7 @@ extern "C" int hapmi_attention_relbias_workspace_elems(const hapmi_relbias *bias
     if (!rc) rc = check_rel(name, bias_host, H, &a);
     if (rc) return rc;
     HAPMI_REQUIRE(elems_host, HAPMI_EINVAL, "%s: null pointer", name);
-    *elems_host = b * H * hapmi_cdiv(S, 128) * window_of(a.R);
+    *elems_host = b * H * hapmi_cdiv(S, 128) * bias_host->n_buckets;
     return HAPMI_OK;
 }
 
@@ -587,14 +630,14 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
     HAPMI_REQUIRE(ld_dtable >= H, HAPMI_EINVAL, "%s: gradient rows of %lld for %lld heads", name, (long long)ld_dtable, (long long)H);
     const int W = window_of(a.R);
     const int64_t row_blocks = hapmi_cdiv(S, 128);
-    HAPMI_REQUIRE(workspace_elems >= b * H * row_blocks * W, HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name,
-                  (long long)workspace_elems, (long long)(b * H * row_blocks * W));
+    const int64_t need = b * H * row_blocks * bias_host->n_buckets;
+    HAPMI_REQUIRE(workspace_elems >= need, HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name, (long long)workspace_elems, (long long)need);
     const bool drop = keep_rows != nullptr;
     const float ks = drop ? 1.0f / (1.0f - p) : 1.0f;
     hipStream_t st = (hipStream_t)stream;
     dim3 grid((unsigned)row_blocks, (unsigned)(b * H)), block(AT_THREADS);
     auto dq = [&](auto kernel) -> int {
-        const size_t lds = (size_t)W * 4 * 9;
+        const size_t lds = (size_t)W * 4 * 5;
         rc = allow_lds(name, kernel, lds);
         if (rc) return rc;
         hipLaunchKernelGGL(kernel, grid, block, lds, st, a, (const bf16_t *)qkv, (const bf16_t *)out, (const bf16_t *)dout, lse, delta_ws,
@@ -611,7 +654,7 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
     if (causal) rc = drop ? dq(relbias_bwd_dq_kernel<true, true>) : dq(relbias_bwd_dq_kernel<true, false>);
     else rc = drop ? dq(relbias_bwd_dq_kernel<false, true>) : dq(relbias_bwd_dq_kernel<false, false>);
     if (rc) return rc;
-    hipLaunchKernelGGL(relbias_dtable_kernel, dim3((unsigned)H), dim3(1024), (size_t)W * 4, st, a, (const float *)workspace, dtable, ld_dtable,
+    hipLaunchKernelGGL(relbias_dtable_kernel, dim3((unsigned)H), dim3(1024), 0, st, (const float *)workspace, dtable, ld_dtable,
                        bias_host->n_buckets, (int)b, (int)H, (int)row_blocks, accumulate);
     HAPMI_CHECK_LAUNCH(name);
     if (causal) return drop ? dkv(relbias_bwd_dkv_kernel<true, true>) : dkv(relbias_bwd_dkv_kernel<true, false>);

@@ -70,6 +70,69 @@ def _span(rows: int, cols: int, ld: int) -> int:
     return 0 if rows <= 0 or cols <= 0 else (rows - 1) * ld + cols
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _operands(what, *specs):
+    """Checks of a call's tensors in one pass over ``specs`` = (name, tensor or None, element type, elements that the kernel
+    touches, written): on the current device, of the type, contiguous, long enough, and nothing that is written shares
+    memory with another operand.  Returns the current stream and the pointers (0 for None), in order."""
+    cur, ptrs, spans = -2, [], []
+    for name, t, dtype, elems, written in specs:
+        if t is None:
+            ptrs.append(0)
+            continue
+        if t.get_device() != cur:
+            _dev(t)
+            if cur >= 0 or t.get_device() != torch.cuda.current_device():
+                raise _lib.HapmiError(f"{what}: {name} is on {t.device}, not on the current device")
+            cur = t.get_device()
+        if t.dtype is not dtype:
+            raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+        n = t.numel()
+        if elems < 0 or elems > n or not t.is_contiguous():
+            _need(t, elems, f"{what} {name}")
+        ptr = t.data_ptr()
+        ptrs.append(ptr)
+        if n:
+            spans.append((ptr, ptr + n * t.element_size(), written))
+    _apart(what, spans)
+    return _raw_stream(cur), ptrs
+
+
+def _exactly(what, n, *tensors):
+    for t in tensors:
+        if t is not None and t.numel() != n:
+            raise TypeError(f"{what}: {n} elements expected in place of {t.numel()}")
+
+
+def _apart(what, spans):
+    spans.sort()
+    end_any = end_written = 0
+    for lo, hi, written in spans:
+        if lo < end_written or (written and lo < end_any):
+            raise ValueError(f"{what}: an output shares memory with another operand")
+        end_any = max(end_any, hi)
+        if written:
+            end_written = max(end_written, hi)
+
+
+def _scratch(what, workspace, elems: int, device):
+    """Float32 scratch of ``elems`` elements: the caller's, or one of this call's own."""
+    if workspace is None:
+        return torch.empty(elems, dtype=torch.float32, device=device)
+    if workspace.dtype != torch.float32:
+        raise TypeError(f"{what}: float32 workspace expected")
+    return workspace
+
+
+def _kept(ptr, owner):
+    """A pointer argument that keeps ``owner`` alive: a recorded launch list then replays with memory that is still there."""
+    ptr = ctypes.c_void_p(ptr)
+    ptr._keep = owner
+    return ptr
+
+
 # ---------------------------------------------------------------------------
 # layout helpers: a tensor sharded on `dim` is [outer, len, inner]
 # ---------------------------------------------------------------------------
@@ -784,20 +847,15 @@ def rotary_table(n_positions: int, rot: int, base: float = 10000.0, device=None)
     return torch.stack([angle.cos(), angle.sin()], -1).float().contiguous()
 
 
-def _qk_norm_args(what, qkv, b, S, H, q_gain, k_gain, rotary, positions):
-    """(head dimension, table positions, rotated dimensions) after the checks that both directions share."""
-    dtype_code(qkv)
+def _head_dim(what, qkv, b, S, H, rotary):
+    """Head dimension of the packed projection, and (positions, rotated dimensions) of the angle table."""
     if b < 0 or S < 1 or H < 1 or qkv.dim() != 3 or qkv.shape[0] != b or qkv.shape[1] != S or qkv.shape[2] % (3 * H):
         raise ValueError(f"{what}: a packed projection [b, S, 3 * H * head_dim] expected")
-    D = qkv.shape[2] // (3 * H)
-    for g in (q_gain, k_gain):
-        if g is not None and (g.dtype != torch.float32 or g.numel() != D or not g.is_contiguous()):
-            raise TypeError(f"{what}: gains must be {D} contiguous float32")
-    if rotary is not None and (rotary.dtype != torch.float32 or rotary.dim() != 3 or rotary.shape[2] != 2 or not rotary.is_contiguous()):
-        raise TypeError(f"{what}: the angle table must be a contiguous float32 [positions, rot / 2, 2] tensor")
-    if positions is not None and (positions.dtype != torch.int32 or positions.numel() != b * S or not positions.is_contiguous()):
-        raise TypeError(f"{what}: positions must be b * S contiguous int32")
-    return D, (rotary.shape[0] if rotary is not None else 0), (2 * rotary.shape[1] if rotary is not None else 0)
+    if rotary is None:
+        return qkv.shape[2] // (3 * H), 0, 0
+    if rotary.dim() != 3 or rotary.shape[2] != 2:
+        raise TypeError(f"{what}: the angle table must be a float32 [positions, rot / 2, 2] tensor")
+    return qkv.shape[2] // (3 * H), rotary.shape[0], 2 * rotary.shape[1]
 
 
 def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None, positions=None, interleaved=False, eps=1e-6):
@@ -806,17 +864,17 @@ def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None,
     None: norm only), values copied; ``out`` may be ``qkv`` itself (in place).  ``positions``: int32 [b, S] (None: the index
     inside the sequence); one outside the table gives NaN.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
     what = "qk_norm_rotary_fwd"
-    _here(what, qkv, out, q_gain, k_gain, rotary, positions)
-    D, n_pos, rot = _qk_norm_args(what, qkv, b, S, H, q_gain, k_gain, rotary, positions)
-    if out.dtype != qkv.dtype:
-        raise TypeError(f"{what}: dtype mismatch")
-    _need(qkv, qkv.numel(), f"{what} qkv")
-    _need(out, qkv.numel(), f"{what} out")
-    if out.data_ptr() != qkv.data_ptr():
-        _no_overlap(what, (out, qkv))
-    _no_overlap(what, *[(out, t) for t in (q_gain, k_gain, rotary, positions)])
-    check(lib().hapmi_qk_norm_rotary_fwd(_ptr(qkv), _ptr(out), _ptr(q_gain), _ptr(k_gain), _ptr(rotary), n_pos, rot, int(interleaved),
-                                         _ptr(positions), b, S, H, D, ctypes.c_float(eps), dtype_code(qkv), _stream()))
+    D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
+    _exactly(what, D, q_gain, k_gain)
+    _exactly(what, b * S, positions)
+    code, n = dtype_code(qkv), b * S * 3 * H * D
+    if out.numel() != n:
+        raise ValueError(f"{what}: out must have qkv's size")
+    apart = out.data_ptr() != qkv.data_ptr()
+    stream, (o_, x_, q_, k_, r_, p_) = _operands(
+        what, ("out", out, qkv.dtype, n, True), ("qkv", qkv if apart else None, qkv.dtype, n, False), ("q_gain", q_gain, torch.float32, D, False),
+        ("k_gain", k_gain, torch.float32, D, False), ("rotary", rotary, torch.float32, n_pos * rot, False), ("positions", positions, torch.int32, b * S, False))
+    check(lib().hapmi_qk_norm_rotary_fwd(x_ if apart else o_, o_, q_, k_, r_, n_pos, rot, interleaved, p_, b, S, H, D, eps, code, stream))
 
 
 def qk_norm_rotary_workspace_elems(D: int) -> int:
@@ -831,25 +889,26 @@ def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_ga
     """Backward of ``qk_norm_rotary_fwd``: ``dqkv`` from ``dout`` (``dqkv`` may be ``dout``: in place) and forward's input
     ``qkv``; ``dq_gain`` / ``dk_gain`` float32 [head_dim] (None: not wanted; ``accumulate``: added to)."""
     what = "qk_norm_rotary_bwd"
-    _here(what, dout, qkv, dqkv, q_gain, k_gain, dq_gain, dk_gain, rotary, positions, workspace)
-    D, n_pos, rot = _qk_norm_args(what, qkv, b, S, H, q_gain, k_gain, rotary, positions)
-    if dout.dtype != qkv.dtype or dqkv.dtype != qkv.dtype:
-        raise TypeError(f"{what}: dtype mismatch")
-    for t in (qkv, dout, dqkv):
-        _need(t, qkv.numel(), what)
-    for g in (dq_gain, dk_gain):
-        if g is not None and (g.dtype != torch.float32 or g.numel() != D or not g.is_contiguous()):
-            raise TypeError(f"{what}: gain gradients must be {D} contiguous float32")
-    if dqkv.data_ptr() != dout.data_ptr():
-        _no_overlap(what, (dqkv, dout))
-    _no_overlap(what, *[(w, t) for w in (dqkv, dq_gain, dk_gain) for t in (qkv, q_gain, k_gain, rotary, positions)], (dq_gain, dk_gain),
-                (dqkv, dq_gain), (dqkv, dk_gain))
-    ws, ws_elems = None, 0
+    D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
+    _exactly(what, D, q_gain, k_gain, dq_gain, dk_gain)
+    _exactly(what, b * S, positions)
+    code, n, ws_elems = dtype_code(qkv), b * S * 3 * H * D, 0
+    _exactly(what, n, dout, dqkv)
     if dq_gain is not None or dk_gain is not None:
-        ws, ws_elems = _scratch(what, workspace, qk_norm_rotary_workspace_elems(D), qkv.device)
-    check(lib().hapmi_qk_norm_rotary_bwd(_ptr(dout), _ptr(qkv), _ptr(dqkv), _ptr(q_gain), _ptr(k_gain), _ptr(dq_gain), _ptr(dk_gain),
-                                         int(accumulate), _ptr(rotary), n_pos, rot, int(interleaved), _ptr(positions), b, S, H, D,
-                                         ctypes.c_float(eps), dtype_code(qkv), ws, ws_elems, _stream()))
+        ws_elems = qk_norm_rotary_workspace_elems(D)
+        workspace = _scratch(what, workspace, ws_elems, qkv.device)
+    else:
+        workspace = None
+    apart = dqkv.data_ptr() != dout.data_ptr()
+    stream, (dx_, do_, x_, q_, k_, dq_, dk_, r_, p_, ws_) = _operands(
+        what, ("dqkv", dqkv, qkv.dtype, n, True), ("dout", dout if apart else None, qkv.dtype, n, False), ("qkv", qkv, qkv.dtype, n, False),
+        ("q_gain", q_gain, torch.float32, D, False), ("k_gain", k_gain, torch.float32, D, False), ("dq_gain", dq_gain, torch.float32, D, True),
+        ("dk_gain", dk_gain, torch.float32, D, True), ("rotary", rotary, torch.float32, n_pos * rot, False),
+        ("positions", positions, torch.int32, b * S, False), ("workspace", workspace, torch.float32, ws_elems, True))
+    if not apart and dout.dtype is not qkv.dtype:
+        raise TypeError(f"{what}: dtype mismatch")
+    check(lib().hapmi_qk_norm_rotary_bwd(do_ if apart else dx_, x_, dx_, q_, k_, dq_, dk_, accumulate, r_, n_pos, rot, interleaved, p_, b, S, H, D,
+                                         eps, code, _kept(ws_, workspace), workspace.numel() if workspace is not None else 0, stream))
 
 
 def softmax_fwd(x, mask, p, rows, width, ld, mask_rows=1):
@@ -942,15 +1001,6 @@ def attention_bwd(qkv, out, dout, lse, mask, dqkv, delta_ws, b, S, H, scale, cau
                                             _ptr(keep_rows), _ptr(keep_cols), ctypes.c_float(p), _stream()))
 
 
-def _here(what, *tensors):
-    """The kernels run on the current device's current stream: every operand has to live there."""
-    _dev(*tensors)
-    cur = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != cur:
-            raise _lib.HapmiError(f"{what}: a tensor on {t.device} while cuda:{cur} is the current device")
-
-
 @functools.lru_cache(maxsize=None)
 def relative_bucket_starts(n_buckets: int, max_distance: int, bidirectional: bool = True):
     """First distance of every bucket of one side of a relative position bias with ``n_buckets`` buckets (two sides share
@@ -989,43 +1039,20 @@ def _bucket_array(n_buckets, max_distance, bidirectional):
 
 
 def _relbias(what, table, H, max_distance, bidirectional, causal):
-    if table.dim() != 2 or table.shape[1] != H or table.dtype != torch.float32 or (table.shape[1] > 1 and table.stride(1) != 1):
+    """The bias description of the C ABI; ``table`` may be the columns of a wider one."""
+    if table.dim() != 2 or table.shape[1] != H or table.dtype != torch.float32 or (H > 1 and table.stride(1) != 1):
         raise ValueError(f"{what}: the table must be a float32 [buckets, {H}] tensor with unit column stride")
+    n = table.shape[0]
     bidirectional = (not causal) if bidirectional is None else bool(bidirectional)
-    arr = _bucket_array(int(table.shape[0]), int(max_distance), bidirectional)
-    a = _lib.RelBias()
-    a.table = table.data_ptr()
-    a.ld = max(table.stride(0), H)
-    a.n_buckets, a.bidirectional = table.shape[0], int(bidirectional)
-    a.starts_host = ctypes.addressof(arr)
+    arr = _bucket_array(n, int(max_distance), bidirectional)
+    a = _lib.RelBias(table.data_ptr(), max(table.stride(0), H), n, bidirectional, ctypes.addressof(arr))
     a._keep = arr
     return a
 
 
-def _check_lengths(what, lengths, b):
-    if lengths is not None and (lengths.dtype != torch.int32 or lengths.numel() != b or not lengths.is_contiguous()):
-        raise TypeError(f"{what}: lengths must be {b} contiguous int32")
-
-
-def _no_overlap(what, *pairs):
-    """Every pair (written, other) must lie in separate memory."""
-    end = lambda t: t.data_ptr() + (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
-    for w, o in pairs:
-        if w is not None and o is not None and w.numel() and o.numel() and w.data_ptr() < end(o) and o.data_ptr() < end(w):
-            raise ValueError(f"{what}: an output shares memory with another operand")
-
-
-def _scratch(what, workspace, elems: int, device):
-    """Pointer to float32 scratch of ``elems`` elements: the caller's, or one of this call's own (which the pointer object
-    keeps, so that a recorded launch list replays with memory that is still there)."""
-    if workspace is None:
-        workspace = torch.empty(elems, dtype=torch.float32, device=device)
-    if workspace.dtype != torch.float32:
-        raise TypeError(f"{what}: float32 workspace expected")
-    _need(workspace, elems, f"{what} workspace")
-    ptr = _ptr(workspace)
-    ptr._keep = workspace
-    return ptr, workspace.numel()
+def _rows_span(t):
+    """Address range of a 2-d tensor of float32 rows that may be strided."""
+    return t.data_ptr(), t.data_ptr() + 4 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])
 
 
 def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128, bidirectional=None, causal=False,
@@ -1033,18 +1060,25 @@ def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128
     """``attention_fwd`` with a learned relative position bias: scores scale * q_i k_j + table[bucket(j - i), head],
     ``table`` float32 [buckets, H] (rows may be strided: the columns of a device's heads).  Buckets as
     ``relative_bucket_starts(buckets, max_distance, bidirectional)`` cuts the distances; ``bidirectional`` None: two sides
-    unless ``causal``.  ``lengths`` (int32 [b]): the sequences of a padded batch; rows behind a sequence's end get zeros and
-    lse = -inf, its keys there are not read.  ``keep_rows`` / ``p``: dropout of the probabilities."""
+    unless ``causal``.  An entry at or below -1e30 hides its bucket's pairs.  ``lengths`` (int32 [b]): the sequences of a padded
+    batch; rows behind a sequence's end get zeros and lse = -inf, its keys there are not read.  ``keep_rows`` / ``p``:
+    dropout of the probabilities, as in ``attention_fwd``."""
     what = "attention_relbias_fwd"
-    _here(what, qkv, table, out, lse, lengths, keep_rows)
-    _check_attn(qkv, out, lse, None, b, S, H)
-    _check_lengths(what, lengths, b)
-    _no_overlap(what, (out, qkv), (lse, qkv), (lse, out), (lse, table), (out, table))
+    _exactly(what, b, lengths)
+    E = H * 64
+    stream, (q_, o_, l_, n_, k_) = _operands(
+        what, ("qkv", qkv, torch.bfloat16, b * S * 3 * E, False), ("out", out, torch.bfloat16, b * S * E, True),
+        ("lse", lse, torch.float32, b * H * S, True), ("lengths", lengths, torch.int32, b, False),
+        ("keep_rows", keep_rows, torch.int32, attention_keep_words(b, S, H) if keep_rows is not None else 0, False))
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
-    if keep_rows is not None:
-        _check_keep(keep_rows, b, S, H, "keep_rows")
-    check(lib().hapmi_attention_relbias_fwd(_ptr(qkv), ctypes.byref(rel), int(causal), _ptr(lengths), _ptr(out), _ptr(lse),
-                                            b, S, H, ctypes.c_float(scale), _ptr(keep_rows), ctypes.c_float(p), _stream()))
+    _on_device(what, table, qkv)
+    check(lib().hapmi_attention_relbias_fwd(q_, ctypes.byref(rel), causal, n_, o_, l_, b, S, H, scale, k_, p, stream))
+
+
+def _on_device(what, t, like):
+    if t.get_device() != like.get_device():
+        _dev(t)
+        raise _lib.HapmiError(f"{what}: tensors on {t.device} and {like.device}")
 
 
 def attention_relbias_workspace_elems(table, b, S, H, max_distance=128, bidirectional=None, causal=False) -> int:
@@ -1062,30 +1096,27 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     ``accumulate``: added to, for a table that several layers share).  ``out`` and ``lse`` as forward left them.
     ``workspace``: float32 scratch of ``attention_relbias_workspace_elems`` (None: taken from torch's allocator)."""
     what = "attention_relbias_bwd"
-    _here(what, qkv, table, out, dout, lse, dqkv, dtable, delta_ws, lengths, keep_rows, keep_cols, workspace)
-    _check_attn(qkv, out, lse, None, b, S, H)
-    _check_lengths(what, lengths, b)
-    _need(dout, b * S * H * 64, "attention dout")
-    _need(dqkv, b * S * 3 * H * 64, "attention dqkv")
-    _need(delta_ws, b * H * S, "attention delta")
-    if dout.dtype != torch.bfloat16 or dqkv.dtype != torch.bfloat16 or delta_ws.dtype != torch.float32:
-        raise TypeError(f"{what}: dtype mismatch")
+    _exactly(what, b, lengths)
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
     if dtable.shape != table.shape or dtable.dtype != torch.float32 or (H > 1 and dtable.stride(1) != 1):
         raise ValueError(f"{what}: dtable must be float32 of the table's shape with unit column stride")
-    _no_overlap(what, *[(w, o) for w in (dqkv, delta_ws) for o in (qkv, out, dout, lse, table)], (dqkv, delta_ws))
     if (keep_rows is None) != (keep_cols is None):
         raise ValueError(f"{what}: keep_rows and keep_cols come together")
-    if keep_rows is not None:
-        _check_keep(keep_rows, b, S, H, "keep_rows")
-        _check_keep(keep_cols, b, S, H, "keep_cols")
+    _on_device(what, table, qkv)
+    _on_device(what, dtable, qkv)
+    _apart(what, [(*_rows_span(table), False), (*_rows_span(dtable), True)])
     need = ctypes.c_int64()
     check(_lib._load().hapmi_attention_relbias_workspace_elems(ctypes.byref(rel), b, S, H, ctypes.byref(need)))
-    ws, ws_elems = _scratch(what, workspace, need.value, qkv.device)
-    check(lib().hapmi_attention_relbias_bwd(
-        _ptr(qkv), ctypes.byref(rel), int(causal), _ptr(lengths), _ptr(out), _ptr(dout), _ptr(lse), _ptr(dqkv), _ptr(dtable),
-        max(dtable.stride(0), H), int(accumulate), _ptr(delta_ws), ws, ws_elems, b, S, H,
-        ctypes.c_float(scale), _ptr(keep_rows), _ptr(keep_cols), ctypes.c_float(p), _stream()))
+    workspace = _scratch(what, workspace, need.value, qkv.device)
+    E, words = H * 64, attention_keep_words(b, S, H) if keep_rows is not None else 0
+    stream, (q_, o_, do_, l_, dq_, dl_, n_, kr_, kc_, ws_) = _operands(
+        what, ("qkv", qkv, torch.bfloat16, b * S * 3 * E, False), ("out", out, torch.bfloat16, b * S * E, False),
+        ("dout", dout, torch.bfloat16, b * S * E, False), ("lse", lse, torch.float32, b * H * S, False),
+        ("dqkv", dqkv, torch.bfloat16, b * S * 3 * E, True), ("delta_ws", delta_ws, torch.float32, b * H * S, True),
+        ("lengths", lengths, torch.int32, b, False), ("keep_rows", keep_rows, torch.int32, words, False),
+        ("keep_cols", keep_cols, torch.int32, words, False), ("workspace", workspace, torch.float32, need.value, True))
+    check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), max(dtable.stride(0), H), accumulate,
+                                            dl_, _kept(ws_, workspace), workspace.numel(), b, S, H, scale, kr_, kc_, p, stream))
 
 
 def head_parallel_attention(x, w_in, b_in, w_out, num_heads, mask=None):
@@ -1453,17 +1484,12 @@ def top2_gate_bwd(r, dgate, dlogits):
                                     B, S, E, _stream()))
 
 
-def _check_balance(what, r, E, lengths, B, S):
-    _check_routing(r, B, S, E)
-    _here(what, *r.values(), lengths)
-    if r["probs"].dtype != torch.float32:
-        raise TypeError(f"{what}: float32 probabilities expected")
-    _check_lengths(what, lengths, B)
-
-
-def _check_counts(what, t, B, E, dtype):
-    if t.dtype != dtype or t.numel() != B * E or not t.is_contiguous():
-        raise TypeError(f"{what}: counts are contiguous int32 [B, E], probability sums float32 [B, E]")
+def _balance_shape(what, r, lengths):
+    if r["probs"].dim() != 3:
+        raise ValueError(f"{what}: probabilities [B, S, E] expected")
+    B, S, E = r["probs"].shape
+    _exactly(what, B, lengths)
+    return B, S, E
 
 
 def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, lengths=None, workspace=None):
@@ -1473,38 +1499,32 @@ def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, leng
     loss = coef * E * mean over the rows of sum_e counts / (choices * n) * prob_sum / n, n the row's tokens: all S, or
     ``lengths`` (int32 [B]) of a padded batch (empty rows do not enter the mean).  Perfectly even routing gives coef."""
     what = "balance_loss_fwd"
-    B, S, E = r["probs"].shape
-    _check_balance(what, r, E, lengths, B, S)
-    _here(what, loss, counts, kept, prob_sum, workspace)
-    if loss.dtype != torch.float32 or loss.numel() != 1:
-        raise TypeError(f"{what}: the loss is one float32")
-    _check_counts(what, counts, B, E, torch.int32)
-    _check_counts(what, kept, B, E, torch.int32)
-    _check_counts(what, prob_sum, B, E, torch.float32)
-    outs = (loss, counts, kept, prob_sum)
-    _no_overlap(what, *[(w, t) for w in outs for t in (*r.values(), lengths)], *[(a, c) for i, a in enumerate(outs) for c in outs[:i]])
+    B, S, E = _balance_shape(what, r, lengths)
+    _exactly(what, 1, loss)
+    _exactly(what, B * E, counts, kept, prob_sum)
     need = ctypes.c_int64()
     check(_lib._load().hapmi_balance_workspace_elems(B, S, E, ctypes.byref(need)))
-    ws, ws_elems = _scratch(what, workspace, need.value, loss.device) if need.value else (None, 0)
-    check(lib().hapmi_balance_loss_fwd(_ptr(r["probs"]), _ptr(r["index"]), _ptr(r["slot"]), _ptr(lengths), _ptr(loss), _ptr(counts), _ptr(kept),
-                                       _ptr(prob_sum), B, S, E, ctypes.c_float(coef), int(choices), ws, ws_elems, _stream()))
+    workspace = _scratch(what, workspace, need.value, loss.device) if need.value else None
+    stream, (p_, i_, s_, n_, l_, c_, k_, ps_, ws_) = _operands(
+        what, ("probs", r["probs"], torch.float32, B * S * E, False), ("index", r["index"], torch.int32, B * S * 2, False),
+        ("slot", r["slot"], torch.int32, B * S * 2, False), ("lengths", lengths, torch.int32, B, False), ("loss", loss, torch.float32, 1, True),
+        ("counts", counts, torch.int32, B * E, True), ("kept", kept, torch.int32, B * E, True), ("prob_sum", prob_sum, torch.float32, B * E, True),
+        ("workspace", workspace, torch.float32, need.value, True))
+    check(lib().hapmi_balance_loss_fwd(p_, i_, s_, n_, l_, c_, k_, ps_, B, S, E, coef, choices, _kept(ws_, workspace),
+                                       workspace.numel() if workspace is not None else 0, stream))
 
 
 def balance_loss_bwd(r, counts, dlogits, choices=2, coef=0.01, grad=1.0, dgate=None, lengths=None):
     """Gradient of ``grad`` times the balance loss with respect to the router's logits, from forward's ``counts``; with
     ``dgate`` (float32 [B, S, 2]) ``dlogits`` also holds what ``top2_gate_bwd`` gives for it, in the same pass."""
     what = "balance_loss_bwd"
-    B, S, E = r["probs"].shape
-    _check_balance(what, r, E, lengths, B, S)
-    _here(what, counts, dlogits, dgate)
-    _check_counts(what, counts, B, E, torch.int32)
-    _need(dlogits, B * S * E, f"{what} dlogits")
-    _need(dgate, B * S * 2, f"{what} dgate")
-    if dlogits.dtype != torch.float32 or (dgate is not None and dgate.dtype != torch.float32):
-        raise TypeError(f"{what}: float32 expected")
-    _no_overlap(what, *[(dlogits, t) for t in (*r.values(), counts, dgate, lengths)])
-    check(lib().hapmi_balance_loss_bwd(_ptr(r["probs"]), _ptr(r["index"]), _ptr(r["slot"]), _ptr(dgate), _ptr(counts), _ptr(lengths), _ptr(dlogits),
-                                       B, S, E, ctypes.c_float(float(coef) * float(grad)), int(choices), _stream()))
+    B, S, E = _balance_shape(what, r, lengths)
+    _exactly(what, B * E, counts)
+    stream, (p_, i_, s_, g_, c_, n_, d_) = _operands(
+        what, ("probs", r["probs"], torch.float32, B * S * E, False), ("index", r["index"], torch.int32, B * S * 2, False),
+        ("slot", r["slot"], torch.int32, B * S * 2, False), ("dgate", dgate, torch.float32, B * S * 2, False),
+        ("counts", counts, torch.int32, B * E, False), ("lengths", lengths, torch.int32, B, False), ("dlogits", dlogits, torch.float32, B * S * E, True))
+    check(lib().hapmi_balance_loss_bwd(p_, i_, s_, g_, c_, n_, d_, B, S, E, coef * grad, choices, stream))
 
 
 def top2_densify(r, E, C):
