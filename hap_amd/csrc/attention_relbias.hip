@@ -38,12 +38,15 @@ struct RelArgs {
     const float *table;                       // [buckets, ld], column = head
     int64_t ld;
     int side, bidir, R;                       // buckets per side; R: first distance of the last bucket, >= 1
-    int starts[REL_MAX_SIDE];                 // first distance of every bucket of a side, starts[0] = 0
+    int starts[REL_MAX_SIDE];                 // first distance of every bucket of a side, starts[0] = 0; then INT32_MAX
     __device__ __forceinline__ int window() const { return 2 * R + 1 + 2 * MARGIN; }
     __device__ __forceinline__ int bucket(int rel) const {
         const int d = bidir ? (rel < 0 ? -rel : rel) : (rel < 0 ? -rel : 0);
-        int k = 0;
-        for (int i = 1; i < side; ++i) k += d >= starts[i] ? 1 : 0;
+        int k = -1;
+        for (int i = 0; i < side; i += 16) {                  // sixteen at a time: one wait for the scalar loads
+#pragma unroll
+            for (int j = 0; j < 16; ++j) k += d >= starts[i + j] ? 1 : 0;
+        }
         return k + (bidir && rel > 0 ? side : 0);
     }
     // relative positions lo .. hi of the window that belong to bucket u (none: lo > hi)
@@ -109,6 +112,11 @@ __device__ __forceinline__ float diagonal_sums(const f32x16 &x) {
     return y;
 }
 
+__device__ __forceinline__ float both_halves_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 __device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) {
     if (!lengths) return S;
     const int n = lengths[b];
@@ -128,10 +136,11 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
     __shared__ __attribute__((aligned(16))) uint32_t keep_s[DROP ? NST : 1][AT_THREADS];
     extern __shared__ float win[];
     const TransposedReader tr;
+    const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
     const int blk = BlockOrder<CAUSAL>::row_block(true), bh = BlockOrder<CAUSAL>::batch_head();
     const int b = bh / H, hh = bh % H;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int n = row_length(lengths, b, S);
     const int qw = blk * 128 + wave * 32, q = qw + c;
     const bf16_t *Q = qkv + (int64_t)b * S * ld + hh * HD;
@@ -142,10 +151,6 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
     f32x16 ot[2] = {zero16(), zero16()};
     float m = -INFINITY, lsum = 0.f;                          // running maximum in units of log 2
     if (kv_end > 0) {
-        frag_t qf[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) qf[s] = load_row_frag(Q + (int64_t)q * ld, q < n, s, h);
-        rel.expand<false>(win, hh, scale);                    // published by the first barrier of the loop
         const DirectTileLoader ldr(ld);
         const float sl2 = scale * LOG2E;
         constexpr int PER_TILE = 2 * DirectTileLoader::LOADS + (DROP ? 1 : 0);
@@ -159,6 +164,10 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
         };
         issue_tile(0, 0);
         if (TILE < kv_end) issue_tile(TILE, 1);
+        frag_t qf[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) qf[s] = load_row_frag(Q + (int64_t)q * ld, q < n, s, h);
+        rel.expand<false>(win, hh, scale);                    // published by the first barrier of the loop
         // consumed before the loop, so that the wait for these loads is not one for all transfers in every iteration
 #pragma unroll
         for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(qf[s].v));
@@ -169,38 +178,69 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
             __syncthreads();
             if (kv0 + 2 * TILE < kv_end) issue_tile(kv0 + 2 * TILE, buf == 0 ? 2 : buf - 1);
             const char *Ks = Ks3[buf], *Vs = Vs3[buf];
+            buf = buf == NST - 1 ? 0 : buf + 1;
+            if (CAUSAL && kv0 > qw + 31) continue;            // the wave's queries see none of the tile's keys
             uint32_t keep = 0xffffffffu;
-            if constexpr (DROP) keep = keep_s[buf][threadIdx.x];
-            const float *w = win + rel.at<64>(kv0 - qw, c, h);
-            f32x16 st[2] = {bias_tile(w), bias_tile(w + 32)};
+            if constexpr (DROP) keep = keep_s[buf == 0 ? NST - 1 : buf - 1][threadIdx.x];
+            const bool whole = kv0 + TILE <= n && !(CAUSAL && kv0 + TILE - 1 > qw);
+            const bool far_hi = kv0 - qw - 31 >= rel.R, far_lo = kv0 - qw + 63 <= -rel.R;
+            // all fragment reads of a group are issued before its first MFMA waits for one, and those of V before the
+            // softmax arithmetic, which hides them
+            frag_t kf[2][4], vf[2][4];
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) st[t] = mma(frag_rowk(Ks, t * 32 + c, s, h), qf[s], st[t]);
-            if (kv0 + TILE > n || (CAUSAL && kv0 + TILE - 1 > qw)) {
+                for (int t = 0; t < 2; ++t) kf[t][s] = frag_rowk(Ks, t * 32 + c, s, h);
+            f32x16 st[2];
+            float shift = 0.f;                                // bias of a tile beyond the window, in units of log 2
+            if (whole && (far_hi || far_lo)) {
+                shift = win[far_hi ? W - 1 : 0] * sl2;
+                __builtin_amdgcn_sched_barrier(0);
+                st[0] = zero16();
+                st[1] = zero16();
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int s = 0; s < 4; ++s)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int kv = kv0 + t * 32 + acc_row(r, h);
-                        if (kv >= n || (CAUSAL && kv > q)) st[t][r] = -INFINITY;
-                    }
+                    for (int t = 0; t < 2; ++t) st[t] = mma(kf[t][s], qf[s], st[t]);
+            } else {
+                const float *w = win + rel.at<64>(kv0 - qw, c, h);
+                st[0] = bias_tile(w);
+                st[1] = bias_tile(w + 32);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) st[t] = mma(kf[t][s], qf[s], st[t]);
+                if (!whole) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int kv = kv0 + t * 32 + acc_row(r, h);
+                            if (kv >= n || (CAUSAL && kv > q)) st[t][r] = -INFINITY;
+                        }
+                }
             }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) vf[u][s] = tr.frag(Vs, u * 32, s);
+            __builtin_amdgcn_sched_barrier(0);
             float mx = st[0][0];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[t][r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float m_new = fmaxf(m, mx * sl2);
-            const float msub = m_new == -INFINITY ? 0.f : m_new;
+            mx = both_halves_max(mx);
+            const float m_new = fmaxf(m, fmaf(mx, sl2, shift));
+            const float msub = m_new == -INFINITY ? 0.f : m_new, off = shift - msub;
             const float alpha = __builtin_amdgcn_exp2f(m - msub);
             float psum = 0.f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(st[t][r], sl2, -msub));
+                    const float p = __builtin_amdgcn_exp2f(fmaf(st[t][r], sl2, off));
                     st[t][r] = p;
                     psum += p;
                 }
@@ -222,9 +262,8 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
             for (int s = 0; s < 4; ++s) {
                 const frag_t pb = acc_to_b(st[s >> 1], s & 1);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) ot[u] = mma(tr.frag(Vs, u * 32, s), pb, ot[u]);
+                for (int u = 0; u < 2; ++u) ot[u] = mma(vf[u][s], pb, ot[u]);
             }
-            buf = buf == NST - 1 ? 0 : buf + 1;
         }
     }
     const float l = lsum + __shfl_xor(lsum, 32, 64);
@@ -254,15 +293,15 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
                                                                   bf16_t *dqkv, float *part, const int32_t *lengths, int S,
                                                                   int H, float scale, const uint32_t *keep_rows,
                                                                   float keep_scale) {
-    __shared__ __attribute__((aligned(16))) char Ks[TILE_BYTES];
-    __shared__ __attribute__((aligned(16))) char Vs[TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char Ks2[2][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char Vs2[2][TILE_BYTES];
     extern __shared__ float win[];                            // the bias window, then the four waves' windows of ds sums
     const TransposedReader tr;
     const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
     const int blk = BlockOrder<CAUSAL>::row_block(true), bh = BlockOrder<CAUSAL>::batch_head();
     const int b = bh / H, hh = bh % H;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int n = row_length(lengths, b, S);
     const int qw = blk * 128 + wave * 32, q = qw + c;
     const bool qok = q < n;
@@ -274,8 +313,11 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
     float *sums = win + W, *own = sums + wave * W;
     for (int i = threadIdx.x; i < 4 * W; i += AT_THREADS) sums[i] = 0.f;
     f32x16 dqt[2] = {zero16(), zero16()};
+    float far_sum[2] = {0.f, 0.f};                            // blocks wholly before / behind the window
     if (kv_end > 0) {
-        rel.expand<false>(win, hh, scale);                    // both published by the loop's first barrier
+        const DirectTileLoader ldr(ld);
+        ldr.issue(K, n, Ks2[0]);
+        ldr.issue(V, n, Vs2[0]);
         frag_t qf[4], dof[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -295,60 +337,93 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
             delta_q += __shfl_xor(delta_q, 32, 64);
             if (qok && h == 0) delta[((int64_t)b * H + hh) * S + q] = delta_q;
         }
-        PairLoader lk(ld), lv(ld);
+        rel.expand<false>(win, hh, scale);                    // this and the zeroed sums: published by the loop's first barrier
         // ds is kept without its factor `scale`; a query that sees nothing (lse = -inf) has p = 0
         const float sl2 = scale * LOG2E, nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
-        lk.load(K, n);
-        lv.load(V, n);
         const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * ((S + TILE - 1) / TILE) * 2 + h : nullptr;
         uint32_t keep = 0xffffffffu, keep_next = 0xffffffffu;
         if constexpr (DROP) keep_next = keep_row[0];
+        int buf = 0;
         for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
-            __syncthreads();
-            lk.store_rows(Ks);
-            lv.store_rows(Vs);
+            __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the tile has landed
+            __syncthreads();                                  // for everybody, and everybody is done with the other buffer
             if constexpr (DROP) keep = keep_next;
-            __syncthreads();
             if (kv0 + TILE < kv_end) {
                 const int nx = kv0 + TILE;
-                lk.load(K + (int64_t)nx * ld, n - nx);
-                lv.load(V + (int64_t)nx * ld, n - nx);
+                ldr.issue(K + (int64_t)nx * ld, n - nx, Ks2[buf ^ 1]);
+                ldr.issue(V + (int64_t)nx * ld, n - nx, Vs2[buf ^ 1]);
                 if constexpr (DROP) keep_next = keep_row[(nx / TILE) * 2];
             }
-            if (qw >= n) continue;                            // a wave without queries only moves tiles and meets barriers
+            const char *Ks = Ks2[buf], *Vs = Vs2[buf];
+            buf ^= 1;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                if (t == 1 && kv0 + 32 >= n) break;
-                const int at = rel.at<32>(kv0 + t * 32 - qw, c, h);
-                f32x16 st = bias_tile(win + at), dp = zero16();
+                const int k0 = kv0 + t * 32, D = k0 - qw;
+                if (qw >= n || k0 >= n || (CAUSAL && D > 31)) continue;        // nothing here that any query sees
+                const bool whole = k0 + 32 <= n && !(CAUSAL && D > -31);
+                const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;
+                f32x16 st, dp = zero16();
+                frag_t kf[4], vf[4], kt[2][2];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    st = mma(frag_rowk(Ks, t * 32 + c, s, h), qf[s], st);
-                    dp = mma(frag_rowk(Vs, t * 32 + c, s, h), dof[s], dp);
+                    kf[s] = frag_rowk(Ks, t * 32 + c, s, h);
+                    vf[s] = frag_rowk(Vs, t * 32 + c, s, h);
                 }
-                if constexpr (DROP) {
+                auto products = [&]() {                       // every group of reads is issued before the arithmetic that hides it
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f;
-                }
-                if (kv0 + t * 32 + 32 > n || (CAUSAL && kv0 + t * 32 + 31 > qw)) {
+                    for (int s = 0; s < 4; ++s) {
+                        st = mma(kf[s], qf[s], st);
+                        dp = mma(vf[s], dof[s], dp);
+                    }
+#pragma unroll
+                    for (int sp = 0; sp < 2; ++sp)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) kt[sp][u] = tr.frag(Ks, u * 32, t * 2 + sp);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (DROP) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f;
+                    }
+                };
+                if (whole && (far_hi || far_lo)) {            // one bucket for the whole block
+                    st = zero16();
+                    products();
+                    const float off = nl + win[far_hi ? W - 1 : 0] * sl2;
+                    float sum = 0.f;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int kv = kv0 + t * 32 + acc_row(r, h);
-                        if (kv >= n || (CAUSAL && kv > q)) st[r] = -INFINITY;
+                        dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, off)) * (dp[r] - delta_q);
+                        sum += dp[r];
                     }
-                }
+                    far_sum[far_hi ? 1 : 0] += sum;
+                } else {
+                    const int at = rel.at<32>(D, c, h);
+                    st = bias_tile(win + at);
+                    products();
+                    if (!whole) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl)) * (dp[r] - delta_q);
-                // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
-                own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
+                        for (int r = 0; r < 16; ++r) {
+                            const int kv = k0 + acc_row(r, h);
+                            if (kv >= n || (CAUSAL && kv > q)) st[r] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl)) * (dp[r] - delta_q);
+                    // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
+                    own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
+                }
 #pragma unroll
                 for (int sp = 0; sp < 2; ++sp) {
                     const frag_t db = acc_to_b(dp, sp);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) dqt[u] = mma(tr.frag(Ks, u * 32, t * 2 + sp), db, dqt[u]);
+                    for (int u = 0; u < 2; ++u) dqt[u] = mma(kt[sp][u], db, dqt[u]);
                 }
             }
         }
+        const float lo = wave_sum(far_sum[0]), hi = wave_sum(far_sum[1]);
+        if (lane == 0) own[0] += lo;
+        if (lane == 0) own[W - 1] += hi;
     }
     if (q < S) {
         bf16_t *drow = dqkv + ((int64_t)b * S + q) * ld + hh * HD;
@@ -410,15 +485,16 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
                                                                    const float *lse, const float *delta, bf16_t *dqkv,
                                                                    const int32_t *lengths, int S, int H, float scale,
                                                                    const uint32_t *keep_cols, float keep_scale) {
-    __shared__ __attribute__((aligned(16))) char Qs[TILE_BYTES];
-    __shared__ __attribute__((aligned(16))) char dOs[TILE_BYTES];
-    __shared__ __attribute__((aligned(16))) float lse_s[TILE], delta_s[TILE];
+    __shared__ __attribute__((aligned(16))) char Qs2[2][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char dOs2[2][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) float lse_s[2][3][TILE], delta_s[2][TILE];
     extern __shared__ float win[];
     const TransposedReader tr;
+    const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
     const int blk = BlockOrder<CAUSAL>::row_block(false), bh = BlockOrder<CAUSAL>::batch_head();
     const int b = bh / H, hh = bh % H;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int n = row_length(lengths, b, S);
     const int kvw = blk * 128 + wave * 32, kv = kvw + c;
     const bool kok = kv < n;
@@ -428,64 +504,104 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
     const float *lse_b = lse + ((int64_t)b * H + hh) * S, *delta_b = delta + ((int64_t)b * H + hh) * S;
     f32x16 dvt[2] = {zero16(), zero16()}, dkt[2] = {zero16(), zero16()};
     if (blk * 128 < n) {
-        rel.expand<true>(win, hh, scale);
         frag_t kf[4], vf[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             kf[s] = load_row_frag(K + (int64_t)kv * ld, kok, s, h);
             vf[s] = load_row_frag(V + (int64_t)kv * ld, kok, s, h);
         }
-        PairLoader lq(ld), ldo(E);
+        const DirectTileLoader lq(ld), ldo(E);
         const float sl2 = scale * LOG2E;
         const int q_begin = CAUSAL ? blk * 128 : 0;           // causal: earlier queries see none of the block's keys
-        lq.load(Q + (int64_t)q_begin * ld, n - q_begin);
-        ldo.load(dO + (int64_t)q_begin * E, n - q_begin);
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
         const u32x2 *keep_col = DROP ? (const u32x2 *)(keep_cols + ((int64_t)bh * S + (kv < S ? kv : S - 1)) * (2 * ((S + TILE - 1) / TILE))) : nullptr;
         u32x2 keep2 = {0xffffffffu, 0xffffffffu}, keep2_next = keep2;
-        if constexpr (DROP) keep2_next = keep_col[q_begin / TILE];
-        for (int q0 = q_begin; q0 < n; q0 += TILE) {
-            __syncthreads();
-            lq.store_rows(Qs);
-            ldo.store_rows(dOs);
-            if constexpr (DROP) keep2 = keep2_next;
+        // a query's log-sum-exp (times log2 e; of one that sees nothing +inf: p = 0) and the same less the bias before and
+        // behind the window, so that a far block needs neither a bias nor an addition a score; and its delta
+        float l_next = 0.f, d_next = 0.f;
+        auto fetch = [&](int q0, int bufi) {
+            lq.issue(Q + (int64_t)q0 * ld, n - q0, Qs2[bufi]);
+            ldo.issue(dO + (int64_t)q0 * E, n - q0, dOs2[bufi]);
+            if constexpr (DROP) keep2_next = keep_col[q0 / TILE];
             if (threadIdx.x < TILE) {
                 const int qq = q0 + threadIdx.x;
-                const float l = qq < n ? lse_b[qq] : -INFINITY;
-                lse_s[threadIdx.x] = l == -INFINITY ? INFINITY : l * LOG2E;        // a query that sees nothing: p = 0
-                delta_s[threadIdx.x] = qq < n ? delta_b[qq] : 0.f;
+                l_next = qq < n ? lse_b[qq] : -INFINITY;
+                d_next = qq < n ? delta_b[qq] : 0.f;
             }
-            __syncthreads();
-            if (q0 + TILE < n) {
-                const int nx = q0 + TILE;
-                lq.load(Q + (int64_t)nx * ld, n - nx);
-                ldo.load(dO + (int64_t)nx * E, n - nx);
-                if constexpr (DROP) keep2_next = keep_col[nx / TILE];
+        };
+        auto stage = [&](int bufi) {
+            if (threadIdx.x < TILE) {
+                const float l = l_next == -INFINITY ? INFINITY : l_next * LOG2E;
+                lse_s[bufi][0][threadIdx.x] = l;
+                lse_s[bufi][1][threadIdx.x] = l - win[W - 1] * sl2;           // (the window here runs over query - key)
+                lse_s[bufi][2][threadIdx.x] = l - win[0] * sl2;
+                delta_s[bufi][threadIdx.x] = d_next;
             }
-            if (kvw >= n) continue;                           // a wave without keys only moves tiles and meets barriers
+        };
+        fetch(q_begin, 0);
+        rel.expand<true>(win, hh, scale);
+        __syncthreads();                                      // the window is there
+        stage(0);
+        int buf = 0;
+        for (int q0 = q_begin; q0 < n; q0 += TILE) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the tile has landed
+            __syncthreads();                                  // for everybody, and everybody is done with the other buffer
+            if constexpr (DROP) keep2 = keep2_next;
+            const bool more = q0 + TILE < n;
+            if (more) fetch(q0 + TILE, buf ^ 1);
+            const char *Qs = Qs2[buf], *dOs = dOs2[buf];
 #pragma unroll 1
             for (int t = 0; t < 2; ++t) {
-                if (t == 1 && q0 + 32 >= n) break;
-                f32x16 sc = bias_tile(win + rel.at<32>(q0 + t * 32 - kvw, c, h)), dp = zero16();
+                const int r0 = q0 + t * 32, D = r0 - kvw;
+                if (kvw >= n || r0 >= n || (CAUSAL && D < -31)) continue;      // nothing here that sees any of the wave's keys
+                const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;         // queries behind / before the keys
+                f32x16 sc, dp = zero16();
+                frag_t qa[4], da[4];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    sc = mma(frag_rowk(Qs, t * 32 + c, s, h), kf[s], sc);
-                    dp = mma(frag_rowk(dOs, t * 32 + c, s, h), vf[s], dp);
+                    qa[s] = frag_rowk(Qs, t * 32 + c, s, h);
+                    da[s] = frag_rowk(dOs, t * 32 + c, s, h);
                 }
+                auto products = [&]() {                       // every group of reads is issued before the arithmetic that hides it
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        sc = mma(qa[s], kf[s], sc);
+                        dp = mma(da[s], vf[s], dp);
+                    }
+                };
+                const float *lse_t = lse_s[buf][0];
+                if (far_hi || far_lo) {
+                    lse_t = lse_s[buf][far_hi ? 1 : 2];
+                    sc = zero16();
+                    products();
+                } else {
+                    sc = bias_tile(win + rel.at<32>(D, c, h));
+                    products();
+                    if (CAUSAL && D < 31) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (kv > r0 + acc_row(r, h)) sc[r] = -INFINITY;
+                    }
+                }
+                frag_t qt[2][2], dt[2][2];
+#pragma unroll
+                for (int sp = 0; sp < 2; ++sp)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        dt[sp][u] = tr.frag(dOs, u * 32, t * 2 + sp);
+                        qt[sp][u] = tr.frag(Qs, u * 32, t * 2 + sp);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
                 const uint32_t keep = t ? keep2.y : keep2.x;
                 if constexpr (DROP) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << acc_row(r, h))) ? dp[r] * keep_scale : 0.f;
                 }
-                if (CAUSAL && kvw + 31 > q0 + t * 32) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (kv > q0 + t * 32 + acc_row(r, h)) sc[r] = -INFINITY;
-                }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int ql = t * 32 + g * 8 + h * 4;
-                    const f32x4 l4 = *(const f32x4 *)(lse_s + ql), d4 = *(const f32x4 *)(delta_s + ql);
+                    const f32x4 l4 = *(const f32x4 *)(lse_t + ql), d4 = *(const f32x4 *)(delta_s[buf] + ql);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = g * 4 + e;
@@ -503,11 +619,13 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
                     const frag_t pb = acc_to_b(sc, sp), db = acc_to_b(dp, sp);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        dvt[u] = mma(tr.frag(dOs, u * 32, t * 2 + sp), pb, dvt[u]);
-                        dkt[u] = mma(tr.frag(Qs, u * 32, t * 2 + sp), db, dkt[u]);
+                        dvt[u] = mma(dt[sp][u], pb, dvt[u]);
+                        dkt[u] = mma(qt[sp][u], db, dkt[u]);
                     }
                 }
             }
+            if (more) stage(buf ^ 1);
+            buf ^= 1;
         }
     }
     if (kv < S) {
@@ -545,6 +663,7 @@ int check_rel(const char *name, const hapmi_relbias *r, int64_t H, RelArgs *a) {
         a->starts[i] = r->starts_host[i];
         HAPMI_REQUIRE(i == 0 || a->starts[i] >= a->starts[i - 1], HAPMI_EINVAL, "%s: the buckets' first distances must not fall", name);
     }
+    for (int i = a->side; i < REL_MAX_SIDE; ++i) a->starts[i] = INT32_MAX;
     const int last = a->starts[a->side - 1];
     HAPMI_REQUIRE(last <= REL_MAX_REACH, HAPMI_ELIMIT, "%s: the last bucket starts at distance %d, at most %d", name, last, REL_MAX_REACH);
     a->bidir = r->bidirectional ? 1 : 0;
