@@ -61,19 +61,51 @@ struct RelArgs {
         else { lo = -(next - 1); hi = first == 0 ? (bidir || next < 1 ? 0 : R + MARGIN) : -first; }
         if (first >= next) { lo = 1; hi = 0; }
     }
-    // the head's bias / scale over the window; REV: entry i belongs to relative position -(i - R - MARGIN)
-    template <bool REV> __device__ __forceinline__ void expand(float *win, int head, float scale) const {
+    // the head's bias / scale over the window; REV: entry i belongs to relative position -(i - R - MARGIN); CAUSAL: keys behind
+    // the query are hidden
+    template <bool REV, bool CAUSAL> __device__ __forceinline__ void expand(float *win, int head, float scale) const {
         for (int i = threadIdx.x; i < window(); i += AT_THREADS) {
             int rel = i - R - MARGIN;
             rel = rel < -R ? -R : (rel > R ? R : rel);
-            const float t = table[(int64_t)bucket(REV ? -rel : rel) * ld + head];
-            win[i] = t <= HIDDEN ? -INFINITY : t / scale;
+            if (REV) rel = -rel;
+            const float t = table[(int64_t)bucket(rel) * ld + head];
+            win[i] = t <= HIDDEN || (CAUSAL && rel > 0) ? -INFINITY : t / scale;
         }
     }
     // word of the window that the lane's row 0 of a block of ROWS x 32 scores reads; D = first row - first column
     template <int ROWS> __device__ __forceinline__ int at(int D, int c, int h) const {
         D = D < -R - (ROWS - 1) ? -R - (ROWS - 1) : (D > R + 31 ? R + 31 : D);
         return D + R + MARGIN + 4 * h - c;
+    }
+};
+
+// A [64 rows][64 d] tile global -> LDS like DirectTileLoader's, for the many tiles of a kernel that lie wholly inside the
+// operand: the lane's byte offsets inside a tile never change, the tile's first row is a scalar base, and a transfer costs no
+// vector arithmetic.  A tile that ends inside repeats the operand's last row.
+struct TileStream {
+    static constexpr int LOADS = 2;
+    int off[LOADS], ld;
+    __device__ __forceinline__ static int row(int i) { return (i * 4 + (int)(threadIdx.x >> 6)) * 8 + (int)((threadIdx.x & 63) >> 3); }
+    __device__ __forceinline__ static int chunk(int i) { return (((int)threadIdx.x & 7) ^ aswz(row(i))) * 16; }
+    __device__ __forceinline__ TileStream(int ld_) : ld(ld_) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) off[i] = row(i) * ld * 2 + chunk(i);
+    }
+    __device__ __forceinline__ void issue(const bf16_t *base, int rows_left, char *lds_tile) const {
+        typedef __attribute__((address_space(3))) char lds_char;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char *)lds_tile + wave * 1024;
+        int o[LOADS] = {off[0], off[1]};
+        if (rows_left < TILE) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) o[i] = (row(i) < rows_left ? row(i) : rows_left - 1) * ld * 2 + chunk(i);
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                         :
+                         : "s"(lds_addr + i * 4096), "v"(o[i]), "s"(base)
+                         : "memory");
     }
 };
 
@@ -151,10 +183,10 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
     f32x16 ot[2] = {zero16(), zero16()};
     float m = -INFINITY, lsum = 0.f;                          // running maximum in units of log 2
     if (kv_end > 0) {
-        const DirectTileLoader ldr(ld);
+        const TileStream ldr(ld);
         const float sl2 = scale * LOG2E;
-        constexpr int PER_TILE = 2 * DirectTileLoader::LOADS + (DROP ? 1 : 0);
-        static_assert(2 * DirectTileLoader::LOADS == 4, "the waits below are written for four (five) transfers per tile");
+        constexpr int PER_TILE = 2 * TileStream::LOADS + (DROP ? 1 : 0);
+        static_assert(2 * TileStream::LOADS == 4, "the waits below are written for four (five) transfers per tile");
         const int n_kt = (S + TILE - 1) / TILE;
         const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * n_kt * 2 + h : nullptr;
         auto issue_tile = [&](int kv0, int bufi) {
@@ -167,7 +199,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
         frag_t qf[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) qf[s] = load_row_frag(Q + (int64_t)q * ld, q < n, s, h);
-        rel.expand<false>(win, hh, scale);                    // published by the first barrier of the loop
+        rel.expand<false, CAUSAL>(win, hh, scale);                    // published by the first barrier of the loop
         // consumed before the loop, so that the wait for these loads is not one for all transfers in every iteration
 #pragma unroll
         for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(qf[s].v));
@@ -182,7 +214,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
             if (CAUSAL && kv0 > qw + 31) continue;            // the wave's queries see none of the tile's keys
             uint32_t keep = 0xffffffffu;
             if constexpr (DROP) keep = keep_s[buf == 0 ? NST - 1 : buf - 1][threadIdx.x];
-            const bool whole = kv0 + TILE <= n && !(CAUSAL && kv0 + TILE - 1 > qw);
+            const bool whole = kv0 + TILE <= n;
             const bool far_hi = kv0 - qw - 31 >= rel.R, far_lo = kv0 - qw + 63 <= -rel.R;
             // all fragment reads of a group are issued before its first MFMA waits for one, and those of V before the
             // softmax arithmetic, which hides them
@@ -215,10 +247,8 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int kv = kv0 + t * 32 + acc_row(r, h);
-                            if (kv >= n || (CAUSAL && kv > q)) st[t][r] = -INFINITY;
-                        }
+                        for (int r = 0; r < 16; ++r)
+                            if (kv0 + t * 32 + acc_row(r, h) >= n) st[t][r] = -INFINITY;
                 }
             }
 #pragma unroll
@@ -232,9 +262,20 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[t][r]);
             mx = both_halves_max(mx);
-            const float m_new = fmaxf(m, fmaf(mx, sl2, shift));
-            const float msub = m_new == -INFINITY ? 0.f : m_new, off = shift - msub;
-            const float alpha = __builtin_amdgcn_exp2f(m - msub);
+            // The subtracted maximum only has to keep the exponentials in range: it moves when some query's has grown by more than
+            // 2^8 (or was -inf), and the accumulators are rescaled then.  Probabilities stay below 2^8 until then, which costs no
+            // precision: both roundings are relative.
+            const float m_tile = fmaf(mx, sl2, shift);
+            if (__builtin_amdgcn_ballot_w64(m_tile > m + 8.f)) {
+                const float m_new = fmaxf(m, m_tile), alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
+                m = m_new;
+                lsum *= alpha;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ot[u][r] *= alpha;
+            }
+            const float off = shift - (m == -INFINITY ? 0.f : m);
             float psum = 0.f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -244,19 +285,12 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
                     st[t][r] = p;
                     psum += p;
                 }
-            m = m_new;
-            lsum = lsum * alpha + psum;
+            lsum += psum;
             if constexpr (DROP) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) st[t][r] = (keep & (1u << (t * 16 + r))) ? st[t][r] : 0.f;
-            }
-            if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) ot[u][r] *= alpha;
             }
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
@@ -288,7 +322,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // dQ and the bias gradient: lanes own query columns, kv tiles are streamed
 // ---------------------------------------------------------------------------------------------
 template <bool CAUSAL, bool DROP>
-__global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *out,
+__global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *out,
                                                                   const bf16_t *dout, const float *lse, float *delta,
                                                                   bf16_t *dqkv, float *part, const int32_t *lengths, int S,
                                                                   int H, float scale, const uint32_t *keep_rows,
@@ -315,7 +349,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
     f32x16 dqt[2] = {zero16(), zero16()};
     float far_sum[2] = {0.f, 0.f};                            // blocks wholly before / behind the window
     if (kv_end > 0) {
-        const DirectTileLoader ldr(ld);
+        const TileStream ldr(ld);
         ldr.issue(K, n, Ks2[0]);
         ldr.issue(V, n, Vs2[0]);
         frag_t qf[4], dof[4];
@@ -337,7 +371,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
             delta_q += __shfl_xor(delta_q, 32, 64);
             if (qok && h == 0) delta[((int64_t)b * H + hh) * S + q] = delta_q;
         }
-        rel.expand<false>(win, hh, scale);                    // this and the zeroed sums: published by the loop's first barrier
+        rel.expand<false, CAUSAL>(win, hh, scale);                    // this and the zeroed sums: published by the loop's first barrier
         // ds is kept without its factor `scale`; a query that sees nothing (lse = -inf) has p = 0
         const float sl2 = scale * LOG2E, nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
         const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * ((S + TILE - 1) / TILE) * 2 + h : nullptr;
@@ -360,10 +394,10 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
             for (int t = 0; t < 2; ++t) {
                 const int k0 = kv0 + t * 32, D = k0 - qw;
                 if (qw >= n || k0 >= n || (CAUSAL && D > 31)) continue;        // nothing here that any query sees
-                const bool whole = k0 + 32 <= n && !(CAUSAL && D > -31);
+                const bool whole = k0 + 32 <= n;
                 const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;
                 f32x16 st, dp = zero16();
-                frag_t kf[4], vf[4], kt[2][2];
+                frag_t kf[4], vf[4];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     kf[s] = frag_rowk(Ks, t * 32 + c, s, h);
@@ -376,11 +410,6 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
                         st = mma(kf[s], qf[s], st);
                         dp = mma(vf[s], dof[s], dp);
                     }
-#pragma unroll
-                    for (int sp = 0; sp < 2; ++sp)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) kt[sp][u] = tr.frag(Ks, u * 32, t * 2 + sp);
-                    __builtin_amdgcn_sched_barrier(0);
                     if constexpr (DROP) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f;
@@ -403,10 +432,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
                     products();
                     if (!whole) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int kv = k0 + acc_row(r, h);
-                            if (kv >= n || (CAUSAL && kv > q)) st[r] = -INFINITY;
-                        }
+                        for (int r = 0; r < 16; ++r)
+                            if (k0 + acc_row(r, h) >= n) st[r] = -INFINITY;
                     }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl)) * (dp[r] - delta_q);
@@ -417,7 +444,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dq_kernel(const Rel
                 for (int sp = 0; sp < 2; ++sp) {
                     const frag_t db = acc_to_b(dp, sp);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) dqt[u] = mma(kt[sp][u], db, dqt[u]);
+                    for (int u = 0; u < 2; ++u) dqt[u] = mma(tr.frag(Ks, u * 32, t * 2 + sp), db, dqt[u]);
                 }
             }
         }
@@ -480,17 +507,24 @@ __global__ __launch_bounds__(1024) void relbias_dtable_kernel(const float *part,
 // ---------------------------------------------------------------------------------------------
 // dK, dV: lanes own kv columns, query tiles are streamed
 // ---------------------------------------------------------------------------------------------
+// A wave works on one 32 x 32 block of scores at a time: 8 matrix products for the scores and dP, 80 vector instructions a
+// lane for P and dS, 8 products for dV and dK.  Two waves fit a SIMD, so the wave itself has to keep the matrix pipe fed:
+// the score products of the NEXT block and the first half of this block's dV / dK products are issued one by one between the
+// vector instructions of this block (the order is pinned), three tiles are kept in LDS because the next block may be the next
+// tile's.  Everything that would be a branch a block is data: causally hidden pairs are -inf in the bias window, queries
+// beyond the end carry lse = +inf, and dP starts from -delta.
+#define PIN __builtin_amdgcn_sched_barrier(0)
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *dout,
                                                                    const float *lse, const float *delta, bf16_t *dqkv,
                                                                    const int32_t *lengths, int S, int H, float scale,
                                                                    const uint32_t *keep_cols, float keep_scale) {
-    __shared__ __attribute__((aligned(16))) char Qs2[2][TILE_BYTES];
-    __shared__ __attribute__((aligned(16))) char dOs2[2][TILE_BYTES];
-    __shared__ __attribute__((aligned(16))) float lse_s[2][3][TILE], delta_s[2][TILE];
+    constexpr int NST = 3;
+    __shared__ __attribute__((aligned(16))) char Qs3[NST][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char dOs3[NST][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) float lse_s[NST][TILE], delta_s[NST][TILE];
     extern __shared__ float win[];
     const TransposedReader tr;
-    const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
     const int blk = BlockOrder<CAUSAL>::row_block(false), bh = BlockOrder<CAUSAL>::batch_head();
     const int b = bh / H, hh = bh % H;
@@ -504,24 +538,18 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
     const float *lse_b = lse + ((int64_t)b * H + hh) * S, *delta_b = delta + ((int64_t)b * H + hh) * S;
     f32x16 dvt[2] = {zero16(), zero16()}, dkt[2] = {zero16(), zero16()};
     if (blk * 128 < n) {
-        frag_t kf[4], vf[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            kf[s] = load_row_frag(K + (int64_t)kv * ld, kok, s, h);
-            vf[s] = load_row_frag(V + (int64_t)kv * ld, kok, s, h);
-        }
-        const DirectTileLoader lq(ld), ldo(E);
+        const TileStream lq(ld), ldo(E);
         const float sl2 = scale * LOG2E;
         const int q_begin = CAUSAL ? blk * 128 : 0;           // causal: earlier queries see none of the block's keys
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
         const u32x2 *keep_col = DROP ? (const u32x2 *)(keep_cols + ((int64_t)bh * S + (kv < S ? kv : S - 1)) * (2 * ((S + TILE - 1) / TILE))) : nullptr;
-        u32x2 keep2 = {0xffffffffu, 0xffffffffu}, keep2_next = keep2;
-        // a query's log-sum-exp (times log2 e; of one that sees nothing +inf: p = 0) and the same less the bias before and
-        // behind the window, so that a far block needs neither a bias nor an addition a score; and its delta
+        u32x2 keep2 = {0u, 0u}, keep2_next = keep2;
+        // a query's log-sum-exp times log2 e (+inf where it sees nothing: p = 0) and its -delta (with dropout +delta, which
+        // then is subtracted behind the mask)
         float l_next = 0.f, d_next = 0.f;
         auto fetch = [&](int q0, int bufi) {
-            lq.issue(Q + (int64_t)q0 * ld, n - q0, Qs2[bufi]);
-            ldo.issue(dO + (int64_t)q0 * E, n - q0, dOs2[bufi]);
+            lq.issue(Q + (int64_t)q0 * ld, n - q0, Qs3[bufi]);
+            ldo.issue(dO + (int64_t)q0 * E, n - q0, dOs3[bufi]);
             if constexpr (DROP) keep2_next = keep_col[q0 / TILE];
             if (threadIdx.x < TILE) {
                 const int qq = q0 + threadIdx.x;
@@ -531,101 +559,169 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
         };
         auto stage = [&](int bufi) {
             if (threadIdx.x < TILE) {
-                const float l = l_next == -INFINITY ? INFINITY : l_next * LOG2E;
-                lse_s[bufi][0][threadIdx.x] = l;
-                lse_s[bufi][1][threadIdx.x] = l - win[W - 1] * sl2;           // (the window here runs over query - key)
-                lse_s[bufi][2][threadIdx.x] = l - win[0] * sl2;
-                delta_s[bufi][threadIdx.x] = d_next;
+                lse_s[bufi][threadIdx.x] = l_next == -INFINITY ? INFINITY : l_next * LOG2E;
+                delta_s[bufi][threadIdx.x] = DROP ? d_next : -d_next;
             }
         };
         fetch(q_begin, 0);
-        rel.expand<true>(win, hh, scale);
-        __syncthreads();                                      // the window is there
+        frag_t kf[4], vf[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            kf[s] = load_row_frag(K + (int64_t)kv * ld, kok, s, h);
+            vf[s] = load_row_frag(V + (int64_t)kv * ld, kok, s, h);
+        }
+        rel.expand<true, CAUSAL>(win, hh, scale);
         stage(0);
-        int buf = 0;
-        for (int q0 = q_begin; q0 < n; q0 += TILE) {
-            __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the tile has landed
-            __syncthreads();                                  // for everybody, and everybody is done with the other buffer
-            if constexpr (DROP) keep2 = keep2_next;
-            const bool more = q0 + TILE < n;
-            if (more) fetch(q0 + TILE, buf ^ 1);
-            const char *Qs = Qs2[buf], *dOs = dOs2[buf];
-#pragma unroll 1
-            for (int t = 0; t < 2; ++t) {
-                const int r0 = q0 + t * 32, D = r0 - kvw;
-                if (kvw >= n || r0 >= n || (CAUSAL && D < -31)) continue;      // nothing here that sees any of the wave's keys
-                const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;         // queries behind / before the keys
-                f32x16 sc, dp = zero16();
-                frag_t qa[4], da[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    qa[s] = frag_rowk(Qs, t * 32 + c, s, h);
-                    da[s] = frag_rowk(dOs, t * 32 + c, s, h);
-                }
-                auto products = [&]() {                       // every group of reads is issued before the arithmetic that hides it
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        sc = mma(qa[s], kf[s], sc);
-                        dp = mma(da[s], vf[s], dp);
-                    }
-                };
-                const float *lse_t = lse_s[buf][0];
-                if (far_hi || far_lo) {
-                    lse_t = lse_s[buf][far_hi ? 1 : 2];
-                    sc = zero16();
-                    products();
-                } else {
-                    sc = bias_tile(win + rel.at<32>(D, c, h));
-                    products();
-                    if (CAUSAL && D < 31) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (kv > r0 + acc_row(r, h)) sc[r] = -INFINITY;
-                    }
-                }
-                frag_t qt[2][2], dt[2][2];
-#pragma unroll
-                for (int sp = 0; sp < 2; ++sp)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        dt[sp][u] = tr.frag(dOs, u * 32, t * 2 + sp);
-                        qt[sp][u] = tr.frag(Qs, u * 32, t * 2 + sp);
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-                const uint32_t keep = t ? keep2.y : keep2.x;
-                if constexpr (DROP) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << acc_row(r, h))) ? dp[r] * keep_scale : 0.f;
-                }
+        if constexpr (DROP) keep2 = keep2_next;
+        __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): the first tile has landed
+        __syncthreads();
+        int buf = 0, nbuf = 1;
+        if (q_begin + TILE < n) fetch(q_begin + TILE, 1);
+
+        f32x16 sc0, dp0, sc1, dp1;
+        frag_t qa[4], da[4];
+        auto read_frag = [&](int bufi, int t, int s) {
+            qa[s] = frag_rowk(Qs3[bufi], t * 32 + c, s, h);
+            da[s] = frag_rowk(dOs3[bufi], t * 32 + c, s, h);
+        };
+        // a block's accumulators before its products: the bias, -delta
+        auto read_start = [&](int bufi, int t, int q0, f32x16 &x, f32x16 &y) {
+            x = bias_tile(win + rel.at<32>(q0 + t * 32 - kvw, c, h));
+            if constexpr (DROP) y = zero16();
+            else {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int ql = t * 32 + g * 8 + h * 4;
-                    const f32x4 l4 = *(const f32x4 *)(lse_t + ql), d4 = *(const f32x4 *)(delta_s[buf] + ql);
+                    const f32x4 d4 = *(const f32x4 *)(delta_s[bufi] + t * 32 + g * 8 + h * 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = g * 4 + e;
-                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, -l4[e]));
-                        sc[r] = p;
-                        dp[r] = p * (dp[r] - d4[e]);
-                    }
-                }
-                if constexpr (DROP) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sc[r] = (keep & (1u << acc_row(r, h))) ? sc[r] * keep_scale : 0.f;
-                }
-#pragma unroll
-                for (int sp = 0; sp < 2; ++sp) {
-                    const frag_t pb = acc_to_b(sc, sp), db = acc_to_b(dp, sp);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        dvt[u] = mma(dt[sp][u], pb, dvt[u]);
-                        dkt[u] = mma(qt[sp][u], db, dkt[u]);
-                    }
+                    for (int e = 0; e < 4; ++e) y[g * 4 + e] = d4[e];
                 }
             }
-            if (more) stage(buf ^ 1);
-            buf ^= 1;
+        };
+        // P, dS, dV, dK of block (cbuf, t) whose scores and dP - delta are in (sc, dp), and the scores of block (nb, nt) of the
+        // query tile at nq0 into (xs, xd).  Behind the last block that is some old tile's data, whose result nobody uses.
+        auto block = [&](f32x16 &sc, f32x16 &dp, f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt, int nq0) {
+            const char *Qs = Qs3[cbuf], *dOs = dOs3[cbuf];
+            const float *lse_t = lse_s[cbuf] + t * 32 + h * 4, *delta_t = delta_s[cbuf] + t * 32 + h * 4;
+            const uint32_t keep = t ? keep2.y : keep2.x;
+            f32x4 l4, d4, l4n, d4n;
+            auto stats = [&](int g, f32x4 &l, f32x4 &d) {
+                l = *(const f32x4 *)(lse_t + g * 8);
+                if constexpr (DROP) d = *(const f32x4 *)(delta_t + g * 8);
+            };
+            auto score = [&](int r) {                         // P and dS of score register r
+                const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, -l4[r & 3]));
+                if constexpr (DROP) {
+                    const bool kp = keep & (1u << acc_row(r, h));
+                    dp[r] = p * ((kp ? dp[r] * keep_scale : 0.f) - d4[r & 3]);
+                    sc[r] = kp ? p * keep_scale : 0.f;
+                } else {
+                    dp[r] = p * dp[r];
+                    sc[r] = p;
+                }
+            };
+            auto next_scores = [&](int s) { xs = mma(qa[s], kf[s], xs); };
+            auto next_dp = [&](int s) { xd = mma(da[s], vf[s], xd); };
+            stats(0, l4, d4);
+            read_frag(nb, nt, 0);
+            read_start(nb, nt, nq0, xs, xd);
+            read_frag(nb, nt, 1);
+            stats(1, l4n, d4n);
+            PIN;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) score(r);
+            l4 = l4n; d4 = d4n;
+            PIN;
+            next_scores(0);
+            PIN;
+            score(4);
+            score(5);
+            PIN;
+            next_dp(0);
+            PIN;
+            score(6);
+            score(7);
+            frag_t pb = acc_to_b(sc, 0), db = acc_to_b(dp, 0), dt[2], qt[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                dt[u] = tr.frag(dOs, u * 32, t * 2);
+                qt[u] = tr.frag(Qs, u * 32, t * 2);
+            }
+            stats(2, l4, d4);
+            read_frag(nb, nt, 2);
+            PIN;
+            next_scores(1);
+            PIN;
+            score(8);
+            PIN;
+            next_dp(1);
+            PIN;
+            score(9);
+            read_frag(nb, nt, 3);
+            stats(3, l4n, d4n);
+            PIN;
+            dvt[0] = mma(dt[0], pb, dvt[0]);
+            PIN;
+            score(10);
+            PIN;
+            dkt[0] = mma(qt[0], db, dkt[0]);
+            PIN;
+            score(11);
+            l4 = l4n; d4 = d4n;
+            PIN;
+            next_scores(2);
+            PIN;
+            score(12);
+            PIN;
+            dvt[1] = mma(dt[1], pb, dvt[1]);
+            PIN;
+            score(13);
+            PIN;
+            dkt[1] = mma(qt[1], db, dkt[1]);
+            PIN;
+            score(14);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                dt[u] = tr.frag(dOs, u * 32, t * 2 + 1);
+                qt[u] = tr.frag(Qs, u * 32, t * 2 + 1);
+            }
+            PIN;
+            next_dp(2);
+            PIN;
+            score(15);
+            pb = acc_to_b(sc, 1);
+            db = acc_to_b(dp, 1);
+            PIN;
+            next_scores(3);
+            next_dp(3);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                dvt[u] = mma(dt[u], pb, dvt[u]);
+                dkt[u] = mma(qt[u], db, dkt[u]);
+            }
+        };
+        read_start(0, 0, q_begin, sc0, dp0);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) read_frag(0, 0, s);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            sc0 = mma(qa[s], kf[s], sc0);
+            dp0 = mma(da[s], vf[s], dp0);
+        }
+        for (int q0 = q_begin; q0 < n; q0 += TILE) {
+            block(sc0, dp0, sc1, dp1, buf, 0, buf, 1, q0);
+            const int fbuf = nbuf == NST - 1 ? 0 : nbuf + 1;
+            u32x2 keep_after = keep2;
+            if (q0 + TILE < n) {
+                stage(nbuf);
+                if constexpr (DROP) keep_after = keep2_next;
+            }
+            __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the next tile has landed
+            __syncthreads();                                  // for everybody, and everybody is done with the tile before this one
+            if (q0 + 2 * TILE < n) fetch(q0 + 2 * TILE, fbuf);
+            block(sc1, dp1, sc0, dp0, buf, 1, nbuf, 0, q0 + TILE);
+            if constexpr (DROP) keep2 = keep_after;
+            buf = nbuf;
+            nbuf = fbuf;
         }
     }
     if (kv < S) {
