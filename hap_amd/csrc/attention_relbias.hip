@@ -599,15 +599,23 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
         };
         // P, dS, dV, dK of block (cbuf, t) whose scores and dP - delta are in (sc, dp), and the scores of block (nb, nt) of the
         // query tile at nq0 into (xs, xd).  Behind the last block that is some old tile's data, whose result nobody uses.
-        auto block = [&](f32x16 &sc, f32x16 &dp, f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt, int nq0) {
+        f32x4 l4, d4, l4n, d4n;                               // row statistics of the four rows being worked on, and of the next four
+        auto stats = [&](int cbuf, int t, int g, f32x4 &l, f32x4 &d) {
+            l = *(const f32x4 *)(lse_s[cbuf] + t * 32 + h * 4 + g * 8);
+            if constexpr (DROP) d = *(const f32x4 *)(delta_s[cbuf] + t * 32 + h * 4 + g * 8);
+        };
+        // first reads for block (cbuf, t) and for the scores of block (nb, nt), issued behind the products of the block before
+        auto prepare = [&](f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt, int nq0) {
+            stats(cbuf, t, 0, l4, d4);
+            stats(cbuf, t, 1, l4n, d4n);
+            read_start(nb, nt, nq0, xs, xd);
+            read_frag(nb, nt, 0);
+            read_frag(nb, nt, 1);
+            PIN;
+        };
+        auto block = [&](f32x16 &sc, f32x16 &dp, f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt) {
             const char *Qs = Qs3[cbuf], *dOs = dOs3[cbuf];
-            const float *lse_t = lse_s[cbuf] + t * 32 + h * 4, *delta_t = delta_s[cbuf] + t * 32 + h * 4;
             const uint32_t keep = t ? keep2.y : keep2.x;
-            f32x4 l4, d4, l4n, d4n;
-            auto stats = [&](int g, f32x4 &l, f32x4 &d) {
-                l = *(const f32x4 *)(lse_t + g * 8);
-                if constexpr (DROP) d = *(const f32x4 *)(delta_t + g * 8);
-            };
             auto score = [&](int r) {                         // P and dS of score register r
                 const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, -l4[r & 3]));
                 if constexpr (DROP) {
@@ -621,15 +629,10 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
             };
             auto next_scores = [&](int s) { xs = mma(qa[s], kf[s], xs); };
             auto next_dp = [&](int s) { xd = mma(da[s], vf[s], xd); };
-            stats(0, l4, d4);
-            read_frag(nb, nt, 0);
-            read_start(nb, nt, nq0, xs, xd);
-            read_frag(nb, nt, 1);
-            stats(1, l4n, d4n);
-            PIN;
 #pragma unroll
             for (int r = 0; r < 4; ++r) score(r);
             l4 = l4n; d4 = d4n;
+            stats(cbuf, t, 2, l4n, d4n);
             PIN;
             next_scores(0);
             PIN;
@@ -646,7 +649,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
                 dt[u] = tr.frag(dOs, u * 32, t * 2);
                 qt[u] = tr.frag(Qs, u * 32, t * 2);
             }
-            stats(2, l4, d4);
+            l4 = l4n; d4 = d4n;
+            stats(cbuf, t, 3, l4n, d4n);
             read_frag(nb, nt, 2);
             PIN;
             next_scores(1);
@@ -657,13 +661,14 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
             PIN;
             score(9);
             read_frag(nb, nt, 3);
-            stats(3, l4n, d4n);
             PIN;
             dvt[0] = mma(dt[0], pb, dvt[0]);
             PIN;
             score(10);
             PIN;
             dkt[0] = mma(qt[0], db, dkt[0]);
+            dt[0] = tr.frag(dOs, 0, t * 2 + 1);
+            qt[0] = tr.frag(Qs, 0, t * 2 + 1);
             PIN;
             score(11);
             l4 = l4n; d4 = d4n;
@@ -677,13 +682,10 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
             score(13);
             PIN;
             dkt[1] = mma(qt[1], db, dkt[1]);
+            dt[1] = tr.frag(dOs, 32, t * 2 + 1);
+            qt[1] = tr.frag(Qs, 32, t * 2 + 1);
             PIN;
             score(14);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                dt[u] = tr.frag(dOs, u * 32, t * 2 + 1);
-                qt[u] = tr.frag(Qs, u * 32, t * 2 + 1);
-            }
             PIN;
             next_dp(2);
             PIN;
@@ -698,6 +700,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
                 dvt[u] = mma(dt[u], pb, dvt[u]);
                 dkt[u] = mma(qt[u], db, dkt[u]);
             }
+            PIN;
         };
         read_start(0, 0, q_begin, sc0, dp0);
 #pragma unroll
@@ -707,8 +710,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
             sc0 = mma(qa[s], kf[s], sc0);
             dp0 = mma(da[s], vf[s], dp0);
         }
+        prepare(sc1, dp1, 0, 0, 0, 1, q_begin);
         for (int q0 = q_begin; q0 < n; q0 += TILE) {
-            block(sc0, dp0, sc1, dp1, buf, 0, buf, 1, q0);
+            block(sc0, dp0, sc1, dp1, buf, 0, buf, 1);
             const int fbuf = nbuf == NST - 1 ? 0 : nbuf + 1;
             u32x2 keep_after = keep2;
             if (q0 + TILE < n) {
@@ -718,7 +722,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
             __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the next tile has landed
             __syncthreads();                                  // for everybody, and everybody is done with the tile before this one
             if (q0 + 2 * TILE < n) fetch(q0 + 2 * TILE, fbuf);
-            block(sc1, dp1, sc0, dp0, buf, 1, nbuf, 0, q0 + TILE);
+            prepare(sc0, dp0, buf, 1, nbuf, 0, q0 + TILE);
+            block(sc1, dp1, sc0, dp0, buf, 1, nbuf, 0);
+            prepare(sc1, dp1, nbuf, 0, nbuf, 1, q0 + TILE);
             if constexpr (DROP) keep2 = keep_after;
             buf = nbuf;
             nbuf = fbuf;
