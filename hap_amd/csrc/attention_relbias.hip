@@ -19,7 +19,7 @@
 // lanes 0 .. 31 with zeros above: the swap of half waves delivers that for the two rows of an accumulator register at
 // once.  That is 4 vector instructions a register, and no atomics: LDS float additions of the 16 registers cost 180 cycles
 // each on this chip (the dQ kernel of [12, 512] x 16 heads took 274 us with them).  The vector is added to the wave's own
-// window in LDS; the block adds its four windows and sums the buckets' ranges, a second kernel adds the blocks, all in a
+// window in LDS; the block adds its four windows and sums the buckets' ranges, the dK / dV kernel adds the blocks, all in a
 // fixed order: the same bits every time.
 #include "common.h"
 #include "attention_tile.h"
@@ -53,9 +53,12 @@ struct RelArgs {
     __device__ __forceinline__ void range(int u, int &lo, int &hi) const {
         int first = 0, next = R + MARGIN + 1;                 // distances of the bucket: first .. next - 1
         const int k = bidir && u >= side ? u - side : u;
-        for (int i = 0; i < side; ++i) {                      // (starts[] is indexed by the loop only: scalar loads)
-            if (i == k) first = starts[i];
-            if (i == k + 1) next = starts[i];
+        for (int i = 0; i < side; i += 16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {                    // (starts[] is indexed by the loops only: scalar loads)
+                if (i + j == k) first = starts[i + j];
+                if (i + j == k + 1 && k + 1 < side) next = starts[i + j];
+            }
         }
         if (bidir && u >= side) { lo = first < 1 ? 1 : first; hi = next - 1; }
         else { lo = -(next - 1); hi = first == 0 ? (bidir || next < 1 ? 0 : R + MARGIN) : -first; }
@@ -64,12 +67,18 @@ struct RelArgs {
     // the head's bias / scale over the window; REV: entry i belongs to relative position -(i - R - MARGIN); CAUSAL: keys behind
     // the query are hidden
     template <bool REV, bool CAUSAL> __device__ __forceinline__ void expand(float *win, int head, float scale) const {
-        for (int i = threadIdx.x; i < window(); i += AT_THREADS) {
+        const int W = window();
+        auto entry = [&](int i) {                             // relative position of entry i, beyond the window the nearest end's
             int rel = i - R - MARGIN;
             rel = rel < -R ? -R : (rel > R ? R : rel);
-            if (REV) rel = -rel;
-            const float t = table[(int64_t)bucket(rel) * ld + head];
-            win[i] = t <= HIDDEN || (CAUSAL && rel > 0) ? -INFINITY : t / scale;
+            return REV ? -rel : rel;
+        };
+        auto put = [&](int i, int rel, float t) { win[i] = t <= HIDDEN || (CAUSAL && rel > 0) ? -INFINITY : t / scale; };
+        for (int i = threadIdx.x; i < W; i += 2 * AT_THREADS) {             // two entries a turn: both loads under way at once
+            const int i1 = i + AT_THREADS, r0 = entry(i), r1 = entry(i1 < W ? i1 : i);
+            const float t0 = table[(int64_t)bucket(r0) * ld + head], t1 = table[(int64_t)bucket(r1) * ld + head];
+            put(i, r0, t0);
+            if (i1 < W) put(i1, r1, t1);
         }
     }
     // word of the window that the lane's row 0 of a block of ROWS x 32 scores reads; D = first row - first column
@@ -482,24 +491,25 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
     }
 }
 
-// dT[u, h] (+)= the blocks' sums part[b][H][row blocks][buckets], in order.  One block per head; 1024 / buckets threads share
-// a bucket, each over a run of blocks, their sums added in order.
-__global__ __launch_bounds__(1024) void relbias_dtable_kernel(const float *part, float *dtable, int64_t ldd, int n_buckets, int b, int H,
-                                                            int row_blocks, int accumulate) {
-    __shared__ float red[1024];
-    const int h = blockIdx.x, u = threadIdx.x % n_buckets, run = threadIdx.x / n_buckets, runs = 1024 / n_buckets;
-    const int64_t items = (int64_t)b * row_blocks;
+// dT[u, head] (+)= the dQ blocks' sums part[b][H][row blocks][buckets], in order, by one block of the dK / dV kernel for each
+// head: AT_THREADS / buckets threads share a bucket, each over every so many-th block, their sums added in order.
+__device__ __forceinline__ void table_gradient(const float *part, float *dtable, int64_t ldd, int n_buckets, int b, int H, int head, int row_blocks,
+                                              int accumulate, float *red) {
+    const int u = threadIdx.x % n_buckets, run = threadIdx.x / n_buckets, runs = AT_THREADS / n_buckets;
     if (run < runs) {
         float v = 0.f;
-#pragma unroll 4
-        for (int64_t i = run; i < items; i += runs) v += part[(((i / row_blocks) * H + h) * row_blocks + i % row_blocks) * n_buckets + u];
+        for (int z = 0; z < b; ++z) {
+            const float *p = part + ((int64_t)z * H + head) * row_blocks * n_buckets + u;
+#pragma unroll 8
+            for (int k = run; k < row_blocks; k += runs) v += p[(int64_t)k * n_buckets];
+        }
         red[threadIdx.x] = v;
     }
     __syncthreads();
     if (run == 0) {
         float v = 0.f;
         for (int i = 0; i < runs; ++i) v += red[i * n_buckets + u];
-        float *d = dtable + (int64_t)u * ldd + h;
+        float *d = dtable + (int64_t)u * ldd + head;
         *d = accumulate ? *d + v : v;
     }
 }
@@ -518,7 +528,8 @@ template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *dout,
                                                                    const float *lse, const float *delta, bf16_t *dqkv,
                                                                    const int32_t *lengths, int S, int H, float scale,
-                                                                   const uint32_t *keep_cols, float keep_scale) {
+                                                                   const uint32_t *keep_cols, float keep_scale, const float *part,
+                                                                   float *dtable, int64_t ldd, int n_buckets, int batch, int accumulate) {
     constexpr int NST = 3;
     __shared__ __attribute__((aligned(16))) char Qs3[NST][TILE_BYTES];
     __shared__ __attribute__((aligned(16))) char dOs3[NST][TILE_BYTES];
@@ -746,6 +757,10 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
                 *(bf16x4 *)(drow + 2 * E + u * 32 + g * 8 + h * 4) = ov;
             }
     }
+    if (b == 0 && blk == (int)gridDim.x - 1) {                // (with the causal mask the block with the least work)
+        __syncthreads();
+        table_gradient(part, dtable, ldd, n_buckets, batch, H, hh, (int)gridDim.x, accumulate, win);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -867,17 +882,15 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
         return HAPMI_OK;
     };
     auto dkv = [&](auto kernel) -> int {
-        hipLaunchKernelGGL(kernel, grid, block, (size_t)W * 4, st, a, (const bf16_t *)qkv, (const bf16_t *)dout, lse, (const float *)delta_ws,
-                           (bf16_t *)dqkv, lengths, (int)S, (int)H, scale, keep_cols, ks);
+        hipLaunchKernelGGL(kernel, grid, block, (size_t)(W > AT_THREADS ? W : AT_THREADS) * 4, st, a, (const bf16_t *)qkv, (const bf16_t *)dout, lse,
+                           (const float *)delta_ws, (bf16_t *)dqkv, lengths, (int)S, (int)H, scale, keep_cols, ks, (const float *)workspace, dtable,
+                           ld_dtable, bias_host->n_buckets, (int)b, accumulate);
         HAPMI_CHECK_LAUNCH(name);
         return HAPMI_OK;
     };
     if (causal) rc = drop ? dq(relbias_bwd_dq_kernel<true, true>) : dq(relbias_bwd_dq_kernel<true, false>);
     else rc = drop ? dq(relbias_bwd_dq_kernel<false, true>) : dq(relbias_bwd_dq_kernel<false, false>);
     if (rc) return rc;
-    hipLaunchKernelGGL(relbias_dtable_kernel, dim3((unsigned)H), dim3(1024), 0, st, (const float *)workspace, dtable, ld_dtable,
-                       bias_host->n_buckets, (int)b, (int)H, (int)row_blocks, accumulate);
-    HAPMI_CHECK_LAUNCH(name);
     if (causal) return drop ? dkv(relbias_bwd_dkv_kernel<true, true>) : dkv(relbias_bwd_dkv_kernel<true, false>);
     return drop ? dkv(relbias_bwd_dkv_kernel<false, true>) : dkv(relbias_bwd_dkv_kernel<false, false>);
 }
