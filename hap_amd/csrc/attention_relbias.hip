@@ -158,6 +158,26 @@ __device__ __forceinline__ float both_halves_max(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// Which 128-row block of which (batch, head) a thread block takes.  Blocks are dealt round-robin over the 8 XCDs in the order
+// of their linear index; the row blocks of one (batch, head) stream the same tiles, so they go to one XCD, next to each
+// other in time.  Neighbouring heads go to different XCDs: in a padded batch they have the same length, and a long sample
+// would otherwise land on one XCD (dK / dV of lengths 334 .. 1001 in [6, 1001] x 12 heads: 62 us with a contiguous eighth of the heads on
+// each XCD).  Causal: the row blocks with the most work start first (BlockOrder), which keeps a head on its XCD too.
+template <bool CAUSAL> struct Order {
+    int blk, bh;
+    __device__ __forceinline__ Order(bool work_grows_with_index) {
+        if (CAUSAL) {
+            blk = BlockOrder<true>::row_block(work_grows_with_index);
+            bh = BlockOrder<true>::batch_head();
+        } else {
+            const int gx = (int)gridDim.x, l = (int)(blockIdx.y * gridDim.x + blockIdx.x), even = (int)gridDim.y / 8 * 8;
+            const int turn = l < even * gx ? l / 8 : l;
+            blk = turn % gx;
+            bh = l < even * gx ? turn / gx * 8 + l % 8 : turn / gx;
+        }
+    }
+};
+
 __device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) {
     if (!lengths) return S;
     const int n = lengths[b];
@@ -179,7 +199,8 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
     const TransposedReader tr;
     const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
-    const int blk = BlockOrder<CAUSAL>::row_block(true), bh = BlockOrder<CAUSAL>::batch_head();
+    const Order<CAUSAL> order(true);
+    const int blk = order.blk, bh = order.bh;
     const int b = bh / H, hh = bh % H;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int n = row_length(lengths, b, S);
@@ -342,7 +363,8 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
     const TransposedReader tr;
     const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
-    const int blk = BlockOrder<CAUSAL>::row_block(true), bh = BlockOrder<CAUSAL>::batch_head();
+    const Order<CAUSAL> order(true);
+    const int blk = order.blk, bh = order.bh;
     const int b = bh / H, hh = bh % H;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int n = row_length(lengths, b, S);
@@ -537,7 +559,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
     extern __shared__ float win[];
     const TransposedReader tr;
     const int E = H * HD, ld = 3 * E;
-    const int blk = BlockOrder<CAUSAL>::row_block(false), bh = BlockOrder<CAUSAL>::batch_head();
+    const Order<CAUSAL> order(false);
+    const int blk = order.blk, bh = order.bh;
     const int b = bh / H, hh = bh % H;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int n = row_length(lengths, b, S);

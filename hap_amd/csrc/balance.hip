@@ -81,84 +81,111 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_count_kernel(const float 
     }
 }
 
-// joins the slabs of every row (slabs == 1: counts, kept, psum are the first kernel's own outputs) and adds up the loss
+// joins the slabs of every row (slabs == 1: counts, kept, psum are the first kernel's own outputs) and adds up the loss; a
+// thread takes V experts of a row, the loads of eight slabs under way at once
+template <int V>
 __global__ __launch_bounds__(1024) void balance_join_kernel(const int32_t *lengths, const int32_t *pcounts, const int32_t *pkept,
                                                           const float *ppsum, int32_t *counts, int32_t *kept, float *psum, float *loss,
                                                           int B, int S, int E, int slabs, float coef, int choices) {
+    typedef int32_t iv __attribute__((ext_vector_type(V)));
+    typedef float fv __attribute__((ext_vector_type(V)));
     __shared__ float red[16];
-    const float G = bal_rows(lengths, B, S, red);
     float v = 0.f;
-    for (int64_t i = threadIdx.x; i < (int64_t)B * E; i += 1024) {
+    for (int64_t i = (int64_t)threadIdx.x * V; i < (int64_t)B * E; i += 1024 * V) {
         const int b = (int)(i / E), e = (int)(i - (int64_t)b * E);
-        int32_t c = 0, k = 0;
-        float p = 0.f;
+        const int64_t at = (int64_t)b * slabs * E + e;
+        iv c = 0, k = 0;
+        fv p = 0.f;
+#pragma unroll 8
         for (int z = 0; z < slabs; ++z) {
-            const int64_t at = ((int64_t)b * slabs + z) * E + e;
-            c += pcounts[at];
-            k += pkept[at];
-            p += ppsum[at];
+            c += *(const iv *)(pcounts + at + z * E);
+            k += *(const iv *)(pkept + at + z * E);
+            p += *(const fv *)(ppsum + at + z * E);
         }
         if (slabs > 1) {
-            counts[i] = c;
-            kept[i] = k;
-            psum[i] = p;
+            *(iv *)(counts + i) = c;
+            *(iv *)(kept + i) = k;
+            *(fv *)(psum + i) = p;
         }
         const float n = (float)bal_length(lengths, b, S);
-        if (n > 0.f) v += (float)c / n * (p / n);
+        if (n > 0.f) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v += (float)c[j] / n * (p[j] / n);
+        }
     }
+    const float G = bal_rows(lengths, B, S, red);
     v = block_sum(v, red);
     if (threadIdx.x == 0) loss[0] = G > 0.f ? coef * (float)E / (G * (float)choices) * v : 0.f;
 }
 
-// a group of lanes per token, V experts a lane
+// a group of lanes per token, V experts a lane; BAL_TURNS tokens of a lane are loaded before the first one is worked on
+constexpr int BAL_TURNS = 4;
 template <int V>
 __global__ __launch_bounds__(BAL_THREADS) void balance_bwd_kernel(const float *probs, const int32_t *index, const int32_t *slot,
                                                                 const float *dgate, const int32_t *counts, const int32_t *lengths,
-                                                                float *dlogits, int B, int S, int E, float coef, int choices, int slab,
+                                                                float *dlogits, int B, int S, int E, float coef, int choices,
                                                                 int group_log2) {
     __shared__ float red[16];
+    typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
     const int b = blockIdx.y, n = bal_length(lengths, b, S);
+    const int j = threadIdx.x & ((1 << group_log2) - 1), e0 = j * V, per = BAL_THREADS >> group_log2;
+    const int s0 = blockIdx.x * per * BAL_TURNS + (int)(threadIdx.x >> group_log2);
+    float p[BAL_TURNS][V], dg[BAL_TURNS][2];
+    int at[BAL_TURNS][2];
+#pragma unroll
+    for (int t = 0; t < BAL_TURNS; ++t) {
+        const int s = s0 + t * per;
+        const int64_t tok = (int64_t)b * S + s;
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[t][i] = 0.f;
+        at[t][0] = at[t][1] = -1;
+        dg[t][0] = dg[t][1] = 0.f;
+        if (s >= S) continue;
+        if (V == 4) {
+            if (e0 < E) {
+                const f32x4 x = *(const f32x4 *)(probs + tok * E + e0);
+#pragma unroll
+                for (int i = 0; i < V; ++i) p[t][i] = x[i];
+            }
+        } else if (e0 < E) {
+            p[t][0] = probs[tok * E + e0];
+        }
+        if (dgate) {
+            const i32x2 ix = *(const i32x2 *)(index + tok * 2), sl = *(const i32x2 *)(slot + tok * 2);
+            const f32x2 g = *(const f32x2 *)(dgate + tok * 2);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                at[t][k] = ix[k];
+                dg[t][k] = sl[k] > 0 ? g[k] : 0.f;
+            }
+        }
+    }
     const float G = bal_rows(lengths, B, S, red);
-    const int j = threadIdx.x & ((1 << group_log2) - 1), e0 = j * V;
     float w[V];
 #pragma unroll
     for (int i = 0; i < V; ++i)
         w[i] = n > 0 && e0 + i < E ? coef * (float)E / (G * (float)choices) * ((float)counts[(int64_t)b * E + e0 + i] / (float)n / (float)n) : 0.f;
-    const int s_end = (int)(blockIdx.x + 1) * slab < S ? (int)(blockIdx.x + 1) * slab : S;
-    for (int s = blockIdx.x * slab + (int)(threadIdx.x >> group_log2); s < s_end; s += BAL_THREADS >> group_log2) {
+#pragma unroll
+    for (int t = 0; t < BAL_TURNS; ++t) {
+        const int s = s0 + t * per;
         const int64_t tok = (int64_t)b * S + s;
-        float p[V], g[V], dot = 0.f;
-        if (V == 4 && e0 < E) {
-            const f32x4 x = *(const f32x4 *)(probs + tok * E + e0);
+        float g[V], dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) p[i] = x[i];
-        } else {
+        for (int i = 0; i < V; ++i) {
+            g[i] = s < n ? w[i] : 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) p[i] = e0 + i < E ? probs[tok * E + e0 + i] : 0.f;
+            for (int k = 0; k < 2; ++k) g[i] += at[t][k] == e0 + i ? dg[t][k] : 0.f;
+            dot += p[t][i] * g[i];
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = s < n ? w[i] : 0.f;
-        if (dgate) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int e = index[tok * 2 + k];
-                const float d = slot[tok * 2 + k] > 0 ? dgate[tok * 2 + k] : 0.f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[i] += e == e0 + i ? d : 0.f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) dot += p[i] * g[i];
         for (int o = 0; o < group_log2; ++o) dot += __shfl_xor(dot, 1 << o, 64);
-        if (V == 4 && e0 < E) {
+        if (s >= S || e0 >= E) continue;
+        if (V == 4) {
             f32x4 x;
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = p[i] * (g[i] - dot);
+            for (int i = 0; i < V; ++i) x[i] = p[t][i] * (g[i] - dot);
             *(f32x4 *)(dlogits + tok * E + e0) = x;
         } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (e0 + i < E) dlogits[tok * E + e0 + i] = p[i] * (g[i] - dot);
+            dlogits[tok * E + e0] = p[t][0] * (g[0] - dot);
         }
     }
 }
@@ -207,8 +234,14 @@ extern "C" int hapmi_balance_loss_fwd(const float *probs, const int32_t *index, 
     if (E % 4 == 0) hipLaunchKernelGGL((balance_count_kernel<4>), grid, block, 0, st, probs, index, slot, lengths, pc, pk, pp, (int)S, (int)E, choices, (int)slab);
     else hipLaunchKernelGGL((balance_count_kernel<1>), grid, block, 0, st, probs, index, slot, lengths, pc, pk, pp, (int)S, (int)E, choices, (int)slab);
     HAPMI_CHECK_LAUNCH(name);
-    hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(1024), 0, st, lengths, (const int32_t *)pc, (const int32_t *)pk, (const float *)pp, counts, kept, prob_sum,
-                       loss, (int)B, (int)S, (int)E, (int)slabs, coef, choices);
+    const bool vec = E % 4 == 0 && ((uintptr_t)pc % 16 == 0 && (uintptr_t)pk % 16 == 0 && (uintptr_t)pp % 16 == 0 && (uintptr_t)counts % 16 == 0 &&
+                                    (uintptr_t)kept % 16 == 0 && (uintptr_t)prob_sum % 16 == 0);
+    auto join = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, st, lengths, (const int32_t *)pc, (const int32_t *)pk, (const float *)pp, counts, kept, prob_sum, loss,
+                           (int)B, (int)S, (int)E, (int)slabs, coef, choices);
+    };
+    if (vec) join(balance_join_kernel<4>);
+    else join(balance_join_kernel<1>);
     HAPMI_CHECK_LAUNCH(name);
     return HAPMI_OK;
 }
@@ -225,10 +258,11 @@ extern "C" int hapmi_balance_loss_bwd(const float *probs, const int32_t *index, 
     const int V = E % 4 == 0 ? 4 : 1;
     int group_log2 = 0;
     while ((V << group_log2) < E) ++group_log2;
-    const int64_t slab = bal_slab(B, S, E);
-    const dim3 grid((unsigned)hapmi_cdiv(S, slab), (unsigned)B), block(BAL_THREADS);
-    if (V == 4) hipLaunchKernelGGL((balance_bwd_kernel<4>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, (int)slab, group_log2);
-    else hipLaunchKernelGGL((balance_bwd_kernel<1>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, (int)slab, group_log2);
+    HAPMI_REQUIRE(!dgate || ((uintptr_t)index % 8 == 0 && (uintptr_t)slot % 8 == 0 && (uintptr_t)dgate % 8 == 0), HAPMI_EALIGN,
+                  "%s: index, slot and dgate must be 8-byte aligned", name);
+    const dim3 grid((unsigned)hapmi_cdiv(S, (BAL_THREADS >> group_log2) * BAL_TURNS), (unsigned)B), block(BAL_THREADS);
+    if (V == 4) hipLaunchKernelGGL((balance_bwd_kernel<4>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, group_log2);
+    else hipLaunchKernelGGL((balance_bwd_kernel<1>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, group_log2);
     HAPMI_CHECK_LAUNCH(name);
     return HAPMI_OK;
 }

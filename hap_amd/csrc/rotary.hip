@@ -16,7 +16,7 @@ namespace {
 
 constexpr int QN_THREADS = 256;
 constexpr int QN_MAX_DIM = 256;
-constexpr int QN_MAX_BLOCKS = 1024;                 // backward: blocks whose gain sums a second kernel adds
+constexpr int QN_MAX_BLOCKS = 768;                  // backward: blocks whose gain sums a second kernel adds; 3 a CU are resident
 
 struct QnArgs {
     const float *q_gain, *k_gain;                   // [D] or NULL (ones)
@@ -136,8 +136,17 @@ template <int V> __device__ __forceinline__ void qn_gain(const float *g, const Q
     }
 }
 
+// sum over an aligned group of 2^group_log2 <= 32 lanes, in every lane: exchanges inside a row of 16 lanes ride on the additions
+// (DPP: neighbours, pairs, then mirrors, whose lanes hold equal sums), the last one swaps rows
+template <int CTRL> __device__ __forceinline__ float qn_dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float qn_group_sum(float v, int group_log2) {
-    for (int i = 0; i < group_log2; ++i) v += __shfl_xor(v, 1 << i, 64);
+    if (group_log2 > 0) v = qn_dpp_add<0xb1>(v);              // quad_perm [1, 0, 3, 2]
+    if (group_log2 > 1) v = qn_dpp_add<0x4e>(v);              // quad_perm [2, 3, 0, 1]
+    if (group_log2 > 2) v = qn_dpp_add<0x141>(v);             // row_half_mirror
+    if (group_log2 > 3) v = qn_dpp_add<0x140>(v);             // row_mirror
+    if (group_log2 > 4) v += __shfl_xor(v, 16, 64);
     return v;
 }
 
@@ -204,15 +213,20 @@ __global__ __launch_bounds__(QN_THREADS) void qk_norm_rotary_fwd_kernel(const Qn
 }
 
 template <typename T, bool GAINS>
-__global__ __launch_bounds__(QN_THREADS) void qk_norm_rotary_bwd_kernel(const QnArgs p, const T *dout, const T *qkv, T *dqkv, float *part) {
+__global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const QnArgs p, const T *dout, const T *qkv, T *dqkv, float *part) {
     constexpr int V = Vec16<T>::N;
     __shared__ float red[GAINS ? 4 * 2 * QN_MAX_DIM : 1];
+    __shared__ __attribute__((aligned(16))) float gains[2][QN_MAX_DIM];     // read again for every row: 32 registers less a lane
+    for (int i = threadIdx.x; i < p.D; i += QN_THREADS) {
+        gains[0][i] = p.q_gain ? p.q_gain[i] : 1.f;
+        gains[1][i] = p.k_gain ? p.k_gain[i] : 1.f;
+    }
+    __syncthreads();
     const int group = 1 << p.group_log2, j = threadIdx.x & (group - 1);
     const QnLane l = qn_lane<T>(p, j);
     const int E = p.H * p.D;
-    float gq[2][V], gk[2][V], acc[2][2][V];
-    qn_gain<V>(p.q_gain, l, gq[0], gq[1]);
-    qn_gain<V>(p.k_gain, l, gk[0], gk[1]);
+    const int ga = (l.a < 0 ? 0 : l.a) * V, gb = (l.b < 0 ? 0 : l.b) * V;
+    float acc[2][2][V];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -251,6 +265,7 @@ __global__ __launch_bounds__(QN_THREADS) void qk_norm_rotary_bwd_kernel(const Qn
             sq = qn_group_sum(sq, p.group_log2);
             const float r = bad ? NAN : 1.0f / sqrtf(sq / p.D + p.eps);
             if (l.turn_a || l.turn_b) qn_turn<V>(p, l, w, -1.f, da, db);
+            asm volatile("" ::: "memory");                    // (the gains are not to be hoisted into registers)
             float dot = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -260,8 +275,8 @@ __global__ __launch_bounds__(QN_THREADS) void qk_norm_rotary_bwd_kernel(const Qn
                     acc[t][0][e] += da[e] * a[e];
                     acc[t][1][e] += db[e] * b[e];
                 }
-                da[e] *= (t ? gk : gq)[0][e];
-                db[e] *= (t ? gk : gq)[1][e];
+                da[e] *= gains[t][ga + e];
+                db[e] *= gains[t][gb + e];
                 dot += da[e] * a[e] + db[e] * b[e];
             }
             dot = qn_group_sum(dot, p.group_log2) / p.D;

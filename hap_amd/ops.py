@@ -877,6 +877,7 @@ def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None,
     check(lib().hapmi_qk_norm_rotary_fwd(x_ if apart else o_, o_, q_, k_, r_, n_pos, rot, interleaved, p_, b, S, H, D, eps, code, stream))
 
 
+@functools.lru_cache(maxsize=256)
 def qk_norm_rotary_workspace_elems(D: int) -> int:
     """Float32 elements of the scratch buffer that ``qk_norm_rotary_bwd`` needs for the gains' gradients."""
     need = ctypes.c_int64()
@@ -1083,7 +1084,13 @@ def _on_device(what, t, like):
 
 def attention_relbias_workspace_elems(table, b, S, H, max_distance=128, bidirectional=None, causal=False) -> int:
     """Float32 elements of the scratch buffer that ``attention_relbias_bwd`` needs."""
-    rel = _relbias("attention_relbias_workspace_elems", table, H, max_distance, bidirectional, causal)
+    return _relbias_workspace_elems(table.shape[0], int(max_distance), (not causal) if bidirectional is None else bool(bidirectional), b, S, H)
+
+
+@functools.lru_cache(maxsize=256)
+def _relbias_workspace_elems(n_buckets, max_distance, bidirectional, b, S, H):
+    arr = _bucket_array(n_buckets, max_distance, bidirectional)
+    rel = _lib.RelBias(0, H, n_buckets, bidirectional, ctypes.addressof(arr))
     need = ctypes.c_int64()
     check(_lib._load().hapmi_attention_relbias_workspace_elems(ctypes.byref(rel), b, S, H, ctypes.byref(need)))
     return need.value
@@ -1105,16 +1112,15 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     _on_device(what, table, qkv)
     _on_device(what, dtable, qkv)
     _apart(what, [(*_rows_span(table), False), (*_rows_span(dtable), True)])
-    need = ctypes.c_int64()
-    check(_lib._load().hapmi_attention_relbias_workspace_elems(ctypes.byref(rel), b, S, H, ctypes.byref(need)))
-    workspace = _scratch(what, workspace, need.value, qkv.device)
+    need = attention_relbias_workspace_elems(table, b, S, H, max_distance, bidirectional, causal)
+    workspace = _scratch(what, workspace, need, qkv.device)
     E, words = H * 64, attention_keep_words(b, S, H) if keep_rows is not None else 0
     stream, (q_, o_, do_, l_, dq_, dl_, n_, kr_, kc_, ws_) = _operands(
         what, ("qkv", qkv, torch.bfloat16, b * S * 3 * E, False), ("out", out, torch.bfloat16, b * S * E, False),
         ("dout", dout, torch.bfloat16, b * S * E, False), ("lse", lse, torch.float32, b * H * S, False),
         ("dqkv", dqkv, torch.bfloat16, b * S * 3 * E, True), ("delta_ws", delta_ws, torch.float32, b * H * S, True),
         ("lengths", lengths, torch.int32, b, False), ("keep_rows", keep_rows, torch.int32, words, False),
-        ("keep_cols", keep_cols, torch.int32, words, False), ("workspace", workspace, torch.float32, need.value, True))
+        ("keep_cols", keep_cols, torch.int32, words, False), ("workspace", workspace, torch.float32, need, True))
     check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), max(dtable.stride(0), H), accumulate,
                                             dl_, _kept(ws_, workspace), workspace.numel(), b, S, H, scale, kr_, kc_, p, stream))
 
@@ -1492,6 +1498,13 @@ def _balance_shape(what, r, lengths):
     return B, S, E
 
 
+@functools.lru_cache(maxsize=256)
+def _balance_workspace_elems(B, S, E):
+    need = ctypes.c_int64()
+    check(_lib._load().hapmi_balance_workspace_elems(B, S, E, ctypes.byref(need)))
+    return need.value
+
+
 def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, lengths=None, workspace=None):
     """Balance loss of the routing records ``r`` (``top2_gate`` / ``switch_gate``) into ``loss`` (float32 [1]) and what it is
     made of: ``counts`` (int32 [B, E]: choices of every expert before capacity; ``choices`` = 1: first choices, 2: both),
@@ -1502,14 +1515,13 @@ def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, leng
     B, S, E = _balance_shape(what, r, lengths)
     _exactly(what, 1, loss)
     _exactly(what, B * E, counts, kept, prob_sum)
-    need = ctypes.c_int64()
-    check(_lib._load().hapmi_balance_workspace_elems(B, S, E, ctypes.byref(need)))
-    workspace = _scratch(what, workspace, need.value, loss.device) if need.value else None
+    need = _balance_workspace_elems(B, S, E)
+    workspace = _scratch(what, workspace, need, loss.device) if need else None
     stream, (p_, i_, s_, n_, l_, c_, k_, ps_, ws_) = _operands(
         what, ("probs", r["probs"], torch.float32, B * S * E, False), ("index", r["index"], torch.int32, B * S * 2, False),
         ("slot", r["slot"], torch.int32, B * S * 2, False), ("lengths", lengths, torch.int32, B, False), ("loss", loss, torch.float32, 1, True),
         ("counts", counts, torch.int32, B * E, True), ("kept", kept, torch.int32, B * E, True), ("prob_sum", prob_sum, torch.float32, B * E, True),
-        ("workspace", workspace, torch.float32, need.value, True))
+        ("workspace", workspace, torch.float32, need, True))
     check(lib().hapmi_balance_loss_fwd(p_, i_, s_, n_, l_, c_, k_, ps_, B, S, E, coef, choices, _kept(ws_, workspace),
                                        workspace.numel() if workspace is not None else 0, stream))
 
