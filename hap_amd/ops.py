@@ -73,31 +73,39 @@ def _span(rows: int, cols: int, ld: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _operands(what, *specs):
-    """Checks of a call's tensors in one pass over ``specs`` = (name, tensor or None, element type, elements that the kernel
-    touches, written): on the current device, of the type, contiguous, long enough, and nothing that is written shares
-    memory with another operand.  Returns the current stream and the pointers (0 for None), in order."""
+def _operands(what, names, dtypes, tensors, elems, written):
+    """Checks of a call's tensors in one pass: on the current device, of the element type, contiguous, at least ``elems`` long,
+    and none of the first ``written`` ones shares memory with another.  None entries are skipped.  Returns the current
+    stream and the pointers (0 for None), in order."""
     cur, ptrs, spans = -2, [], []
-    for name, t, dtype, elems, written in specs:
+    for t, dtype, n in zip(tensors, dtypes, elems):
         if t is None:
             ptrs.append(0)
             continue
-        if t.get_device() != cur:
-            _dev(t)
-            if cur >= 0 or t.get_device() != torch.cuda.current_device():
-                raise _lib.HapmiError(f"{what}: {name} is on {t.device}, not on the current device")
-            cur = t.get_device()
-        if t.dtype is not dtype:
-            raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
-        n = t.numel()
-        if elems < 0 or elems > n or not t.is_contiguous():
-            _need(t, elems, f"{what} {name}")
+        size = t.numel()
+        if t.get_device() != cur or t.dtype is not dtype or not 0 <= n <= size or not t.is_contiguous():
+            cur = _odd_operand(what, names[len(ptrs)], t, dtype, n, cur)
         ptr = t.data_ptr()
+        if size:
+            spans.append((ptr, ptr + size * _ITEM[dtype], len(ptrs) < written))
         ptrs.append(ptr)
-        if n:
-            spans.append((ptr, ptr + n * t.element_size(), written))
     _apart(what, spans)
     return _raw_stream(cur), ptrs
+
+
+_ITEM = {torch.float32: 4, torch.int32: 4, torch.bfloat16: 2}
+
+
+def _odd_operand(what, name, t, dtype, elems, cur):
+    """The first operand (whose device becomes the call's), or one that is refused."""
+    if t.get_device() != cur:
+        _dev(t)
+        if cur != -2 or t.get_device() != torch.cuda.current_device():
+            raise _lib.HapmiError(f"{what}: {name} is on {t.device}, not on the current device")
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    _need(t, elems, f"{what} {name}")
+    return t.get_device()
 
 
 def _exactly(what, n, *tensors):
@@ -107,12 +115,20 @@ def _exactly(what, n, *tensors):
 
 
 def _apart(what, spans):
+    """No (start, end, written) range that is written may overlap another one."""
     spans.sort()
-    end_any = end_written = 0
+    end = 0
+    for lo, hi, _ in spans:
+        if lo < end:
+            break
+        end = hi
+    else:
+        return
+    end = end_written = 0
     for lo, hi, written in spans:
-        if lo < end_written or (written and lo < end_any):
+        if lo < end_written or (written and lo < end):
             raise ValueError(f"{what}: an output shares memory with another operand")
-        end_any = max(end_any, hi)
+        end = max(end, hi)
         if written:
             end_written = max(end_written, hi)
 
@@ -127,7 +143,10 @@ def _scratch(what, workspace, elems: int, device):
 
 
 def _kept(ptr, owner):
-    """A pointer argument that keeps ``owner`` alive: a recorded launch list then replays with memory that is still there."""
+    """The pointer argument of ``owner``; while a launch list is being recorded an object that keeps ``owner`` alive, so that
+    the list replays with memory that is still there."""
+    if _lib._recorder is None:
+        return ptr
     ptr = ctypes.c_void_p(ptr)
     ptr._keep = owner
     return ptr
@@ -871,9 +890,10 @@ def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None,
     if out.numel() != n:
         raise ValueError(f"{what}: out must have qkv's size")
     apart = out.data_ptr() != qkv.data_ptr()
+    dt = qkv.dtype
     stream, (o_, x_, q_, k_, r_, p_) = _operands(
-        what, ("out", out, qkv.dtype, n, True), ("qkv", qkv if apart else None, qkv.dtype, n, False), ("q_gain", q_gain, torch.float32, D, False),
-        ("k_gain", k_gain, torch.float32, D, False), ("rotary", rotary, torch.float32, n_pos * rot, False), ("positions", positions, torch.int32, b * S, False))
+        what, ("out", "qkv", "q_gain", "k_gain", "rotary", "positions"), (dt, dt, torch.float32, torch.float32, torch.float32, torch.int32),
+        (out, qkv if apart else None, q_gain, k_gain, rotary, positions), (n, n, D, D, n_pos * rot, b * S), 1)
     check(lib().hapmi_qk_norm_rotary_fwd(x_ if apart else o_, o_, q_, k_, r_, n_pos, rot, interleaved, p_, b, S, H, D, eps, code, stream))
 
 
@@ -901,11 +921,12 @@ def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_ga
     else:
         workspace = None
     apart = dqkv.data_ptr() != dout.data_ptr()
-    stream, (dx_, do_, x_, q_, k_, dq_, dk_, r_, p_, ws_) = _operands(
-        what, ("dqkv", dqkv, qkv.dtype, n, True), ("dout", dout if apart else None, qkv.dtype, n, False), ("qkv", qkv, qkv.dtype, n, False),
-        ("q_gain", q_gain, torch.float32, D, False), ("k_gain", k_gain, torch.float32, D, False), ("dq_gain", dq_gain, torch.float32, D, True),
-        ("dk_gain", dk_gain, torch.float32, D, True), ("rotary", rotary, torch.float32, n_pos * rot, False),
-        ("positions", positions, torch.int32, b * S, False), ("workspace", workspace, torch.float32, ws_elems, True))
+    dt, f32 = qkv.dtype, torch.float32
+    stream, (dx_, dq_, dk_, ws_, do_, x_, q_, k_, r_, p_) = _operands(
+        what, ("dqkv", "dq_gain", "dk_gain", "workspace", "dout", "qkv", "q_gain", "k_gain", "rotary", "positions"),
+        (dt, f32, f32, f32, dt, dt, f32, f32, f32, torch.int32),
+        (dqkv, dq_gain, dk_gain, workspace, dout if apart else None, qkv, q_gain, k_gain, rotary, positions),
+        (n, D, D, ws_elems, n, n, D, D, n_pos * rot, b * S), 4)
     if not apart and dout.dtype is not qkv.dtype:
         raise TypeError(f"{what}: dtype mismatch")
     check(lib().hapmi_qk_norm_rotary_bwd(do_ if apart else dx_, x_, dx_, q_, k_, dq_, dk_, accumulate, r_, n_pos, rot, interleaved, p_, b, S, H, D,
@@ -1056,6 +1077,11 @@ def _rows_span(t):
     return t.data_ptr(), t.data_ptr() + 4 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])
 
 
+_RELBIAS_FWD_TYPES = (torch.bfloat16, torch.float32, torch.bfloat16, torch.int32, torch.int32)
+_RELBIAS_BWD_TYPES = (torch.bfloat16, torch.float32, torch.float32, torch.bfloat16, torch.bfloat16, torch.bfloat16, torch.float32, torch.int32,
+                      torch.int32, torch.int32)
+
+
 def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128, bidirectional=None, causal=False,
                           lengths=None, keep_rows=None, p=0.0):
     """``attention_fwd`` with a learned relative position bias: scores scale * q_i k_j + table[bucket(j - i), head],
@@ -1066,11 +1092,9 @@ def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128
     dropout of the probabilities, as in ``attention_fwd``."""
     what = "attention_relbias_fwd"
     _exactly(what, b, lengths)
-    E = H * 64
-    stream, (q_, o_, l_, n_, k_) = _operands(
-        what, ("qkv", qkv, torch.bfloat16, b * S * 3 * E, False), ("out", out, torch.bfloat16, b * S * E, True),
-        ("lse", lse, torch.float32, b * H * S, True), ("lengths", lengths, torch.int32, b, False),
-        ("keep_rows", keep_rows, torch.int32, attention_keep_words(b, S, H) if keep_rows is not None else 0, False))
+    n = b * S * H
+    stream, (o_, l_, q_, n_, k_) = _operands(what, ("out", "lse", "qkv", "lengths", "keep_rows"), _RELBIAS_FWD_TYPES, (out, lse, qkv, lengths, keep_rows),
+                                             (n * 64, n, n * 192, b, attention_keep_words(b, S, H) if keep_rows is not None else 0), 2)
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
     _on_device(what, table, qkv)
     check(lib().hapmi_attention_relbias_fwd(q_, ctypes.byref(rel), causal, n_, o_, l_, b, S, H, scale, k_, p, stream))
@@ -1114,13 +1138,10 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     _apart(what, [(*_rows_span(table), False), (*_rows_span(dtable), True)])
     need = attention_relbias_workspace_elems(table, b, S, H, max_distance, bidirectional, causal)
     workspace = _scratch(what, workspace, need, qkv.device)
-    E, words = H * 64, attention_keep_words(b, S, H) if keep_rows is not None else 0
-    stream, (q_, o_, do_, l_, dq_, dl_, n_, kr_, kc_, ws_) = _operands(
-        what, ("qkv", qkv, torch.bfloat16, b * S * 3 * E, False), ("out", out, torch.bfloat16, b * S * E, False),
-        ("dout", dout, torch.bfloat16, b * S * E, False), ("lse", lse, torch.float32, b * H * S, False),
-        ("dqkv", dqkv, torch.bfloat16, b * S * 3 * E, True), ("delta_ws", delta_ws, torch.float32, b * H * S, True),
-        ("lengths", lengths, torch.int32, b, False), ("keep_rows", keep_rows, torch.int32, words, False),
-        ("keep_cols", keep_cols, torch.int32, words, False), ("workspace", workspace, torch.float32, need, True))
+    n, words = b * S * H, attention_keep_words(b, S, H) if keep_rows is not None else 0
+    stream, (dq_, dl_, ws_, q_, o_, do_, l_, n_, kr_, kc_) = _operands(
+        what, ("dqkv", "delta_ws", "workspace", "qkv", "out", "dout", "lse", "lengths", "keep_rows", "keep_cols"), _RELBIAS_BWD_TYPES,
+        (dqkv, delta_ws, workspace, qkv, out, dout, lse, lengths, keep_rows, keep_cols), (n * 192, n, need, n * 192, n * 64, n * 64, n, b, words, words), 3)
     check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), max(dtable.stride(0), H), accumulate,
                                             dl_, _kept(ws_, workspace), workspace.numel(), b, S, H, scale, kr_, kc_, p, stream))
 
@@ -1498,6 +1519,10 @@ def _balance_shape(what, r, lengths):
     return B, S, E
 
 
+_BALANCE_FWD_TYPES = (torch.float32, torch.int32, torch.int32, torch.float32, torch.float32, torch.float32, torch.int32, torch.int32, torch.int32)
+_BALANCE_BWD_TYPES = (torch.float32, torch.float32, torch.int32, torch.int32, torch.float32, torch.int32, torch.int32)
+
+
 @functools.lru_cache(maxsize=256)
 def _balance_workspace_elems(B, S, E):
     need = ctypes.c_int64()
@@ -1517,11 +1542,10 @@ def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, leng
     _exactly(what, B * E, counts, kept, prob_sum)
     need = _balance_workspace_elems(B, S, E)
     workspace = _scratch(what, workspace, need, loss.device) if need else None
-    stream, (p_, i_, s_, n_, l_, c_, k_, ps_, ws_) = _operands(
-        what, ("probs", r["probs"], torch.float32, B * S * E, False), ("index", r["index"], torch.int32, B * S * 2, False),
-        ("slot", r["slot"], torch.int32, B * S * 2, False), ("lengths", lengths, torch.int32, B, False), ("loss", loss, torch.float32, 1, True),
-        ("counts", counts, torch.int32, B * E, True), ("kept", kept, torch.int32, B * E, True), ("prob_sum", prob_sum, torch.float32, B * E, True),
-        ("workspace", workspace, torch.float32, need, True))
+    n, m = B * E, B * S * 2
+    stream, (l_, c_, k_, ps_, ws_, p_, i_, s_, n_) = _operands(
+        what, ("loss", "counts", "kept", "prob_sum", "workspace", "probs", "index", "slot", "lengths"), _BALANCE_FWD_TYPES,
+        (loss, counts, kept, prob_sum, workspace, r["probs"], r["index"], r["slot"], lengths), (1, n, n, n, need, S * n, m, m, B), 5)
     check(lib().hapmi_balance_loss_fwd(p_, i_, s_, n_, l_, c_, k_, ps_, B, S, E, coef, choices, _kept(ws_, workspace),
                                        workspace.numel() if workspace is not None else 0, stream))
 
@@ -1532,10 +1556,10 @@ def balance_loss_bwd(r, counts, dlogits, choices=2, coef=0.01, grad=1.0, dgate=N
     what = "balance_loss_bwd"
     B, S, E = _balance_shape(what, r, lengths)
     _exactly(what, B * E, counts)
-    stream, (p_, i_, s_, g_, c_, n_, d_) = _operands(
-        what, ("probs", r["probs"], torch.float32, B * S * E, False), ("index", r["index"], torch.int32, B * S * 2, False),
-        ("slot", r["slot"], torch.int32, B * S * 2, False), ("dgate", dgate, torch.float32, B * S * 2, False),
-        ("counts", counts, torch.int32, B * E, False), ("lengths", lengths, torch.int32, B, False), ("dlogits", dlogits, torch.float32, B * S * E, True))
+    n, m = B * E, B * S * 2
+    stream, (d_, p_, i_, s_, g_, c_, n_) = _operands(
+        what, ("dlogits", "probs", "index", "slot", "dgate", "counts", "lengths"), _BALANCE_BWD_TYPES,
+        (dlogits, r["probs"], r["index"], r["slot"], dgate, counts, lengths), (S * n, S * n, m, m, m, n, B), 1)
     check(lib().hapmi_balance_loss_bwd(p_, i_, s_, g_, c_, n_, d_, B, S, E, coef * grad, choices, stream))
 
 
