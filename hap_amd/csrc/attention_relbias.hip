@@ -405,6 +405,22 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
         rel.expand<false, CAUSAL>(win, hh, scale);                    // this and the zeroed sums: published by the loop's first barrier
         // ds is kept without its factor `scale`; a query that sees nothing (lse = -inf) has p = 0
         const float sl2 = scale * LOG2E, nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
+        // dP - delta in the matrix pipe: a product of ones (every key row) and -delta_q cut into three bf16 terms, which hold all 24
+        // bits of it; one matrix instruction a block in place of 16 subtractions a lane
+        frag_t ones, minus_delta;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ones.v[e] = (bf16_t)1.f;
+            minus_delta.v[e] = (bf16_t)0.f;
+        }
+        if (h == 0) {
+            float rest = -delta_q;
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                minus_delta.v[e] = (bf16_t)rest;
+                rest -= (float)minus_delta.v[e];
+            }
+        }
         const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * ((S + TILE - 1) / TILE) * 2 + h : nullptr;
         uint32_t keep = 0xffffffffu, keep_next = 0xffffffffu;
         if constexpr (DROP) keep_next = keep_row[0];
@@ -441,9 +457,11 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                         st = mma(kf[s], qf[s], st);
                         dp = mma(vf[s], dof[s], dp);
                     }
-                    if constexpr (DROP) {
+                    if constexpr (DROP) {                     // (the mask is applied before delta is subtracted)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) dp[r] = (keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f;
+                        for (int r = 0; r < 16; ++r) dp[r] = ((keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f) - delta_q;
+                    } else {
+                        dp = mma(ones, minus_delta, dp);
                     }
                 };
                 if (whole && (far_hi || far_lo)) {            // one bucket for the whole block
@@ -453,7 +471,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                     float sum = 0.f;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, off)) * (dp[r] - delta_q);
+                        dp[r] *= __builtin_amdgcn_exp2f(fmaf(st[r], sl2, off));
                         sum += dp[r];
                     }
                     far_sum[far_hi ? 1 : 0] += sum;
@@ -467,7 +485,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                             if (k0 + acc_row(r, h) >= n) st[r] = -INFINITY;
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl)) * (dp[r] - delta_q);
+                    for (int r = 0; r < 16; ++r) dp[r] *= __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl));
                     // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
                     own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
                 }
@@ -520,11 +538,9 @@ __device__ __forceinline__ void table_gradient(const float *part, float *dtable,
     const int u = threadIdx.x % n_buckets, run = threadIdx.x / n_buckets, runs = AT_THREADS / n_buckets;
     if (run < runs) {
         float v = 0.f;
-        for (int z = 0; z < b; ++z) {
-            const float *p = part + ((int64_t)z * H + head) * row_blocks * n_buckets + u;
+        const int items = b * row_blocks;                     // (b H <= 65535 and row_blocks < 2^17: fits)
 #pragma unroll 8
-            for (int k = run; k < row_blocks; k += runs) v += p[(int64_t)k * n_buckets];
-        }
+        for (int i = run; i < items; i += runs) v += part[(((int64_t)(i / row_blocks) * H + head) * row_blocks + i % row_blocks) * n_buckets + u];
         red[threadIdx.x] = v;
     }
     __syncthreads();
