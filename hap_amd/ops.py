@@ -71,61 +71,58 @@ def _span(rows: int, cols: int, ld: int) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _operands(what, names, dtypes, tensors, elems, written):
-    """Checks of a call's tensors in one pass: on the current device, of the element type, contiguous, at least ``elems`` long,
-    and none of the first ``written`` ones shares memory with another.  None entries are skipped.  Returns the current
-    stream and the pointers (0 for None), in order."""
-    cur, ptrs, spans = -2, [], []
+def _operands(what, names, dtypes, tensors, elems, written, exact=()):
+    """Checks of a call's tensors in one pass: on the current device, of the element type, contiguous, at least ``elems`` long
+    (those named in ``exact``: just as long), and none of the first ``written`` ones shares memory with another.  None entries
+    are skipped, the first one is a tensor.  Returns the current stream and the pointers (0 for None), in order."""
+    ptrs, spans = [], []
+    cur = tensors[0].get_device()
+    if cur < 0 or cur != _current_device():
+        _dev(tensors[0])
+        raise _lib.HapmiError(f"{what}: {names[0]} is on {tensors[0].device}, not on the current device")
     for t, dtype, n in zip(tensors, dtypes, elems):
         if t is None:
             ptrs.append(0)
             continue
         size = t.numel()
-        if t.get_device() != cur or t.dtype is not dtype or not 0 <= n <= size or not t.is_contiguous():
-            cur = _odd_operand(what, names[len(ptrs)], t, dtype, n, cur)
+        if size != n or t.dtype is not dtype or t.get_device() != cur or not t.is_contiguous():
+            _odd_operand(what, names[len(ptrs)], t, dtype, n, cur, exact)
         ptr = t.data_ptr()
         if size:
             spans.append((ptr, ptr + size * _ITEM[dtype], len(ptrs) < written))
         ptrs.append(ptr)
-    _apart(what, spans)
+    spans.sort()
+    end = 0
+    for lo, hi, _ in spans:
+        if lo < end:                                                 # shared memory: allowed between operands that are only read
+            _apart(what, spans)
+            break
+        end = hi
     return _raw_stream(cur), ptrs
 
 
 _ITEM = {torch.float32: 4, torch.int32: 4, torch.bfloat16: 2}
 
 
-def _odd_operand(what, name, t, dtype, elems, cur):
-    """The first operand (whose device becomes the call's), or one that is refused."""
+def _odd_operand(what, name, t, dtype, elems, cur, exact):
+    """An operand that is longer than needed, or one that is refused."""
     if t.get_device() != cur:
         _dev(t)
-        if cur != -2 or t.get_device() != torch.cuda.current_device():
-            raise _lib.HapmiError(f"{what}: {name} is on {t.device}, not on the current device")
+        raise _lib.HapmiError(f"{what}: {name} is on {t.device}, not on the current device")
     if t.dtype is not dtype:
         raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    if name in exact and t.numel() != elems:
+        raise TypeError(f"{what}: {name} must have {elems} elements, not {t.numel()}")
     _need(t, elems, f"{what} {name}")
-    return t.get_device()
-
-
-def _exactly(what, n, *tensors):
-    for t in tensors:
-        if t is not None and t.numel() != n:
-            raise TypeError(f"{what}: {n} elements expected in place of {t.numel()}")
 
 
 def _apart(what, spans):
     """No (start, end, written) range that is written may overlap another one."""
-    spans.sort()
-    end = 0
-    for lo, hi, _ in spans:
-        if lo < end:
-            break
-        end = hi
-    else:
-        return
     end = end_written = 0
-    for lo, hi, written in spans:
+    for lo, hi, written in sorted(spans):
         if lo < end_written or (written and lo < end):
             raise ValueError(f"{what}: an output shares memory with another operand")
         end = max(end, hi)
@@ -868,13 +865,19 @@ def rotary_table(n_positions: int, rot: int, base: float = 10000.0, device=None)
 
 def _head_dim(what, qkv, b, S, H, rotary):
     """Head dimension of the packed projection, and (positions, rotated dimensions) of the angle table."""
-    if b < 0 or S < 1 or H < 1 or qkv.dim() != 3 or qkv.shape[0] != b or qkv.shape[1] != S or qkv.shape[2] % (3 * H):
+    shape = qkv.shape
+    if len(shape) != 3 or b < 0 or S < 1 or H < 1 or shape[0] != b or shape[1] != S or shape[2] % (3 * H):
         raise ValueError(f"{what}: a packed projection [b, S, 3 * H * head_dim] expected")
     if rotary is None:
-        return qkv.shape[2] // (3 * H), 0, 0
-    if rotary.dim() != 3 or rotary.shape[2] != 2:
+        return shape[2] // (3 * H), 0, 0
+    table = rotary.shape
+    if len(table) != 3 or table[2] != 2:
         raise TypeError(f"{what}: the angle table must be a float32 [positions, rot / 2, 2] tensor")
-    return qkv.shape[2] // (3 * H), rotary.shape[0], 2 * rotary.shape[1]
+    return shape[2] // (3 * H), table[0], 2 * table[1]
+
+
+_QK_FWD_EXACT = ("out", "q_gain", "k_gain", "positions")
+_QK_BWD_EXACT = ("dqkv", "dout", "q_gain", "k_gain", "dq_gain", "dk_gain", "positions")
 
 
 def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None, positions=None, interleaved=False, eps=1e-6):
@@ -884,16 +887,12 @@ def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None,
     inside the sequence); one outside the table gives NaN.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
     what = "qk_norm_rotary_fwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
-    _exactly(what, D, q_gain, k_gain)
-    _exactly(what, b * S, positions)
     code, n = dtype_code(qkv), b * S * 3 * H * D
-    if out.numel() != n:
-        raise ValueError(f"{what}: out must have qkv's size")
     apart = out.data_ptr() != qkv.data_ptr()
     dt = qkv.dtype
     stream, (o_, x_, q_, k_, r_, p_) = _operands(
         what, ("out", "qkv", "q_gain", "k_gain", "rotary", "positions"), (dt, dt, torch.float32, torch.float32, torch.float32, torch.int32),
-        (out, qkv if apart else None, q_gain, k_gain, rotary, positions), (n, n, D, D, n_pos * rot, b * S), 1)
+        (out, qkv if apart else None, q_gain, k_gain, rotary, positions), (n, n, D, D, n_pos * rot, b * S), 1, _QK_FWD_EXACT)
     check(lib().hapmi_qk_norm_rotary_fwd(x_ if apart else o_, o_, q_, k_, r_, n_pos, rot, interleaved, p_, b, S, H, D, eps, code, stream))
 
 
@@ -911,10 +910,7 @@ def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_ga
     ``qkv``; ``dq_gain`` / ``dk_gain`` float32 [head_dim] (None: not wanted; ``accumulate``: added to)."""
     what = "qk_norm_rotary_bwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
-    _exactly(what, D, q_gain, k_gain, dq_gain, dk_gain)
-    _exactly(what, b * S, positions)
     code, n, ws_elems = dtype_code(qkv), b * S * 3 * H * D, 0
-    _exactly(what, n, dout, dqkv)
     if dq_gain is not None or dk_gain is not None:
         ws_elems = qk_norm_rotary_workspace_elems(D)
         workspace = _scratch(what, workspace, ws_elems, qkv.device)
@@ -926,9 +922,7 @@ def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_ga
         what, ("dqkv", "dq_gain", "dk_gain", "workspace", "dout", "qkv", "q_gain", "k_gain", "rotary", "positions"),
         (dt, f32, f32, f32, dt, dt, f32, f32, f32, torch.int32),
         (dqkv, dq_gain, dk_gain, workspace, dout if apart else None, qkv, q_gain, k_gain, rotary, positions),
-        (n, D, D, ws_elems, n, n, D, D, n_pos * rot, b * S), 4)
-    if not apart and dout.dtype is not qkv.dtype:
-        raise TypeError(f"{what}: dtype mismatch")
+        (n, D, D, ws_elems, n, n, D, D, n_pos * rot, b * S), 4, _QK_BWD_EXACT)
     check(lib().hapmi_qk_norm_rotary_bwd(do_ if apart else dx_, x_, dx_, q_, k_, dq_, dk_, accumulate, r_, n_pos, rot, interleaved, p_, b, S, H, D,
                                          eps, code, _kept(ws_, workspace), workspace.numel() if workspace is not None else 0, stream))
 
@@ -1091,10 +1085,9 @@ def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128
     batch; rows behind a sequence's end get zeros and lse = -inf, its keys there are not read.  ``keep_rows`` / ``p``:
     dropout of the probabilities, as in ``attention_fwd``."""
     what = "attention_relbias_fwd"
-    _exactly(what, b, lengths)
     n = b * S * H
     stream, (o_, l_, q_, n_, k_) = _operands(what, ("out", "lse", "qkv", "lengths", "keep_rows"), _RELBIAS_FWD_TYPES, (out, lse, qkv, lengths, keep_rows),
-                                             (n * 64, n, n * 192, b, attention_keep_words(b, S, H) if keep_rows is not None else 0), 2)
+                                             (n * 64, n, n * 192, b, attention_keep_words(b, S, H) if keep_rows is not None else 0), 2, ("lengths",))
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
     _on_device(what, table, qkv)
     check(lib().hapmi_attention_relbias_fwd(q_, ctypes.byref(rel), causal, n_, o_, l_, b, S, H, scale, k_, p, stream))
@@ -1127,7 +1120,6 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     ``accumulate``: added to, for a table that several layers share).  ``out`` and ``lse`` as forward left them.
     ``workspace``: float32 scratch of ``attention_relbias_workspace_elems`` (None: taken from torch's allocator)."""
     what = "attention_relbias_bwd"
-    _exactly(what, b, lengths)
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
     if dtable.shape != table.shape or dtable.dtype != torch.float32 or (H > 1 and dtable.stride(1) != 1):
         raise ValueError(f"{what}: dtable must be float32 of the table's shape with unit column stride")
@@ -1141,7 +1133,7 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     n, words = b * S * H, attention_keep_words(b, S, H) if keep_rows is not None else 0
     stream, (dq_, dl_, ws_, q_, o_, do_, l_, n_, kr_, kc_) = _operands(
         what, ("dqkv", "delta_ws", "workspace", "qkv", "out", "dout", "lse", "lengths", "keep_rows", "keep_cols"), _RELBIAS_BWD_TYPES,
-        (dqkv, delta_ws, workspace, qkv, out, dout, lse, lengths, keep_rows, keep_cols), (n * 192, n, need, n * 192, n * 64, n * 64, n, b, words, words), 3)
+        (dqkv, delta_ws, workspace, qkv, out, dout, lse, lengths, keep_rows, keep_cols), (n * 192, n, need, n * 192, n * 64, n * 64, n, b, words, words), 3, ("lengths",))
     check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), max(dtable.stride(0), H), accumulate,
                                             dl_, _kept(ws_, workspace), workspace.numel(), b, S, H, scale, kr_, kc_, p, stream))
 
@@ -1511,12 +1503,7 @@ def top2_gate_bwd(r, dgate, dlogits):
                                     B, S, E, _stream()))
 
 
-def _balance_shape(what, r, lengths):
-    if r["probs"].dim() != 3:
-        raise ValueError(f"{what}: probabilities [B, S, E] expected")
-    B, S, E = r["probs"].shape
-    _exactly(what, B, lengths)
-    return B, S, E
+_BALANCE_EXACT = ("loss", "counts", "kept", "prob_sum", "lengths")
 
 
 _BALANCE_FWD_TYPES = (torch.float32, torch.int32, torch.int32, torch.float32, torch.float32, torch.float32, torch.int32, torch.int32, torch.int32)
@@ -1537,15 +1524,14 @@ def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, leng
     loss = coef * E * mean over the rows of sum_e counts / (choices * n) * prob_sum / n, n the row's tokens: all S, or
     ``lengths`` (int32 [B]) of a padded batch (empty rows do not enter the mean).  Perfectly even routing gives coef."""
     what = "balance_loss_fwd"
-    B, S, E = _balance_shape(what, r, lengths)
-    _exactly(what, 1, loss)
-    _exactly(what, B * E, counts, kept, prob_sum)
+    probs = r["probs"]
+    B, S, E = probs.shape
     need = _balance_workspace_elems(B, S, E)
     workspace = _scratch(what, workspace, need, loss.device) if need else None
     n, m = B * E, B * S * 2
     stream, (l_, c_, k_, ps_, ws_, p_, i_, s_, n_) = _operands(
         what, ("loss", "counts", "kept", "prob_sum", "workspace", "probs", "index", "slot", "lengths"), _BALANCE_FWD_TYPES,
-        (loss, counts, kept, prob_sum, workspace, r["probs"], r["index"], r["slot"], lengths), (1, n, n, n, need, S * n, m, m, B), 5)
+        (loss, counts, kept, prob_sum, workspace, probs, r["index"], r["slot"], lengths), (1, n, n, n, need, S * n, m, m, B), 5, _BALANCE_EXACT)
     check(lib().hapmi_balance_loss_fwd(p_, i_, s_, n_, l_, c_, k_, ps_, B, S, E, coef, choices, _kept(ws_, workspace),
                                        workspace.numel() if workspace is not None else 0, stream))
 
@@ -1554,12 +1540,12 @@ def balance_loss_bwd(r, counts, dlogits, choices=2, coef=0.01, grad=1.0, dgate=N
     """Gradient of ``grad`` times the balance loss with respect to the router's logits, from forward's ``counts``; with
     ``dgate`` (float32 [B, S, 2]) ``dlogits`` also holds what ``top2_gate_bwd`` gives for it, in the same pass."""
     what = "balance_loss_bwd"
-    B, S, E = _balance_shape(what, r, lengths)
-    _exactly(what, B * E, counts)
+    probs = r["probs"]
+    B, S, E = probs.shape
     n, m = B * E, B * S * 2
     stream, (d_, p_, i_, s_, g_, c_, n_) = _operands(
         what, ("dlogits", "probs", "index", "slot", "dgate", "counts", "lengths"), _BALANCE_BWD_TYPES,
-        (dlogits, r["probs"], r["index"], r["slot"], dgate, counts, lengths), (S * n, S * n, m, m, m, n, B), 1)
+        (dlogits, probs, r["index"], r["slot"], dgate, counts, lengths), (S * n, S * n, m, m, m, n, B), 1, _BALANCE_EXACT)
     check(lib().hapmi_balance_loss_bwd(p_, i_, s_, g_, c_, n_, d_, B, S, E, coef * grad, choices, stream))
 
 
