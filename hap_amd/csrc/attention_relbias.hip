@@ -26,6 +26,9 @@
 
 namespace {
 
+// pins the order of what stands before and behind it
+#define PIN __builtin_amdgcn_sched_barrier(0)
+
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int REL_MAX_SIDE = HAPMI_RELBIAS_MAX_SIDE;
 constexpr int REL_MAX_REACH = HAPMI_RELBIAS_MAX_REACH;
@@ -444,6 +447,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                 const bool whole = k0 + 32 <= n;
                 const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;
                 f32x16 st, dp = zero16();
+                frag_t db[2];
                 frag_t kf[4], vf[4];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
@@ -475,6 +479,8 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                         sum += dp[r];
                     }
                     far_sum[far_hi ? 1 : 0] += sum;
+                    db[0] = acc_to_b(dp, 0);
+                    db[1] = acc_to_b(dp, 1);
                 } else {
                     const int at = rel.at<32>(D, c, h);
                     st = bias_tile(win + at);
@@ -486,14 +492,16 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                     }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) dp[r] *= __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl));
+                    db[0] = acc_to_b(dp, 0);
+                    db[1] = acc_to_b(dp, 1);
+                    asm volatile("" : "+v"(db[0].v), "+v"(db[1].v));      // rounded here: the sums below then need no copies of dp
                     // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
                     own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
                 }
 #pragma unroll
                 for (int sp = 0; sp < 2; ++sp) {
-                    const frag_t db = acc_to_b(dp, sp);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) dqt[u] = mma(tr.frag(Ks, u * 32, t * 2 + sp), db, dqt[u]);
+                    for (int u = 0; u < 2; ++u) dqt[u] = mma(tr.frag(Ks, u * 32, t * 2 + sp), db[sp], dqt[u]);
                 }
             }
         }
@@ -561,7 +569,6 @@ __device__ __forceinline__ void table_gradient(const float *part, float *dtable,
 // vector instructions of this block (the order is pinned), three tiles are kept in LDS because the next block may be the next
 // tile's.  Everything that would be a branch a block is data: causally hidden pairs are -inf in the bias window, queries
 // beyond the end carry lse = +inf, and dP starts from -delta.
-#define PIN __builtin_amdgcn_sched_barrier(0)
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *dout,
                                                                    const float *lse, const float *delta, bf16_t *dqkv,
