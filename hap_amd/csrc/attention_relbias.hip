@@ -635,156 +635,190 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
         int buf = 0, nbuf = 1;
         if (q_begin + TILE < n) fetch(q_begin + TILE, 1);
 
-        f32x16 sc0, dp0, sc1, dp1;
-        frag_t qa[4], da[4];
-        auto read_frag = [&](int bufi, int t, int s) {
-            qa[s] = frag_rowk(Qs3[bufi], t * 32 + c, s, h);
-            da[s] = frag_rowk(dOs3[bufi], t * 32 + c, s, h);
-        };
-        // a block's accumulators before its products: the bias, -delta
-        auto read_start = [&](int bufi, int t, int q0, f32x16 &x, f32x16 &y) {
-            x = bias_tile(win + rel.at<32>(q0 + t * 32 - kvw, c, h));
-            if constexpr (DROP) y = zero16();
-            else {
+        // sixteen row values of a lane's block, in register order
+        auto row_values = [&](const float *rows, int t) {
+            f32x16 y;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 d4 = *(const f32x4 *)(delta_s[bufi] + t * 32 + g * 8 + h * 4);
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 r4 = *(const f32x4 *)(rows + t * 32 + g * 8 + h * 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[g * 4 + e] = d4[e];
-                }
+                for (int e = 0; e < 4; ++e) y[g * 4 + e] = r4[e];
             }
+            return y;
         };
-        // P, dS, dV, dK of block (cbuf, t) whose scores and dP - delta are in (sc, dp), and the scores of block (nb, nt) of the
-        // query tile at nq0 into (xs, xd).  Behind the last block that is some old tile's data, whose result nobody uses.
-        f32x4 l4, d4, l4n, d4n;                               // row statistics of the four rows being worked on, and of the next four
-        auto stats = [&](int cbuf, int t, int g, f32x4 &l, f32x4 &d) {
-            l = *(const f32x4 *)(lse_s[cbuf] + t * 32 + h * 4 + g * 8);
-            if constexpr (DROP) d = *(const f32x4 *)(delta_s[cbuf] + t * 32 + h * 4 + g * 8);
-        };
-        // first reads for block (cbuf, t) and for the scores of block (nb, nt), issued behind the products of the block before
-        auto prepare = [&](f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt, int nq0) {
-            stats(cbuf, t, 0, l4, d4);
-            stats(cbuf, t, 1, l4n, d4n);
-            read_start(nb, nt, nq0, xs, xd);
-            read_frag(nb, nt, 0);
-            read_frag(nb, nt, 1);
-            PIN;
-        };
-        auto block = [&](f32x16 &sc, f32x16 &dp, f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt) {
-            const char *Qs = Qs3[cbuf], *dOs = dOs3[cbuf];
-            const uint32_t keep = t ? keep2.y : keep2.x;
-            auto score = [&](int r) {                         // P and dS of score register r
-                const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, -l4[r & 3]));
-                if constexpr (DROP) {
-                    const bool kp = keep & (1u << acc_row(r, h));
-                    dp[r] = p * ((kp ? dp[r] * keep_scale : 0.f) - d4[r & 3]);
-                    sc[r] = kp ? p * keep_scale : 0.f;
-                } else {
+        if constexpr (DROP) {
+            // The mask keeps delta out of the products and needs the keep words, and the pinned order below then spills (backward of
+            // [12, 512] x 16 heads with dropout: 134 us with it, 102 us with these plain blocks).
+            for (int q0 = q_begin; q0 < n; q0 += TILE) {
+                const char *Qs = Qs3[buf], *dOs = dOs3[buf];
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t) {
+                    if (kvw >= n || q0 + t * 32 >= n || (CAUSAL && q0 + t * 32 + 31 < kvw)) continue;
+                    f32x16 sc = bias_tile(win + rel.at<32>(q0 + t * 32 - kvw, c, h)), dp = zero16();
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        sc = mma(frag_rowk(Qs, t * 32 + c, s, h), kf[s], sc);
+                        dp = mma(frag_rowk(dOs, t * 32 + c, s, h), vf[s], dp);
+                    }
+                    const uint32_t keep = t ? keep2.y : keep2.x;
+                    const f32x16 l = row_values(lse_s[buf], t), d = row_values(delta_s[buf], t);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, -l[r]));
+                        const bool kp = keep & (1u << acc_row(r, h));
+                        dp[r] = p * ((kp ? dp[r] * keep_scale : 0.f) - d[r]);
+                        sc[r] = kp ? p * keep_scale : 0.f;
+                    }
+#pragma unroll
+                    for (int sp = 0; sp < 2; ++sp) {
+                        const frag_t pb = acc_to_b(sc, sp), db = acc_to_b(dp, sp);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            dvt[u] = mma(tr.frag(dOs, u * 32, t * 2 + sp), pb, dvt[u]);
+                            dkt[u] = mma(tr.frag(Qs, u * 32, t * 2 + sp), db, dkt[u]);
+                        }
+                    }
+                }
+                const int fbuf = nbuf == NST - 1 ? 0 : nbuf + 1;
+                if (q0 + TILE < n) {
+                    stage(nbuf);
+                    keep2 = keep2_next;
+                }
+                __builtin_amdgcn_s_waitcnt(0x0F70);           // vmcnt(0): the next tile has landed
+                __syncthreads();                              // for everybody, and everybody is done with the tile before this one
+                if (q0 + 2 * TILE < n) fetch(q0 + 2 * TILE, fbuf);
+                buf = nbuf;
+                nbuf = fbuf;
+            }
+        } else {
+            f32x16 sc0, dp0, sc1, dp1;
+            frag_t qa[4], da[4];
+            auto read_frag = [&](int bufi, int t, int s) {
+                qa[s] = frag_rowk(Qs3[bufi], t * 32 + c, s, h);
+                da[s] = frag_rowk(dOs3[bufi], t * 32 + c, s, h);
+            };
+            // a block's accumulators before its products: the bias, -delta
+            auto read_start = [&](int bufi, int t, int q0, f32x16 &x, f32x16 &y) {
+                x = bias_tile(win + rel.at<32>(q0 + t * 32 - kvw, c, h));
+                y = row_values(delta_s[bufi], t);
+            };
+            // P, dS, dV, dK of block (cbuf, t) whose scores and dP - delta are in (sc, dp), and the scores of block (nb, nt) of the
+            // query tile at nq0 into (xs, xd).  Behind the last block that is some old tile's data, whose result nobody uses.
+            f32x4 l4, l4n;                                        // log-sum-exps of the four rows being worked on, and of the next four
+            auto stats = [&](int cbuf, int t, int g) { return *(const f32x4 *)(lse_s[cbuf] + t * 32 + h * 4 + g * 8); };
+            // first reads for block (cbuf, t) and for the scores of block (nb, nt), issued behind the products of the block before
+            auto prepare = [&](f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt, int nq0) {
+                l4 = stats(cbuf, t, 0);
+                l4n = stats(cbuf, t, 1);
+                read_start(nb, nt, nq0, xs, xd);
+                read_frag(nb, nt, 0);
+                read_frag(nb, nt, 1);
+                PIN;
+            };
+            auto block = [&](f32x16 &sc, f32x16 &dp, f32x16 &xs, f32x16 &xd, int cbuf, int t, int nb, int nt) {
+                const char *Qs = Qs3[cbuf], *dOs = dOs3[cbuf];
+                auto score = [&](int r) {                         // P and dS of score register r
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, -l4[r & 3]));
                     dp[r] = p * dp[r];
                     sc[r] = p;
+                };
+                auto next_scores = [&](int s) { xs = mma(qa[s], kf[s], xs); };
+                auto next_dp = [&](int s) { xd = mma(da[s], vf[s], xd); };
+#pragma unroll
+                for (int r = 0; r < 4; ++r) score(r);
+                l4 = l4n;
+                l4n = stats(cbuf, t, 2);
+                PIN;
+                next_scores(0);
+                PIN;
+                score(4);
+                score(5);
+                PIN;
+                next_dp(0);
+                PIN;
+                score(6);
+                score(7);
+                frag_t pb = acc_to_b(sc, 0), db = acc_to_b(dp, 0), dt[2], qt[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    dt[u] = tr.frag(dOs, u * 32, t * 2);
+                    qt[u] = tr.frag(Qs, u * 32, t * 2);
                 }
+                l4 = l4n;
+                l4n = stats(cbuf, t, 3);
+                read_frag(nb, nt, 2);
+                PIN;
+                next_scores(1);
+                PIN;
+                score(8);
+                PIN;
+                next_dp(1);
+                PIN;
+                score(9);
+                read_frag(nb, nt, 3);
+                PIN;
+                dvt[0] = mma(dt[0], pb, dvt[0]);
+                PIN;
+                score(10);
+                PIN;
+                dkt[0] = mma(qt[0], db, dkt[0]);
+                dt[0] = tr.frag(dOs, 0, t * 2 + 1);
+                qt[0] = tr.frag(Qs, 0, t * 2 + 1);
+                PIN;
+                score(11);
+                l4 = l4n;
+                PIN;
+                next_scores(2);
+                PIN;
+                score(12);
+                PIN;
+                dvt[1] = mma(dt[1], pb, dvt[1]);
+                PIN;
+                score(13);
+                PIN;
+                dkt[1] = mma(qt[1], db, dkt[1]);
+                dt[1] = tr.frag(dOs, 32, t * 2 + 1);
+                qt[1] = tr.frag(Qs, 32, t * 2 + 1);
+                PIN;
+                score(14);
+                PIN;
+                next_dp(2);
+                PIN;
+                score(15);
+                pb = acc_to_b(sc, 1);
+                db = acc_to_b(dp, 1);
+                PIN;
+                next_scores(3);
+                next_dp(3);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    dvt[u] = mma(dt[u], pb, dvt[u]);
+                    dkt[u] = mma(qt[u], db, dkt[u]);
+                }
+                PIN;
             };
-            auto next_scores = [&](int s) { xs = mma(qa[s], kf[s], xs); };
-            auto next_dp = [&](int s) { xd = mma(da[s], vf[s], xd); };
+            read_start(0, 0, q_begin, sc0, dp0);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) score(r);
-            l4 = l4n; d4 = d4n;
-            stats(cbuf, t, 2, l4n, d4n);
-            PIN;
-            next_scores(0);
-            PIN;
-            score(4);
-            score(5);
-            PIN;
-            next_dp(0);
-            PIN;
-            score(6);
-            score(7);
-            frag_t pb = acc_to_b(sc, 0), db = acc_to_b(dp, 0), dt[2], qt[2];
+            for (int s = 0; s < 4; ++s) read_frag(0, 0, s);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                dt[u] = tr.frag(dOs, u * 32, t * 2);
-                qt[u] = tr.frag(Qs, u * 32, t * 2);
+            for (int s = 0; s < 4; ++s) {
+                sc0 = mma(qa[s], kf[s], sc0);
+                dp0 = mma(da[s], vf[s], dp0);
             }
-            l4 = l4n; d4 = d4n;
-            stats(cbuf, t, 3, l4n, d4n);
-            read_frag(nb, nt, 2);
-            PIN;
-            next_scores(1);
-            PIN;
-            score(8);
-            PIN;
-            next_dp(1);
-            PIN;
-            score(9);
-            read_frag(nb, nt, 3);
-            PIN;
-            dvt[0] = mma(dt[0], pb, dvt[0]);
-            PIN;
-            score(10);
-            PIN;
-            dkt[0] = mma(qt[0], db, dkt[0]);
-            dt[0] = tr.frag(dOs, 0, t * 2 + 1);
-            qt[0] = tr.frag(Qs, 0, t * 2 + 1);
-            PIN;
-            score(11);
-            l4 = l4n; d4 = d4n;
-            PIN;
-            next_scores(2);
-            PIN;
-            score(12);
-            PIN;
-            dvt[1] = mma(dt[1], pb, dvt[1]);
-            PIN;
-            score(13);
-            PIN;
-            dkt[1] = mma(qt[1], db, dkt[1]);
-            dt[1] = tr.frag(dOs, 32, t * 2 + 1);
-            qt[1] = tr.frag(Qs, 32, t * 2 + 1);
-            PIN;
-            score(14);
-            PIN;
-            next_dp(2);
-            PIN;
-            score(15);
-            pb = acc_to_b(sc, 1);
-            db = acc_to_b(dp, 1);
-            PIN;
-            next_scores(3);
-            next_dp(3);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                dvt[u] = mma(dt[u], pb, dvt[u]);
-                dkt[u] = mma(qt[u], db, dkt[u]);
+            prepare(sc1, dp1, 0, 0, 0, 1, q_begin);
+            for (int q0 = q_begin; q0 < n; q0 += TILE) {
+                block(sc0, dp0, sc1, dp1, buf, 0, buf, 1);
+                const int fbuf = nbuf == NST - 1 ? 0 : nbuf + 1;
+                if (q0 + TILE < n) stage(nbuf);
+                __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the next tile has landed
+                __syncthreads();                                  // for everybody, and everybody is done with the tile before this one
+                if (q0 + 2 * TILE < n) fetch(q0 + 2 * TILE, fbuf);
+                prepare(sc0, dp0, buf, 1, nbuf, 0, q0 + TILE);
+                block(sc1, dp1, sc0, dp0, buf, 1, nbuf, 0);
+                prepare(sc1, dp1, nbuf, 0, nbuf, 1, q0 + TILE);
+                buf = nbuf;
+                nbuf = fbuf;
             }
-            PIN;
-        };
-        read_start(0, 0, q_begin, sc0, dp0);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) read_frag(0, 0, s);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            sc0 = mma(qa[s], kf[s], sc0);
-            dp0 = mma(da[s], vf[s], dp0);
-        }
-        prepare(sc1, dp1, 0, 0, 0, 1, q_begin);
-        for (int q0 = q_begin; q0 < n; q0 += TILE) {
-            block(sc0, dp0, sc1, dp1, buf, 0, buf, 1);
-            const int fbuf = nbuf == NST - 1 ? 0 : nbuf + 1;
-            u32x2 keep_after = keep2;
-            if (q0 + TILE < n) {
-                stage(nbuf);
-                if constexpr (DROP) keep_after = keep2_next;
-            }
-            __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the next tile has landed
-            __syncthreads();                                  // for everybody, and everybody is done with the tile before this one
-            if (q0 + 2 * TILE < n) fetch(q0 + 2 * TILE, fbuf);
-            prepare(sc0, dp0, buf, 1, nbuf, 0, q0 + TILE);
-            block(sc1, dp1, sc0, dp0, buf, 1, nbuf, 0);
-            prepare(sc1, dp1, nbuf, 0, nbuf, 1, q0 + TILE);
-            if constexpr (DROP) keep2 = keep_after;
-            buf = nbuf;
-            nbuf = fbuf;
         }
     }
     if (kv < S) {

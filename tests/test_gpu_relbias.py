@@ -67,6 +67,7 @@ def compare(res, qkv, table, dout, H, max_distance, bidirectional, causal, lengt
 
 
 CASES = [  # b, S, H, buckets, max_distance, bidirectional, causal
+    (1, 50, 2, 2, 5, True, False),
     (1, 1, 1, 2, 2, False, False), (2, 2, 3, 4, 2, True, False), (1, 31, 2, 8, 20, True, False), (1, 32, 2, 32, 128, False, True),
     (2, 33, 1, 32, 128, True, False), (1, 63, 3, 6, 9, True, True), (1, 64, 2, 32, 128, True, False), (1, 65, 2, 5, 17, False, True),
     (2, 127, 2, 48, 300, True, False), (1, 128, 5, 32, 128, False, True), (1, 129, 1, 2, 2, False, True), (1, 200, 4, 32, 128, False, False),
