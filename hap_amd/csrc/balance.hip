@@ -177,7 +177,7 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_bwd_kernel(const float *p
             for (int k = 0; k < 2; ++k) g[i] += at[t][k] == e0 + i ? dg[t][k] : 0.f;
             dot += p[t][i] * g[i];
         }
-        for (int o = 0; o < group_log2; ++o) dot += __shfl_xor(dot, 1 << o, 64);
+        dot = group_sum(dot, group_log2);
         if (s >= S || e0 >= E) continue;
         if (V == 4) {
             f32x4 x;

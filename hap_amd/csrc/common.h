@@ -70,6 +70,21 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// sum over an aligned group of 2^group_log2 <= 64 lanes, in every lane: exchanges inside a row of 16 lanes ride on the additions
+// (DPP: neighbours, pairs, then mirrors, whose lanes hold equal sums), the last two cross rows
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float group_sum(float v, int group_log2) {
+    if (group_log2 > 0) v = dpp_add<0xb1>(v);              // quad_perm [1, 0, 3, 2]
+    if (group_log2 > 1) v = dpp_add<0x4e>(v);              // quad_perm [2, 3, 0, 1]
+    if (group_log2 > 2) v = dpp_add<0x141>(v);             // row_half_mirror
+    if (group_log2 > 3) v = dpp_add<0x140>(v);             // row_mirror
+    if (group_log2 > 4) v += __shfl_xor(v, 16, 64);
+    if (group_log2 > 5) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
 // block-wide reductions for blocks of up to 1024 threads (16 waves); `red` is 16 floats of LDS
 __device__ __forceinline__ float block_sum(float v, float *red) {
     v = wave_sum(v);

@@ -136,20 +136,6 @@ template <int V> __device__ __forceinline__ void qn_gain(const float *g, const Q
     }
 }
 
-// sum over an aligned group of 2^group_log2 <= 32 lanes, in every lane: exchanges inside a row of 16 lanes ride on the additions
-// (DPP: neighbours, pairs, then mirrors, whose lanes hold equal sums), the last one swaps rows
-template <int CTRL> __device__ __forceinline__ float qn_dpp_add(float v) {
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-__device__ __forceinline__ float qn_group_sum(float v, int group_log2) {
-    if (group_log2 > 0) v = qn_dpp_add<0xb1>(v);              // quad_perm [1, 0, 3, 2]
-    if (group_log2 > 1) v = qn_dpp_add<0x4e>(v);              // quad_perm [2, 3, 0, 1]
-    if (group_log2 > 2) v = qn_dpp_add<0x141>(v);             // row_half_mirror
-    if (group_log2 > 3) v = qn_dpp_add<0x140>(v);             // row_mirror
-    if (group_log2 > 4) v += __shfl_xor(v, 16, 64);
-    return v;
-}
-
 // A position outside the table poisons the token's rotated heads instead of reading beyond it (as an id outside an
 // embedding table does).
 __device__ __forceinline__ int64_t qn_position(const QnArgs &p, int64_t token, bool &bad) {
@@ -194,7 +180,7 @@ __global__ __launch_bounds__(QN_THREADS) void qk_norm_rotary_fwd_kernel(const Qn
                 b[e] = x[t].b.get(e);
                 sq += a[e] * a[e] + b[e] * b[e];
             }
-            sq = qn_group_sum(sq, p.group_log2);
+            sq = group_sum(sq, p.group_log2);
             const float r = bad ? NAN : 1.0f / sqrtf(sq / p.D + p.eps);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -262,7 +248,7 @@ __global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const
                 db[e] = d[t].b.get(e);
                 sq += a[e] * a[e] + b[e] * b[e];
             }
-            sq = qn_group_sum(sq, p.group_log2);
+            sq = group_sum(sq, p.group_log2);
             const float r = bad ? NAN : 1.0f / sqrtf(sq / p.D + p.eps);
             if (l.turn_a || l.turn_b) qn_turn<V>(p, l, w, -1.f, da, db);
             asm volatile("" ::: "memory");                    // (the gains are not to be hoisted into registers)
@@ -279,7 +265,7 @@ __global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const
                 db[e] *= gains[t][gb + e];
                 dot += da[e] * a[e] + db[e] * b[e];
             }
-            dot = qn_group_sum(dot, p.group_log2) / p.D;
+            dot = group_sum(dot, p.group_log2) / p.D;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 x[t].a.set(e, r * (da[e] - a[e] * dot));
