@@ -119,6 +119,33 @@ struct TileStream {
     }
 };
 
+// The wave's own 32 rows of 64, the operand that stays in its registers, come through LDS as well: a transfer reads whole 128-byte
+// rows, where a fragment read from memory touches 32 bytes of 32 rows.  The wave waits for its transfers (vmcnt) and needs no
+// barrier.  Rows from `rows` on repeat the last one, and are replaced by zeros when they are read.
+__device__ __forceinline__ void issue_own_rows(const bf16_t *first_row, int ld, int rows, char *lds) {
+    typedef __attribute__((address_space(3))) char lds_char;
+    if (rows <= 0) return;
+    const int lane = threadIdx.x & 63;
+    const uint32_t lds_addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char *)lds);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 3);
+        const int off = (r < rows ? r : rows - 1) * ld * 2 + ((lane & 7) ^ aswz(r)) * 16;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(lds_addr + i * 1024), "v"(off), "s"(first_row)
+                     : "memory");
+    }
+}
+__device__ __forceinline__ void own_frags(const char *lds, int c, int h, bool valid, frag_t (&f)[4]) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        f[s] = frag_rowk(lds, c, s, h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[s].v[e] = valid ? f[s].v[e] : (bf16_t)0.f;
+    }
+}
+
 // initial accumulator of a 32 x 32 score block: rows of the block are runs of four words
 __device__ __forceinline__ f32x16 bias_tile(const float *w) {
     f32x16 a;
@@ -220,7 +247,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
     __shared__ __attribute__((aligned(16))) char Ks3[NST][TILE_BYTES];
     __shared__ __attribute__((aligned(16))) char Vs3[NST][TILE_BYTES];
     __shared__ __attribute__((aligned(16))) uint32_t keep_s[DROP ? NST : 1][AT_THREADS];
-    extern __shared__ float win[];
+    extern __shared__ __attribute__((aligned(16))) float win[];
     const TransposedReader tr;
     const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
@@ -249,15 +276,15 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
             ldr.issue(V + (int64_t)kv0 * ld, n - kv0, Vs3[bufi]);
             if constexpr (DROP) issue_word(keep_row + (kv0 / TILE) * 2, &keep_s[bufi][0]);
         };
+        // the queries come through the third stage, which takes its first tile behind the loop's first barrier
+        char *own = (wave < 2 ? Ks3[2] : Vs3[2]) + (wave & 1) * 4096;
+        issue_own_rows(Q + (int64_t)qw * ld, ld, n - qw, own);
         issue_tile(0, 0);
+        rel.expand<false, CAUSAL>(win, hh, scale);            // published by the first barrier of the loop
+        __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): queries and first tile have landed
         if (TILE < kv_end) issue_tile(TILE, 1);
         frag_t qf[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) qf[s] = load_row_frag(Q + (int64_t)q * ld, q < n, s, h);
-        rel.expand<false, CAUSAL>(win, hh, scale);                    // published by the first barrier of the loop
-        // consumed before the loop, so that the wait for these loads is not one for all transfers in every iteration
-#pragma unroll
-        for (int s = 0; s < 4; ++s) asm volatile("" : "+v"(qf[s].v));
+        own_frags(own, c, h, q < n, qf);
         int buf = 0;
         for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
             if (kv0 + TILE < kv_end) __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | PER_TILE);   // vmcnt: only the next tile may be outstanding
@@ -367,6 +394,10 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // ---------------------------------------------------------------------------------------------
 // dQ and the bias gradient: lanes own query columns, kv tiles are streamed
 // ---------------------------------------------------------------------------------------------
+// words of a window and of the sums behind it, which the waves' dO rows pass through first
+__host__ __device__ __forceinline__ int dq_window_words(int W) { return (W + 3) & ~3; }
+__host__ __device__ __forceinline__ int dq_lds_words(int W) { return dq_window_words(W) + (W > 1024 ? 4 * W : 4096); }
+
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *out,
                                                                   const bf16_t *dout, const float *lse, float *delta,
@@ -375,7 +406,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                                                                   float keep_scale) {
     __shared__ __attribute__((aligned(16))) char Ks2[2][TILE_BYTES];
     __shared__ __attribute__((aligned(16))) char Vs2[2][TILE_BYTES];
-    extern __shared__ float win[];                            // the bias window, then the four waves' windows of ds sums
+    extern __shared__ __attribute__((aligned(16))) float win[];                            // the bias window, then the four waves' windows of ds sums
     const TransposedReader tr;
     const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
@@ -391,34 +422,42 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
     const bf16_t *dO = dout + (int64_t)b * S * E + hh * HD;
     const int q_blk_end = blk * 128 + 128;
     const int kv_end = blk * 128 >= n ? 0 : ((CAUSAL && q_blk_end < n) ? q_blk_end : n);
-    float *sums = win + W, *own = sums + wave * W;
-    for (int i = threadIdx.x; i < 4 * W; i += AT_THREADS) sums[i] = 0.f;
+    float *sums = win + dq_window_words(W), *own = sums + wave * W;
     f32x16 dqt[2] = {zero16(), zero16()};
     float far_sum[2] = {0.f, 0.f};                            // blocks wholly before / behind the window
     if (kv_end > 0) {
         const TileStream ldr(ld);
+        // queries through the second stage, dO through the room of the ds sums
+        char *own_q = (wave < 2 ? Ks2[1] : Vs2[1]) + (wave & 1) * 4096, *own_do = (char *)sums + wave * 4096;
+        issue_own_rows(Q + (int64_t)qw * ld, ld, n - qw, own_q);
+        issue_own_rows(dO + (int64_t)qw * E, E, n - qw, own_do);
         ldr.issue(K, n, Ks2[0]);
         ldr.issue(V, n, Vs2[0]);
-        frag_t qf[4], dof[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            qf[s] = load_row_frag(Q + (int64_t)q * ld, qok, s, h);
-            dof[s] = load_row_frag(dO + (int64_t)q * E, qok, s, h);
-        }
         const float lse_q = qok ? lse[((int64_t)b * H + hh) * S + q] : -INFINITY;
+        const bf16_t *O = out + ((int64_t)b * S + qw) * E + hh * HD;
+        frag_t of[4];                                         // row i * 8 + lane / 8, columns 8 (lane % 8) ..
+#pragma unroll
+        for (int i = 0; i < 4; ++i) of[i] = load_row_frag(O + (int64_t)(i * 8 + (lane >> 3)) * E + (lane & 7) * 8, qw + i * 8 + (lane >> 3) < n, 0, 0);
+        rel.expand<false, CAUSAL>(win, hh, scale);            // published by the loop's first barrier
+        __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): queries, dO and the first tile have landed
+        frag_t qf[4], dof[4];
+        own_frags(own_q, c, h, qok, qf);
+        own_frags(own_do, c, h, qok, dof);
         float delta_q = 0.f;
-        {
-            const bf16_t *O = out + (int64_t)b * S * E + hh * HD;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const frag_t of = load_row_frag(O + (int64_t)q * E, qok, s, h);
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 3);
+            const frag_t dr = *(const frag_t *)(own_do + r * ROW_BYTES + (((lane & 7) ^ aswz(r)) << 4));
+            float v = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) delta_q += (float)of.v[e] * (float)dof[s].v[e];
-            }
-            delta_q += __shfl_xor(delta_q, 32, 64);
-            if (qok && h == 0) delta[((int64_t)b * H + hh) * S + q] = delta_q;
+            for (int e = 0; e < 8; ++e) v += (float)of[i].v[e] * (float)dr.v[e];
+            v = qw + r < n ? group_sum(v, 3) : 0.f;
+            if (qw + r < n && (lane & 7) == 0) delta[((int64_t)b * H + hh) * S + qw + r] = v;
+            const float mine = __shfl(v, (c & 7) * 8, 64);    // rows 8 i .. + 7 to their columns
+            if (c >> 3 == i) delta_q = mine;
         }
-        rel.expand<false, CAUSAL>(win, hh, scale);                    // this and the zeroed sums: published by the loop's first barrier
+        __syncthreads();                                      // everybody has read its dO: the room is the sums' now
+        for (int i = lane; i < W; i += 64) own[i] = 0.f;
         // ds is kept without its factor `scale`; a query that sees nothing (lse = -inf) has p = 0
         const float sl2 = scale * LOG2E, nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
         // dP - delta in the matrix pipe: a product of ones (every key row) and -delta_q cut into three bf16 terms, which hold all 24
@@ -522,6 +561,8 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
         if (lane == 0) own[0] += lo;
         if (lane == 0) own[W - 1] += hi;
     }
+    if (kv_end == 0)
+        for (int i = lane; i < W; i += 64) own[i] = 0.f;
     // the block's bucket sums: window words over the four waves, then every bucket's range by a group of eight lanes
     __syncthreads();                                          // (everybody is done with the tiles, too)
     store_rows(Ks2[0] + wave * 4096, dqkv + ((int64_t)b * S + qw) * ld + hh * HD, ld, S - qw,
@@ -582,7 +623,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
     __shared__ __attribute__((aligned(16))) char Qs3[NST][TILE_BYTES];
     __shared__ __attribute__((aligned(16))) char dOs3[NST][TILE_BYTES];
     __shared__ __attribute__((aligned(16))) float lse_s[NST][TILE], delta_s[NST][TILE];
-    extern __shared__ float win[];
+    extern __shared__ __attribute__((aligned(16))) float win[];
     const TransposedReader tr;
     const int E = H * HD, ld = 3 * E;
     const Order<CAUSAL> order(false);
@@ -623,17 +664,17 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
                 delta_s[bufi][threadIdx.x] = DROP ? d_next : -d_next;
             }
         };
+        // keys and values through the stages that take no tile before the barrier below
+        issue_own_rows(K + (int64_t)kvw * ld, ld, n - kvw, Qs3[1] + wave * 4096);
+        issue_own_rows(V + (int64_t)kvw * ld, ld, n - kvw, dOs3[1] + wave * 4096);
         fetch(q_begin, 0);
-        frag_t kf[4], vf[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            kf[s] = load_row_frag(K + (int64_t)kv * ld, kok, s, h);
-            vf[s] = load_row_frag(V + (int64_t)kv * ld, kok, s, h);
-        }
         rel.expand<true, CAUSAL>(win, hh, scale);
         stage(0);
         if constexpr (DROP) keep2 = keep2_next;
-        __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): the first tile has landed
+        __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): keys, values and the first tile have landed
+        frag_t kf[4], vf[4];
+        own_frags(Qs3[1] + wave * 4096, c, h, kok, kf);
+        own_frags(dOs3[1] + wave * 4096, c, h, kok, vf);
         __syncthreads();
         int buf = 0, nbuf = 1;
         if (q_begin + TILE < n) fetch(q_begin + TILE, 1);
@@ -922,7 +963,7 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
     hipStream_t st = (hipStream_t)stream;
     dim3 grid((unsigned)row_blocks, (unsigned)(b * H)), block(AT_THREADS);
     auto dq = [&](auto kernel) -> int {
-        const size_t lds = (size_t)W * 4 * 5;
+        const size_t lds = (size_t)dq_lds_words(W) * 4;
         rc = allow_lds(name, kernel, lds);
         if (rc) return rc;
         hipLaunchKernelGGL(kernel, grid, block, lds, st, a, (const bf16_t *)qkv, (const bf16_t *)out, (const bf16_t *)dout, lse, delta_ws,
