@@ -82,40 +82,69 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_count_kernel(const float 
 }
 
 // joins the slabs of every row (slabs == 1: counts, kept, psum are the first kernel's own outputs) and adds up the loss; a
-// thread takes V experts of a row, the loads of eight slabs under way at once
+// thread takes V experts of a row, the loads of eight slabs under way at once.  One compute unit's read rate bounds it (64 rows
+// x 8 slabs of 64 experts: 6.2 us by one block), so the kept counts, which the loss does not need, are a second block's: 5.0 us
 template <int V>
 __global__ __launch_bounds__(1024) void balance_join_kernel(const int32_t *lengths, const int32_t *pcounts, const int32_t *pkept,
                                                           const float *ppsum, int32_t *counts, int32_t *kept, float *psum, float *loss,
                                                           int B, int S, int E, int slabs, float coef, int choices) {
     typedef int32_t iv __attribute__((ext_vector_type(V)));
     typedef float fv __attribute__((ext_vector_type(V)));
-    __shared__ float red[16];
+    __shared__ float red[2][16];
     float v = 0.f;
+    if (blockIdx.x == 1) {                          // (launched with slabs > 1 only)
+        for (int64_t i = (int64_t)threadIdx.x * V; i < (int64_t)B * E; i += 1024 * V) {
+            const int b = (int)(i / E), e = (int)(i - (int64_t)b * E);
+            const int64_t at = (int64_t)b * slabs * E + e;
+            iv k = 0;
+#pragma unroll 8
+            for (int z = 0; z < slabs; ++z) k += *(const iv *)(pkept + at + z * E);
+            *(iv *)(kept + i) = k;
+        }
+        return;
+    }
+    // the lengths are on their way while the slabs are loaded, and both sums meet at one barrier
+    const int first = lengths && (int)threadIdx.x < B ? lengths[threadIdx.x] : 0;
     for (int64_t i = (int64_t)threadIdx.x * V; i < (int64_t)B * E; i += 1024 * V) {
         const int b = (int)(i / E), e = (int)(i - (int64_t)b * E);
         const int64_t at = (int64_t)b * slabs * E + e;
-        iv c = 0, k = 0;
+        const int n_b = lengths ? lengths[b] : S;
+        iv c = 0;
         fv p = 0.f;
 #pragma unroll 8
         for (int z = 0; z < slabs; ++z) {
             c += *(const iv *)(pcounts + at + z * E);
-            k += *(const iv *)(pkept + at + z * E);
             p += *(const fv *)(ppsum + at + z * E);
         }
         if (slabs > 1) {
             *(iv *)(counts + i) = c;
-            *(iv *)(kept + i) = k;
             *(fv *)(psum + i) = p;
         }
-        const float n = (float)bal_length(lengths, b, S);
+        const float n = (float)(n_b < 0 ? 0 : (n_b > S ? S : n_b));
         if (n > 0.f) {
 #pragma unroll
             for (int j = 0; j < V; ++j) v += (float)c[j] / n * (p[j] / n);
         }
     }
-    const float G = bal_rows(lengths, B, S, red);
-    v = block_sum(v, red);
-    if (threadIdx.x == 0) loss[0] = G > 0.f ? coef * (float)E / (G * (float)choices) * v : 0.f;
+    float rows = first > 0 ? 1.f : 0.f;             // rows with tokens: whole numbers below 2^24, exact in any order
+    if (lengths)
+        for (int i = 1024 + (int)threadIdx.x; i < B; i += 1024) rows += lengths[i] > 0 ? 1.f : 0.f;
+    v = wave_sum(v);
+    rows = wave_sum(rows);
+    if ((threadIdx.x & 63) == 0) {
+        red[0][threadIdx.x >> 6] = v;
+        red[1][threadIdx.x >> 6] = rows;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float t = 0.f, G = 0.f;
+        for (int i = 0; i < 16; ++i) {
+            t += red[0][i];
+            G += red[1][i];
+        }
+        if (!lengths) G = (float)B;
+        loss[0] = G > 0.f ? coef * (float)E / (G * (float)choices) * t : 0.f;
+    }
 }
 
 // a group of lanes per token, V experts a lane; BAL_TURNS tokens of a lane are loaded before the first one is worked on
@@ -237,7 +266,7 @@ extern "C" int hapmi_balance_loss_fwd(const float *probs, const int32_t *index, 
     const bool vec = E % 4 == 0 && ((uintptr_t)pc % 16 == 0 && (uintptr_t)pk % 16 == 0 && (uintptr_t)pp % 16 == 0 && (uintptr_t)counts % 16 == 0 &&
                                     (uintptr_t)kept % 16 == 0 && (uintptr_t)prob_sum % 16 == 0);
     auto join = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, st, lengths, (const int32_t *)pc, (const int32_t *)pk, (const float *)pp, counts, kept, prob_sum, loss,
+        hipLaunchKernelGGL(kernel, dim3(slabs > 1 ? 2 : 1), dim3(1024), 0, st, lengths, (const int32_t *)pc, (const int32_t *)pk, (const float *)pp, counts, kept, prob_sum, loss,
                            (int)B, (int)S, (int)E, (int)slabs, coef, choices);
     };
     if (vec) join(balance_join_kernel<4>);
