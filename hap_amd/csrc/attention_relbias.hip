@@ -93,28 +93,30 @@ struct RelArgs {
 // operand: the lane's byte offsets inside a tile never change, the tile's first row is a scalar base, and a transfer costs no
 // vector arithmetic.  A tile that ends inside repeats the operand's last row.
 struct TileStream {
-    static constexpr int LOADS = 2;
-    int off[LOADS], ld;
-    __device__ __forceinline__ static int row(int i) { return (i * 4 + (int)(threadIdx.x >> 6)) * 8 + (int)((threadIdx.x & 63) >> 3); }
-    __device__ __forceinline__ static int chunk(int i) { return (((int)threadIdx.x & 7) ^ aswz(row(i))) * 16; }
-    __device__ __forceinline__ TileStream(int ld_) : ld(ld_) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) off[i] = row(i) * ld * 2 + chunk(i);
-    }
+    static constexpr int LOADS = 2;                           // wave instructions a tile: rows 0 .. 31 and 32 .. 63
+    int off, ld;
+    __device__ __forceinline__ static int row(int tid) { return (tid >> 6) * 8 + ((tid & 63) >> 3); }
+    __device__ __forceinline__ static int chunk(int tid) { return ((tid & 7) ^ aswz(row(tid))) * 16; }        // (32 rows on the same)
+    __device__ __forceinline__ TileStream(int ld_) : off(row(threadIdx.x) * ld_ * 2 + chunk(threadIdx.x)), ld(ld_) {}
     __device__ __forceinline__ void issue(const bf16_t *base, int rows_left, char *lds_tile) const {
         typedef __attribute__((address_space(3))) char lds_char;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char *)lds_tile + wave * 1024;
-        int o[LOADS] = {off[0], off[1]};
+        int o[LOADS] = {off, off};
+        const bf16_t *from[LOADS] = {base, base + 32 * ld};
         if (rows_left < TILE) {
+            int tid = threadIdx.x;
+            asm volatile("" : "+v"(tid));                     // (nothing of this is kept in registers over the whole tiles)
+            from[1] = base;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) o[i] = (row(i) < rows_left ? row(i) : rows_left - 1) * ld * 2 + chunk(i);
+            for (int i = 0; i < LOADS; ++i)
+                o[i] = (row(tid) + i * 32 < rows_left ? row(tid) + i * 32 : rows_left - 1) * ld * 2 + chunk(tid);
         }
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                          :
-                         : "s"(lds_addr + i * 4096), "v"(o[i]), "s"(base)
+                         : "s"(lds_addr + i * 4096), "v"(o[i]), "s"(from[i])
                          : "memory");
     }
 };
@@ -145,6 +147,9 @@ __device__ __forceinline__ void own_frags(const char *lds, int c, int h, bool va
         for (int e = 0; e < 8; ++e) f[s].v[e] = valid ? f[s].v[e] : (bf16_t)0.f;
     }
 }
+
+// the same in all lanes, in a scalar register
+__device__ __forceinline__ float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 
 // initial accumulator of a 32 x 32 score block: rows of the block are runs of four words
 __device__ __forceinline__ f32x16 bias_tile(const float *w) {
@@ -191,7 +196,9 @@ __device__ __forceinline__ float both_halves_max(float x) {
 // Stored from the registers, 8 bytes a lane, it takes 8 instructions that touch 32 rows each: the forward, dQ and dK / dV
 // kernels of [12, 512] x 16 heads took 25.1, 44.2 and 41.6 us then, and 24.1, 43.4 and 38.8 us this way.
 template <typename F> __device__ __forceinline__ void store_rows(char *lds, bf16_t *first_row, int ld, int rows, F value) {
-    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));                            // (no address of this is worth a register before)
+    const int c = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
     float m = -INFINITY, lsum = 0.f;                          // running maximum in units of log 2
     if (kv_end > 0) {
         const TileStream ldr(ld);
-        const float sl2 = scale * LOG2E;
+        const float sl2 = uniform(scale * LOG2E);
         constexpr int PER_TILE = 2 * TileStream::LOADS + (DROP ? 1 : 0);
         static_assert(2 * TileStream::LOADS == 4, "the waits below are written for four (five) transfers per tile");
         const int n_kt = (S + TILE - 1) / TILE;
@@ -394,9 +401,9 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // ---------------------------------------------------------------------------------------------
 // dQ and the bias gradient: lanes own query columns, kv tiles are streamed
 // ---------------------------------------------------------------------------------------------
-// words of a window and of the sums behind it, which the waves' dO rows pass through first
-__host__ __device__ __forceinline__ int dq_window_words(int W) { return (W + 3) & ~3; }
-__host__ __device__ __forceinline__ int dq_lds_words(int W) { return dq_window_words(W) + (W > 1024 ? 4 * W : 4096); }
+__host__ __device__ __forceinline__ int round4(int n) { return (n + 3) & ~3; }
+// a window, and the waves' sums, whose room their dO rows pass through first
+__host__ __device__ __forceinline__ int dq_lds_words(int W) { return round4(W) + (W > 1024 ? 4 * round4(W) : 4096); }
 
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *out,
@@ -406,7 +413,8 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                                                                   float keep_scale) {
     __shared__ __attribute__((aligned(16))) char Ks2[2][TILE_BYTES];
     __shared__ __attribute__((aligned(16))) char Vs2[2][TILE_BYTES];
-    extern __shared__ __attribute__((aligned(16))) float win[];                            // the bias window, then the four waves' windows of ds sums
+    __shared__ int ranges[2 * REL_MAX_SIDE][2];               // the buckets' first and last relative position in the window
+    extern __shared__ __attribute__((aligned(16))) float win[];             // the bias window, then the four waves' windows of ds sums
     const TransposedReader tr;
     const int W = rel.window();
     const int E = H * HD, ld = 3 * E;
@@ -422,7 +430,14 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
     const bf16_t *dO = dout + (int64_t)b * S * E + hh * HD;
     const int q_blk_end = blk * 128 + 128;
     const int kv_end = blk * 128 >= n ? 0 : ((CAUSAL && q_blk_end < n) ? q_blk_end : n);
-    float *sums = win + dq_window_words(W), *own = sums + wave * W;
+    const int WS = round4(W), n_buckets = rel.side << rel.bidir;
+    float *sums = win + WS, *own = sums + wave * WS;
+    auto set_ranges = [&]() {
+        if ((int)threadIdx.x < n_buckets) rel.range(threadIdx.x, ranges[threadIdx.x][0], ranges[threadIdx.x][1]);
+    };
+    auto clear_own = [&]() {
+        for (int i = lane * 4; i < WS; i += 256) *(f32x4 *)(own + i) = (f32x4)(0.f);
+    };
     f32x16 dqt[2] = {zero16(), zero16()};
     float far_sum[2] = {0.f, 0.f};                            // blocks wholly before / behind the window
     if (kv_end > 0) {
@@ -438,6 +453,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
         frag_t of[4];                                         // row i * 8 + lane / 8, columns 8 (lane % 8) ..
 #pragma unroll
         for (int i = 0; i < 4; ++i) of[i] = load_row_frag(O + (int64_t)(i * 8 + (lane >> 3)) * E + (lane & 7) * 8, qw + i * 8 + (lane >> 3) < n, 0, 0);
+        set_ranges();
         rel.expand<false, CAUSAL>(win, hh, scale);            // published by the loop's first barrier
         __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): queries, dO and the first tile have landed
         frag_t qf[4], dof[4];
@@ -457,9 +473,9 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
             if (c >> 3 == i) delta_q = mine;
         }
         __syncthreads();                                      // everybody has read its dO: the room is the sums' now
-        for (int i = lane; i < W; i += 64) own[i] = 0.f;
+        clear_own();
         // ds is kept without its factor `scale`; a query that sees nothing (lse = -inf) has p = 0
-        const float sl2 = scale * LOG2E, nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
+        const float sl2 = uniform(scale * LOG2E), nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
         // dP - delta in the matrix pipe: a product of ones (every key row) and -delta_q cut into three bf16 terms, which hold all 24
         // bits of it; one matrix instruction a block in place of 16 subtractions a lane
         frag_t ones, minus_delta;
@@ -557,29 +573,38 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
                 }
             }
         }
-        const float lo = wave_sum(far_sum[0]), hi = wave_sum(far_sum[1]);
-        if (lane == 0) own[0] += lo;
-        if (lane == 0) own[W - 1] += hi;
+        const float lo = group_sum(far_sum[0], 6), hi = group_sum(far_sum[1], 6);
+        if (lane == 0) {
+            own[0] += lo;
+            own[W - 1] += hi;
+        }
     }
-    if (kv_end == 0)
-        for (int i = lane; i < W; i += 64) own[i] = 0.f;
+    if (kv_end == 0) {
+        clear_own();
+        set_ranges();
+    }
     // the block's bucket sums: window words over the four waves, then every bucket's range by a group of eight lanes
     __syncthreads();                                          // (everybody is done with the tiles, too)
     store_rows(Ks2[0] + wave * 4096, dqkv + ((int64_t)b * S + qw) * ld + hh * HD, ld, S - qw,
                [&](int u, int i) { return qok ? dqt[u][i] * scale : 0.f; });
-    for (int i = threadIdx.x; i < W; i += AT_THREADS) win[i] = ((sums[i] + sums[W + i]) + sums[2 * W + i]) + sums[3 * W + i];
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));                            // addresses below are not worth registers in the loop above
+    for (int i = tid * 4; i < WS; i += AT_THREADS * 4)
+        *(f32x4 *)(win + i) = ((*(const f32x4 *)(sums + i) + *(const f32x4 *)(sums + WS + i)) + *(const f32x4 *)(sums + 2 * WS + i)) +
+                              *(const f32x4 *)(sums + 3 * WS + i);
     __syncthreads();
-    const int n_buckets = rel.side << rel.bidir;
     float *mine = part + ((int64_t)bh * ((S + 127) / 128) + blk) * n_buckets;
-    for (int u = threadIdx.x >> 3; u < n_buckets; u += AT_THREADS / 8) {
-        int lo, hi;
-        rel.range(u, lo, hi);
+    for (int u = tid >> 3; u < n_buckets; u += AT_THREADS / 8) {
+        const int lo = ranges[u][0] + rel.R + MARGIN, hi = ranges[u][1] + rel.R + MARGIN;
         float v = 0.f;
-        for (int r = lo + (threadIdx.x & 7); r <= hi; r += 8) v += win[r + rel.R + MARGIN];
-        v += __shfl_xor(v, 1, 64);
-        v += __shfl_xor(v, 2, 64);
-        v += __shfl_xor(v, 4, 64);
-        if ((threadIdx.x & 7) == 0) mine[u] = v;
+        for (int i = lo + (tid & 7); i <= hi; i += 32) {          // four reads under way at once
+            float w4[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w4[j] = i + j * 8 <= hi ? win[i + j * 8] : 0.f;
+            v += (w4[0] + w4[1]) + (w4[2] + w4[3]);
+        }
+        v = group_sum(v, 3);
+        if ((tid & 7) == 0) mine[u] = v;
     }
 }
 
@@ -640,7 +665,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
     f32x16 dvt[2] = {zero16(), zero16()}, dkt[2] = {zero16(), zero16()};
     if (blk * 128 < n) {
         const TileStream lq(ld), ldo(E);
-        const float sl2 = scale * LOG2E;
+        const float sl2 = uniform(scale * LOG2E);
         const int q_begin = CAUSAL ? blk * 128 : 0;           // causal: earlier queries see none of the block's keys
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
         const u32x2 *keep_col = DROP ? (const u32x2 *)(keep_cols + ((int64_t)bh * S + (kv < S ? kv : S - 1)) * (2 * ((S + TILE - 1) / TILE))) : nullptr;
