@@ -33,7 +33,10 @@ constexpr int REL_MAX_REACH = HAPMI_RELBIAS_MAX_REACH;
 // A 64 x 32 block of scores spans 95 diagonals: the window carries this many saturated entries on either side, and the
 // offset of a block that lies wholly beyond the window is clamped so that it reads nothing else.
 constexpr int MARGIN = 95;
-constexpr float HIDDEN = -1e30f;              // a bias at or below this hides the pair (the type's lowest value included)
+// A bias at or below this hides the pair (the type's lowest value included).  float32 scores of that size are multiples of 8, and
+// a log-sum-exp of them is good to 1e8 * 2^-22 = 24: up to here weights made from it stay inside the exponentials' range (2^34),
+// further down they would not.
+constexpr float HIDDEN = -1e8f;
 
 struct RelArgs {
     const float *table;                       // [buckets, ld], column = head

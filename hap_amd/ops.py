@@ -1081,7 +1081,8 @@ def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128
     """``attention_fwd`` with a learned relative position bias: scores scale * q_i k_j + table[bucket(j - i), head],
     ``table`` float32 [buckets, H] (rows may be strided: the columns of a device's heads).  Buckets as
     ``relative_bucket_starts(buckets, max_distance, bidirectional)`` cuts the distances; ``bidirectional`` None: two sides
-    unless ``causal``.  An entry at or below -1e30 hides its bucket's pairs.  ``lengths`` (int32 [b]): the sequences of a padded
+    unless ``causal``.  An entry at or below -1e8 hides its bucket's pairs; the
+    others stay below 1e8 in size (scores are float32, and a weight made from a score of size x is good to x * 2^-22).  ``lengths`` (int32 [b]): the sequences of a padded
     batch; rows behind a sequence's end get zeros and lse = -inf, its keys there are not read.  ``keep_rows`` / ``p``:
     dropout of the probabilities, as in ``attention_fwd``."""
     what = "attention_relbias_fwd"

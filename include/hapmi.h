@@ -343,7 +343,8 @@ int hapmi_attention_bwd_dropout(const void *qkv, const void *out, const void *do
 /* The same attention with a learned relative position bias: s_ij = scale <q_i, k_j> + table[bucket(j - i), h], h being the
  * head (column of the table), and the table's gradient.  No counterpart in the reference, whose models add their
  * positions to the input (models.py:79-81, 167, 504-509).
- *   table          float32 [n_buckets][ld], ld >= H; an entry at or below -1e30 hides the pairs of its bucket
+ *   table          float32 [n_buckets][ld], ld >= H; an entry at or below -1e8 hides the pairs of its bucket, the others are
+ *                  below 1e8 in size (scores are float32: a weight made from one of size x is good to x * 2^-22)
  *   starts_host    the first distance of every bucket of one side: n_buckets / 2 (bidirectional) or n_buckets numbers,
  *                  starts[0] = 0, never falling; bucket k of a side holds the distances starts[k] .. starts[k + 1] - 1, the
  *                  last one all from its start on (a bucket whose start equals the next one's is never used).

@@ -31,12 +31,12 @@ def bucket_matrix(S, n_buckets, max_distance, bidirectional):
 
 
 def relbias_forward(qkv, table, H, scale, max_distance, bidirectional, causal, lengths=None, keep=None, p=0.0):
-    """(out [b, S, H, 64], lse [b, H, S], probabilities [b, H, S, S], |terms| of out) in float64; a bias at or below -1e30
+    """(out [b, S, H, 64], lse [b, H, S], probabilities [b, H, S, S], |terms| of out) in float64; a bias at or below -1e8
     hides its pairs; a query without visible keys gives zeros and -inf.  ``keep``: bool [b, H, S, S] dropout decisions."""
     b, S = qkv.shape[:2]
     q, k, v = (t.transpose(1, 2) for t in qkv.double().view(b, S, 3, H, -1).unbind(2))
     t = table.double()
-    t = torch.where(t <= -1e30, torch.full_like(t, -math.inf), t)
+    t = torch.where(t <= -1e8, torch.full_like(t, -math.inf), t)
     s = q @ k.transpose(-1, -2) * scale + t[bucket_matrix(S, table.shape[0], max_distance, bidirectional)].permute(2, 0, 1)
     at = torch.arange(S)
     hidden = torch.zeros(b, 1, S, S, dtype=torch.bool)

@@ -101,7 +101,7 @@ def test_padded_batches(cuda, S, lengths, causal):
         assert (res[2][z, n:] == 0).all() and torch.isneginf(res[1][z, :, n:]).all()
 
 
-@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float32).min, -1e30])
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float32).min, -1e30, -1e8])
 def test_hidden_buckets(cuda, low):
     """A bias at the type's lowest value hides its pairs; a query left with nothing gets zeros and no gradient."""
     qkv, table, dout = make(5, 2, 150, 2, 32)
@@ -130,6 +130,22 @@ def test_large_scores_do_not_overflow(cuda):
     assert all(torch.isfinite(t).all() for t in (out, dqkv, dtable))
     within(lse, wlse, 0.03 + 2 ** -22 * wlse.abs(), "lse")
     assert ((out.double().cpu().view_as(want) - want).norm() / want.norm()).item() < 0.1
+
+
+@pytest.mark.parametrize("low", [-1e4, -65504.0, -1e6, -9e7])
+def test_low_biases_that_hide_nothing(cuda, low):
+    """Every pair has the same very low bias: a softmax does not see it.  float32 scores of that size keep 2^-24 * |low| * log2 e
+    of theirs apart at best, so all weights are compared with the even ones: results are averages of the values."""
+    qkv, table, dout = make(9, 1, 150, 2, 32)
+    qkv[..., :2 * 2 * HD] = 0                                  # queries and keys
+    table[:] = low
+    out, lse, dqkv, dtable = run(cuda, qkv, table, dout, 2)
+    mean = qkv.double().view(1, 150, 3, 2, HD)[:, :, 2].mean(1, keepdim=True)
+    size = qkv.double().view(1, 150, 3, 2, HD)[:, :, 2].abs().mean(1, keepdim=True)
+    # weights: one rounding to bf16 each (2^-8, all the same way); the mean's own rounding
+    assert ((out.double().cpu().view(1, 150, 2, HD) - mean).abs() <= 2 ** -8 * size + 2 ** -8 * mean.abs() + 1e-6).all()
+    within(lse, torch.full((1, 2, 150), low + 5.0106353, dtype=torch.float64), 2 ** -22 * abs(low) + 1e-4, "lse")
+    assert torch.isfinite(dqkv.float()).all() and torch.isfinite(dtable).all()
 
 
 @pytest.mark.parametrize("S,causal", [(64, False), (129, True), (200, False), (33, True)])
