@@ -1056,12 +1056,12 @@ def _bucket_array(n_buckets, max_distance, bidirectional):
 
 def _relbias(what, table, H, max_distance, bidirectional, causal):
     """The bias description of the C ABI; ``table`` may be the columns of a wider one."""
-    if table.dim() != 2 or table.shape[1] != H or table.dtype != torch.float32 or (H > 1 and table.stride(1) != 1):
-        raise ValueError(f"{what}: the table must be a float32 [buckets, {H}] tensor with unit column stride")
+    if table.dim() != 2 or table.shape[1] != H or table.dtype != torch.float32 or (H > 1 and table.stride(1) != 1) or table.stride(0) < H:
+        raise ValueError(f"{what}: the table must be a float32 [buckets, {H}] tensor with unit column stride and rows apart")
     n = table.shape[0]
     bidirectional = (not causal) if bidirectional is None else bool(bidirectional)
     arr = _bucket_array(n, int(max_distance), bidirectional)
-    a = _lib.RelBias(table.data_ptr(), max(table.stride(0), H), n, bidirectional, ctypes.addressof(arr))
+    a = _lib.RelBias(table.data_ptr(), table.stride(0), n, bidirectional, ctypes.addressof(arr))
     a._keep = arr
     return a
 
@@ -1083,7 +1083,8 @@ def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128
     ``relative_bucket_starts(buckets, max_distance, bidirectional)`` cuts the distances; ``bidirectional`` None: two sides
     unless ``causal``.  An entry at or below -1e8 hides its bucket's pairs; the
     others stay below 1e8 in size (scores are float32, and a weight made from a score of size x is good to x * 2^-22).  ``lengths`` (int32 [b]): the sequences of a padded
-    batch; rows behind a sequence's end get zeros and lse = -inf, its keys there are not read.  ``keep_rows`` / ``p``:
+    batch; rows behind a sequence's end get zeros and lse = -inf, its keys there are not read (inside it, pairs that the causal
+    mask or the bias hides are multiplied with weight zero: non-finite values there spread).  ``keep_rows`` / ``p``:
     dropout of the probabilities, as in ``attention_fwd``."""
     what = "attention_relbias_fwd"
     n = b * S * H
@@ -1122,8 +1123,8 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     ``workspace``: float32 scratch of ``attention_relbias_workspace_elems`` (None: taken from torch's allocator)."""
     what = "attention_relbias_bwd"
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
-    if dtable.shape != table.shape or dtable.dtype != torch.float32 or (H > 1 and dtable.stride(1) != 1):
-        raise ValueError(f"{what}: dtable must be float32 of the table's shape with unit column stride")
+    if dtable.shape != table.shape or dtable.dtype != torch.float32 or (H > 1 and dtable.stride(1) != 1) or dtable.stride(0) < H:
+        raise ValueError(f"{what}: dtable must be float32 of the table's shape with unit column stride and rows apart")
     if (keep_rows is None) != (keep_cols is None):
         raise ValueError(f"{what}: keep_rows and keep_cols come together")
     _on_device(what, table, qkv)
@@ -1135,7 +1136,7 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     stream, (dq_, dl_, ws_, q_, o_, do_, l_, n_, kr_, kc_) = _operands(
         what, ("dqkv", "delta_ws", "workspace", "qkv", "out", "dout", "lse", "lengths", "keep_rows", "keep_cols"), _RELBIAS_BWD_TYPES,
         (dqkv, delta_ws, workspace, qkv, out, dout, lse, lengths, keep_rows, keep_cols), (n * 192, n, need, n * 192, n * 64, n * 64, n, b, words, words), 3, ("lengths",))
-    check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), max(dtable.stride(0), H), accumulate,
+    check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), dtable.stride(0), accumulate,
                                             dl_, _kept(ws_, workspace), workspace.numel(), b, S, H, scale, kr_, kc_, p, stream))
 
 

@@ -363,7 +363,9 @@ typedef struct {
 } hapmi_relbias;
 /* causal != 0: key j is visible to query i iff j <= i.  lengths: int32[b] on the device or NULL: the sequences of a padded
  * batch; of sample z the first lengths[z] (clamped to 0 .. S) positions exist, later keys are not read and later rows get
- * zeros (out, dqkv) and -inf (lse).  A query that sees nothing gets the same.  keep_rows / keep_cols / p: dropout of the
+ * zeros (out, dqkv) and -inf (lse).  A query that sees nothing gets the same.  A pair hidden by the causal mask or by its
+ * bias has weight zero, but is multiplied: an infinity or NaN in a key or value inside a sequence's length may reach the
+ * other queries of the sequence, as it does in a product with explicit zeros.  keep_rows / keep_cols / p: dropout of the
  * probabilities as in hapmi_attention_fwd_dropout (NULL = none).  scale > 0.
  * Backward takes out and lse as forward left them, writes dqkv completely and dtable[n_buckets][ld_dtable]'s columns
  * 0 .. H - 1 (accumulate != 0: adds to them; b >= 1); delta_ws is float32 scratch of b*H*S elements, workspace float32 scratch

@@ -3,6 +3,7 @@ on the host, before any device is touched (the pointers below are never followed
 import ctypes
 
 import pytest
+import torch
 
 from hap_amd._lib import BF16, F32, HapmiError, RelBias, _load
 from hap_amd import ops
@@ -141,7 +142,6 @@ def test_balance_loss():
 
 
 def test_cpu_tensors_are_refused():
-    import torch
     t = torch.zeros(1, 4, 192, dtype=torch.bfloat16)
     with pytest.raises(HapmiError, match="GPU tensors only"):
         ops.qk_norm_rotary_fwd(t, t, 1, 4, 1)
@@ -151,3 +151,17 @@ def test_cpu_tensors_are_refused():
         ops.rotary_table(0, 8)
     with pytest.raises(ValueError):
         ops.rotary_table(8, 7)
+
+
+def test_bias_tables_whose_rows_overlap():
+    """A table broadcast over its buckets, or one with rows closer than its heads, would be read beyond its memory."""
+    whole = torch.zeros(8, 4)
+    row = torch.zeros(1, 4)
+    for odd in (row.expand(8, 4), torch.zeros(64).as_strided((8, 4), (3, 1)), torch.zeros(8, 8)[:, ::2], whole.double(), whole[:, :3], whole[0]):
+        with pytest.raises(ValueError, match="table must be"):
+            ops._relbias("x", odd, 4, 8, False, True)
+    assert ops._relbias("x", torch.zeros(8, 6)[:, 1:5], 4, 8, False, True).ld == 6
+    x = torch.zeros(1, 2, 3 * 4 * 64)
+    for odd in (row.expand(8, 4), torch.zeros(8, 3), torch.zeros(8, 8)[:, ::2]):
+        with pytest.raises(ValueError, match="dtable must be"):
+            ops.attention_relbias_bwd(x, whole, x, x, x, x, odd, x, 1, 2, 4, 0.125, max_distance=8, causal=True)
