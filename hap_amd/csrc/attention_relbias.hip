@@ -18,7 +18,8 @@
 // shift that rides on the addition), so that lane l always holds the diagonal (row) - l.  A row's 32 columns have to lie in
 // lanes 0 .. 31 with zeros above: the swap of half waves delivers that for the two rows of an accumulator register at
 // once.  That is 4 vector instructions a register, and no atomics: LDS float additions of the 16 registers cost 180 cycles
-// each on this chip (the dQ kernel of [12, 512] x 16 heads took 274 us with them).  The vector is added to the wave's own
+// each on this chip (the dQ kernel of [12, 512] x 16 heads took 274 us with them and 46 us without; 38 us by now).  The vector is
+// added to the wave's own
 // window in LDS; the block adds its four windows and sums the buckets' ranges, the dK / dV kernel adds the blocks, all in a
 // fixed order: the same bits every time.
 #include "common.h"
@@ -224,7 +225,7 @@ template <typename F> __device__ __forceinline__ void store_rows(char *lds, bf16
 // of their linear index; the row blocks of one (batch, head) stream the same tiles, so they go to one XCD, next to each
 // other in time.  Neighbouring heads go to different XCDs: in a padded batch they have the same length, and a long sample
 // would otherwise land on one XCD (dK / dV of lengths 334 .. 1001 in [6, 1001] x 12 heads: 62 us with a contiguous eighth of the heads on
-// each XCD).  Causal: the row blocks with the most work start first (BlockOrder), which keeps a head on its XCD too.
+// each XCD, 44 us so).  Causal: the row blocks with the most work start first (BlockOrder), which keeps a head on its XCD too.
 template <bool CAUSAL> struct Order {
     int blk, bh;
     __device__ __forceinline__ Order(bool work_grows_with_index) {
@@ -249,6 +250,14 @@ __device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) 
 // ---------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------
+// One pass over the keys with a running maximum and sum; a wave holds 32 queries, a block of four waves 128, and the 64-key
+// tiles pass through three LDS stages, so that a transfer has two tiles' arithmetic to arrive in.  Three blocks a CU: all 768
+// of the encoder shape are resident at once.  Bound by vector instructions: a score costs a multiply-add, an exponential, an
+// addition, half a maximum and half a conversion.  [12, 512] x 16 heads: 24 us, 0.54 PFLOP/s, vector pipe 62 % and matrix pipe
+// 28 % of the cycles (8 us of it fixed: launch, prologue, results); [1, 8192] x 16 heads, causal: 164 .. 179 us from card to
+// card, 0.80 PFLOP/s of the visible half, vector pipe 72 %, matrix pipe 42 %, HBM 65 + 17 MB.
+// Without effect or worse: four parallel chains for the maximum, products pinned between the exponentials (184 for 177 us), no
+// maximum unless a sum of weights gets large (198 us: the test stands between the exponentials and the products).
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArgs rel, const bf16_t *qkv, bf16_t *out, float *lse,
                                                                const int32_t *lengths, int S, int H, float scale,
@@ -404,6 +413,12 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // ---------------------------------------------------------------------------------------------
 // dQ and the bias gradient: lanes own query columns, kv tiles are streamed
 // ---------------------------------------------------------------------------------------------
+// 13 matrix products and about 80 vector instructions a lane for a 32 x 32 block of scores, 64 more where it touches the bias
+// window (the diagonal sums).  Three waves a SIMD hide each other's latencies; two, each of which also works on the next
+// block's scores, were slower where the card is full: 46.0 us for 41.8 on [12, 512] x 16 heads, 147 for 141 us on [2, 4096]
+// causal (70.5 for 76.5 us on [2, 2048], which fills it once over).  [12, 512] x 16 heads: 38 us, matrix pipe 27 %, vector pipe
+// 54 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one; [2, 4096] x 16 heads, causal:
+// 137 us, matrix pipe 43 %, vector pipe 61 %.
 __host__ __device__ __forceinline__ int round4(int n) { return (n + 3) & ~3; }
 // a window, and the waves' sums, whose room their dO rows pass through first
 __host__ __device__ __forceinline__ int dq_lds_words(int W) { return round4(W) + (W > 1024 ? 4 * round4(W) : 4096); }
@@ -638,9 +653,13 @@ __device__ __forceinline__ void table_gradient(const float *part, float *dtable,
 // A wave works on one 32 x 32 block of scores at a time: 8 matrix products for the scores and dP, 80 vector instructions a
 // lane for P and dS, 8 products for dV and dK.  Two waves fit a SIMD, so the wave itself has to keep the matrix pipe fed:
 // the score products of the NEXT block and the first half of this block's dV / dK products stand one by one between the
-// vector instructions of this block (pinning that order on top changed nothing: 44 us either way on [12, 512] x 16 heads; without
-// the look-ahead 49 us), three tiles are kept in LDS because the next block may be the next tile's.  Everything that would be a branch a block is data: causally hidden pairs are -inf in the bias window, queries
-// beyond the end carry lse = +inf, and dP starts from -delta.
+// instructions of this block, and three tiles are kept in LDS because the next block may be the next tile's.  Everything that
+// would be a branch a block is data: causally hidden pairs are -inf in the bias window, queries beyond the end carry
+// lse = +inf, and dP starts from -delta.  Plain blocks with three waves a SIMD instead: 36.9 us for 37.3 on [12, 512] x 16 heads,
+// but 29.0 for 25.2 us on [8, 512] and 88 for 74 us on [2, 2048].  What it spends adds up rather than overlaps (leaving out the
+// matrix products 108 of 182 us on [4, 2048], the LDS reads 138, the exponentials 178).  [12, 512] x 16 heads: 38 us, 0.68
+// PFLOP/s, matrix pipe 34 %, vector pipe 43 %, LDS 39 %, HBM 51 + 25 MB; [2, 4096] x 16 heads, causal: 153 .. 161 us, matrix
+// pipe 46 %, vector pipe 46 %, LDS 48 %.
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *dout,
                                                                    const float *lse, const float *delta, bf16_t *dqkv,

@@ -9,7 +9,8 @@
 // Memory bound: forward reads and writes a row once, backward reads x and dy and writes dx.  A group of 1 .. 32 lanes
 // holds one head of a token, every lane two 16-byte vectors chosen so that both halves of every rotated pair are its
 // own: the rotation needs no exchange, the mean one butterfly over the group.  The lane takes the query and the key of
-// its (token, head) together and reads the angles once for both.
+// its (token, head) together and reads the angles once for both.  bf16, 16 heads of 64: forward of [12, 512] 16.4 us, 75 MB at
+// 4.6 TB/s; backward of [4, 8192] with both gains 117 us, 547 MB at 4.7 TB/s (a large copy: 5.2 TB/s).
 #include "common.h"
 
 namespace {
