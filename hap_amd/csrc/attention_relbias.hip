@@ -414,23 +414,24 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // dQ and the bias gradient: lanes own query columns, kv tiles are streamed
 // ---------------------------------------------------------------------------------------------
 // 13 matrix products and about 80 vector instructions a lane for a 32 x 32 block of scores, 64 more where it touches the bias
-// window (the diagonal sums).  Three waves a SIMD hide each other's latencies; two, each of which also works on the next
-// block's scores, were slower where the card is full: 46.0 us for 41.8 on [12, 512] x 16 heads, 147 for 141 us on [2, 4096]
-// causal (70.5 for 76.5 us on [2, 2048], which fills it once over).  [12, 512] x 16 heads: 38 us, matrix pipe 27 %, vector pipe
+// window (the diagonal sums).  Three waves a SIMD hide each other's latencies; where the launch does not fill the card, two
+// that also work on the next block's scores are faster (AHEAD; fits_two_a_cu has both sides).  [12, 512] x 16 heads: 38 us, matrix pipe 27 %, vector pipe
 // 54 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one; [2, 4096] x 16 heads, causal:
 // 137 us, matrix pipe 43 %, vector pipe 61 %.
 __host__ __device__ __forceinline__ int round4(int n) { return (n + 3) & ~3; }
 // a window, and the waves' sums, whose room their dO rows pass through first
 __host__ __device__ __forceinline__ int dq_lds_words(int W) { return round4(W) + (W > 1024 ? 4 * round4(W) : 4096); }
 
-template <bool CAUSAL, bool DROP>
-__global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *out,
+template <bool CAUSAL, bool DROP, bool AHEAD>
+__global__ __launch_bounds__(AT_THREADS, AHEAD ? 2 : 3) void relbias_bwd_dq_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *out,
                                                                   const bf16_t *dout, const float *lse, float *delta,
                                                                   bf16_t *dqkv, float *part, const int32_t *lengths, int S,
                                                                   int H, float scale, const uint32_t *keep_rows,
                                                                   float keep_scale) {
-    __shared__ __attribute__((aligned(16))) char Ks2[2][TILE_BYTES];
-    __shared__ __attribute__((aligned(16))) char Vs2[2][TILE_BYTES];
+    static_assert(!(DROP && AHEAD), "the mask keeps delta out of the products");
+    constexpr int NST = AHEAD ? 3 : 2;
+    __shared__ __attribute__((aligned(16))) char Kst[NST][TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) char Vst[NST][TILE_BYTES];
     __shared__ int ranges[2 * REL_MAX_SIDE][2];               // the buckets' first and last relative position in the window
     extern __shared__ __attribute__((aligned(16))) float win[];             // the bias window, then the four waves' windows of ds sums
     const TransposedReader tr;
@@ -461,11 +462,11 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
     if (kv_end > 0) {
         const TileStream ldr(ld);
         // queries through the second stage, dO through the room of the ds sums
-        char *own_q = (wave < 2 ? Ks2[1] : Vs2[1]) + (wave & 1) * 4096, *own_do = (char *)sums + wave * 4096;
+        char *own_q = (wave < 2 ? Kst[1] : Vst[1]) + (wave & 1) * 4096, *own_do = (char *)sums + wave * 4096;
         issue_own_rows(Q + (int64_t)qw * ld, ld, n - qw, own_q);
         issue_own_rows(dO + (int64_t)qw * E, E, n - qw, own_do);
-        ldr.issue(K, n, Ks2[0]);
-        ldr.issue(V, n, Vs2[0]);
+        ldr.issue(K, n, Kst[0]);
+        ldr.issue(V, n, Vst[0]);
         const float lse_q = qok ? lse[((int64_t)b * H + hh) * S + q] : -INFINITY;
         const bf16_t *O = out + ((int64_t)b * S + qw) * E + hh * HD;
         frag_t of[4];                                         // row i * 8 + lane / 8, columns 8 (lane % 8) ..
@@ -494,100 +495,205 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
         clear_own();
         // ds is kept without its factor `scale`; a query that sees nothing (lse = -inf) has p = 0
         const float sl2 = uniform(scale * LOG2E), nl = lse_q == -INFINITY ? -INFINITY : -lse_q * LOG2E;
-        // dP - delta in the matrix pipe: a product of ones (every key row) and -delta_q cut into three bf16 terms, which hold all 24
-        // bits of it; one matrix instruction a block in place of 16 subtractions a lane
-        frag_t ones, minus_delta;
+        if constexpr (AHEAD) {
+            // One block's score products stand between the vector instructions of the block before it; dP's accumulators start from
+            // -delta, the scores' from the bias.
+            __syncthreads();                                  // the window and the first tile are there
+            auto fetch = [&](int kv0, int bufi) {
+                ldr.issue(K + (int64_t)kv0 * ld, n - kv0, Kst[bufi]);
+                ldr.issue(V + (int64_t)kv0 * ld, n - kv0, Vst[bufi]);
+            };
+            if (TILE < kv_end) fetch(TILE, 1);
+            int buf = 0, nbuf = 1;
+            f32x16 minus_delta, sc0, dp0, sc1, dp1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            ones.v[e] = (bf16_t)1.f;
-            minus_delta.v[e] = (bf16_t)0.f;
-        }
-        if (h == 0) {
-            float rest = -delta_q;
+            for (int r = 0; r < 16; ++r) minus_delta[r] = -delta_q;
+            frag_t ka[4], va[4];
+            auto read_frag = [&](int bufi, int t, int s) {
+                ka[s] = frag_rowk(Kst[bufi], t * 32 + c, s, h);
+                va[s] = frag_rowk(Vst[bufi], t * 32 + c, s, h);
+            };
+            // first reads for the scores of block (nb, nt) of the tile at nk0
+            auto prepare = [&](f32x16 &xs, int nb, int nt, int nk0) {
+                xs = bias_tile(win + rel.at<32>(nk0 + nt * 32 - qw, c, h));
+                read_frag(nb, nt, 0);
+                read_frag(nb, nt, 1);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            // dS, dQ and the table's sums of block (cbuf, t) at key k0, whose scores and dP - delta are in (sc, dp), and the scores of
+            // block (nb, nt) into (xs, xd).  Behind the last block that is some old tile's data, whose result nobody uses.
+            auto block = [&](f32x16 &sc, f32x16 &dp, f32x16 &xs, f32x16 &xd, int cbuf, int t, int k0, int nb, int nt) {
+                const char *Ks = Kst[cbuf];
+                if (k0 + 32 > n) {                            // keys behind the end
 #pragma unroll
-            for (int e = 0; e < 3; ++e) {
-                minus_delta.v[e] = (bf16_t)rest;
-                rest -= (float)minus_delta.v[e];
-            }
-        }
-        const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * ((S + TILE - 1) / TILE) * 2 + h : nullptr;
-        uint32_t keep = 0xffffffffu, keep_next = 0xffffffffu;
-        if constexpr (DROP) keep_next = keep_row[0];
-        int buf = 0;
-        for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
-            __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the tile has landed
-            __syncthreads();                                  // for everybody, and everybody is done with the other buffer
-            if constexpr (DROP) keep = keep_next;
-            if (kv0 + TILE < kv_end) {
-                const int nx = kv0 + TILE;
-                ldr.issue(K + (int64_t)nx * ld, n - nx, Ks2[buf ^ 1]);
-                ldr.issue(V + (int64_t)nx * ld, n - nx, Vs2[buf ^ 1]);
-                if constexpr (DROP) keep_next = keep_row[(nx / TILE) * 2];
-            }
-            const char *Ks = Ks2[buf], *Vs = Vs2[buf];
-            buf ^= 1;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int k0 = kv0 + t * 32, D = k0 - qw;
-                if (qw >= n || k0 >= n || (CAUSAL && D > 31)) continue;        // nothing here that any query sees
-                const bool whole = k0 + 32 <= n;
-                const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;
-                f32x16 st, dp = zero16();
-                frag_t db[2];
-                frag_t kf[4], vf[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    kf[s] = frag_rowk(Ks, t * 32 + c, s, h);
-                    vf[s] = frag_rowk(Vs, t * 32 + c, s, h);
+                    for (int r = 0; r < 16; ++r)
+                        if (k0 + acc_row(r, h) >= n) sc[r] = -INFINITY;
                 }
-                auto products = [&]() {                       // every group of reads is issued before the arithmetic that hides it
-                    __builtin_amdgcn_sched_barrier(0);
+                auto score = [&](int r) { dp[r] *= __builtin_amdgcn_exp2f(fmaf(sc[r], sl2, nl)); };
+                auto next_scores = [&](int s) { xs = mma(ka[s], qf[s], xs); };
+                frag_t kt[2];
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        st = mma(kf[s], qf[s], st);
-                        dp = mma(vf[s], dof[s], dp);
-                    }
-                    if constexpr (DROP) {                     // (the mask is applied before delta is subtracted)
+                for (int r = 0; r < 4; ++r) score(r);
+                next_scores(0);
+                score(4);
+                score(5);
+                xd = mma(va[0], dof[0], minus_delta);
+                score(6);
+                score(7);
+                frag_t db = acc_to_b(dp, 0);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) dp[r] = ((keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f) - delta_q;
-                    } else {
-                        dp = mma(ones, minus_delta, dp);
-                    }
-                };
-                if (whole && (far_hi || far_lo)) {            // one bucket for the whole block
-                    st = zero16();
-                    products();
-                    const float off = nl + win[far_hi ? W - 1 : 0] * sl2;
+                for (int u = 0; u < 2; ++u) kt[u] = tr.frag(Ks, u * 32, t * 2);
+                read_frag(nb, nt, 2);
+                next_scores(1);
+                score(8);
+                score(9);
+                xd = mma(va[1], dof[1], xd);
+                read_frag(nb, nt, 3);
+                score(10);
+                dqt[0] = mma(kt[0], db, dqt[0]);
+                score(11);
+                kt[0] = tr.frag(Ks, 0, t * 2 + 1);
+                dqt[1] = mma(kt[1], db, dqt[1]);
+                score(12);
+                kt[1] = tr.frag(Ks, 32, t * 2 + 1);
+                next_scores(2);
+                score(13);
+                xd = mma(va[2], dof[2], xd);
+                score(14);
+                score(15);
+                db = acc_to_b(dp, 1);
+                next_scores(3);
+                xd = mma(va[3], dof[3], xd);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) dqt[u] = mma(kt[u], db, dqt[u]);
+                const int D = k0 - qw;
+                const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;
+                if (far_hi || far_lo) {
                     float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        dp[r] *= __builtin_amdgcn_exp2f(fmaf(st[r], sl2, off));
-                        sum += dp[r];
-                    }
+                    for (int r = 0; r < 16; ++r) sum += dp[r];
                     far_sum[far_hi ? 1 : 0] += sum;
-                    db[0] = acc_to_b(dp, 0);
-                    db[1] = acc_to_b(dp, 1);
                 } else {
-                    const int at = rel.at<32>(D, c, h);
-                    st = bias_tile(win + at);
-                    products();
-                    if (!whole) {
+                    own[rel.at<32>(D, 0, 0) + 31 - lane] += diagonal_sums(dp);
+                }
+            };
+            sc0 = bias_tile(win + rel.at<32>(-qw, c, h));
+            dp0 = minus_delta;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (k0 + acc_row(r, h) >= n) st[r] = -INFINITY;
+            for (int s = 0; s < 4; ++s) {
+                read_frag(0, 0, s);
+                sc0 = mma(ka[s], qf[s], sc0);
+                dp0 = mma(va[s], dof[s], dp0);
+            }
+            prepare(sc1, 0, 1, 0);
+            for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
+                block(sc0, dp0, sc1, dp1, buf, 0, kv0, buf, 1);
+                const int fbuf = nbuf == NST - 1 ? 0 : nbuf + 1;
+                __builtin_amdgcn_s_waitcnt(0x0F70);           // vmcnt(0): the next tile has landed
+                __syncthreads();                              // for everybody, and everybody is done with the tile before this one
+                if (kv0 + 2 * TILE < kv_end) fetch(kv0 + 2 * TILE, fbuf);
+                prepare(sc0, nbuf, 0, kv0 + TILE);
+                block(sc1, dp1, sc0, dp0, buf, 1, kv0 + 32, nbuf, 0);
+                prepare(sc1, nbuf, 1, kv0 + TILE);
+                buf = nbuf;
+                nbuf = fbuf;
+            }
+        } else {
+            // dP - delta in the matrix pipe: a product of ones (every key row) and -delta_q cut into three bf16 terms, which hold all 24
+            // bits of it; one matrix instruction a block in place of 16 subtractions a lane
+            frag_t ones, minus_delta;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                ones.v[e] = (bf16_t)1.f;
+                minus_delta.v[e] = (bf16_t)0.f;
+            }
+            if (h == 0) {
+                float rest = -delta_q;
+#pragma unroll
+                for (int e = 0; e < 3; ++e) {
+                    minus_delta.v[e] = (bf16_t)rest;
+                    rest -= (float)minus_delta.v[e];
+                }
+            }
+            const uint32_t *keep_row = DROP ? keep_rows + ((int64_t)bh * S + (q < S ? q : S - 1)) * ((S + TILE - 1) / TILE) * 2 + h : nullptr;
+            uint32_t keep = 0xffffffffu, keep_next = 0xffffffffu;
+            if constexpr (DROP) keep_next = keep_row[0];
+            int buf = 0;
+            for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
+                __builtin_amdgcn_s_waitcnt(0x0F70);               // vmcnt(0): the tile has landed
+                __syncthreads();                                  // for everybody, and everybody is done with the other buffer
+                if constexpr (DROP) keep = keep_next;
+                if (kv0 + TILE < kv_end) {
+                    const int nx = kv0 + TILE;
+                    ldr.issue(K + (int64_t)nx * ld, n - nx, Kst[buf ^ 1]);
+                    ldr.issue(V + (int64_t)nx * ld, n - nx, Vst[buf ^ 1]);
+                    if constexpr (DROP) keep_next = keep_row[(nx / TILE) * 2];
+                }
+                const char *Ks = Kst[buf], *Vs = Vst[buf];
+                buf ^= 1;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int k0 = kv0 + t * 32, D = k0 - qw;
+                    if (qw >= n || k0 >= n || (CAUSAL && D > 31)) continue;        // nothing here that any query sees
+                    const bool whole = k0 + 32 <= n;
+                    const bool far_hi = D - 31 >= rel.R, far_lo = D + 31 <= -rel.R;
+                    f32x16 st, dp = zero16();
+                    frag_t db[2];
+                    frag_t kf[4], vf[4];
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        kf[s] = frag_rowk(Ks, t * 32 + c, s, h);
+                        vf[s] = frag_rowk(Vs, t * 32 + c, s, h);
+                    }
+                    auto products = [&]() {                       // every group of reads is issued before the arithmetic that hides it
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            st = mma(kf[s], qf[s], st);
+                            dp = mma(vf[s], dof[s], dp);
+                        }
+                        if constexpr (DROP) {                     // (the mask is applied before delta is subtracted)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) dp[r] = ((keep & (1u << (t * 16 + r))) ? dp[r] * keep_scale : 0.f) - delta_q;
+                        } else {
+                            dp = mma(ones, minus_delta, dp);
+                        }
+                    };
+                    if (whole && (far_hi || far_lo)) {            // one bucket for the whole block
+                        st = zero16();
+                        products();
+                        const float off = nl + win[far_hi ? W - 1 : 0] * sl2;
+                        float sum = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            dp[r] *= __builtin_amdgcn_exp2f(fmaf(st[r], sl2, off));
+                            sum += dp[r];
+                        }
+                        far_sum[far_hi ? 1 : 0] += sum;
+                        db[0] = acc_to_b(dp, 0);
+                        db[1] = acc_to_b(dp, 1);
+                    } else {
+                        const int at = rel.at<32>(D, c, h);
+                        st = bias_tile(win + at);
+                        products();
+                        if (!whole) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                if (k0 + acc_row(r, h) >= n) st[r] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) dp[r] *= __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl));
+                        db[0] = acc_to_b(dp, 0);
+                        db[1] = acc_to_b(dp, 1);
+                        asm volatile("" : "+v"(db[0].v), "+v"(db[1].v));      // rounded here: the sums below then need no copies of dp
+                        // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
+                        own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) dp[r] *= __builtin_amdgcn_exp2f(fmaf(st[r], sl2, nl));
-                    db[0] = acc_to_b(dp, 0);
-                    db[1] = acc_to_b(dp, 1);
-                    asm volatile("" : "+v"(db[0].v), "+v"(db[1].v));      // rounded here: the sums below then need no copies of dp
-                    // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
-                    own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
-                }
+                    for (int sp = 0; sp < 2; ++sp) {
 #pragma unroll
-                for (int sp = 0; sp < 2; ++sp) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) dqt[u] = mma(tr.frag(Ks, u * 32, t * 2 + sp), db[sp], dqt[u]);
+                        for (int u = 0; u < 2; ++u) dqt[u] = mma(tr.frag(Ks, u * 32, t * 2 + sp), db[sp], dqt[u]);
+                    }
                 }
             }
         }
@@ -603,7 +709,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_bwd_dq_kernel(const Rel
     }
     // the block's bucket sums: window words over the four waves, then every bucket's range by a group of eight lanes
     __syncthreads();                                          // (everybody is done with the tiles, too)
-    store_rows(Ks2[0] + wave * 4096, dqkv + ((int64_t)b * S + qw) * ld + hh * HD, ld, S - qw,
+    store_rows(Kst[0] + wave * 4096, dqkv + ((int64_t)b * S + qw) * ld + hh * HD, ld, S - qw,
                [&](int u, int i) { return qok ? dqt[u][i] * scale : 0.f; });
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));                            // addresses below are not worth registers in the loop above
@@ -936,6 +1042,13 @@ int check_shape(const char *name, int64_t b, int64_t S, int64_t H, float scale, 
     return HAPMI_OK;
 }
 
+// Whether two blocks on each of the 256 CUs hold the whole launch.  Then a third wave a SIMD has nothing to work on, and the kernels that
+// keep two busy with the next block's scores are ahead (dQ, two a CU for three: [2, 2048] x 16 heads, 512 blocks, 69.9 us for 74.7;
+// [1, 4096] x 8 causal, 256 blocks, 80.6 for 90.9; [8, 512] x 16, 512 blocks, 29.0 for 29.7), beyond it they are behind ([12, 512] x 16
+// heads, 768 blocks: 46.0 for 41.8; [2, 4096] causal, 1024 blocks: 147 for 141).  Of a padded batch two thirds are taken to be there
+// ([6, 1001] x 12 heads of 334 .. 1001 tokens, 576 blocks: 48.6 for 50.6).
+bool fits_two_a_cu(int64_t blocks, bool padded) { return (padded ? blocks * 2 / 3 : blocks) <= 2 * 256; }
+
 bool aligned(const void *p, uintptr_t n) { return (uintptr_t)p % n == 0; }
 
 // more than 64 KiB of LDS a block has to be asked for once per kernel and device; asking again is harmless
@@ -1025,8 +1138,9 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
         HAPMI_CHECK_LAUNCH(name);
         return HAPMI_OK;
     };
-    if (causal) rc = drop ? dq(relbias_bwd_dq_kernel<true, true>) : dq(relbias_bwd_dq_kernel<true, false>);
-    else rc = drop ? dq(relbias_bwd_dq_kernel<false, true>) : dq(relbias_bwd_dq_kernel<false, false>);
+    if (drop) rc = causal ? dq(relbias_bwd_dq_kernel<true, true, false>) : dq(relbias_bwd_dq_kernel<false, true, false>);
+    else if (fits_two_a_cu(row_blocks * b * H, lengths != nullptr)) rc = causal ? dq(relbias_bwd_dq_kernel<true, false, true>) : dq(relbias_bwd_dq_kernel<false, false, true>);
+    else rc = causal ? dq(relbias_bwd_dq_kernel<true, false, false>) : dq(relbias_bwd_dq_kernel<false, false, false>);
     if (rc) return rc;
     if (causal) return drop ? dkv(relbias_bwd_dkv_kernel<true, true>) : dkv(relbias_bwd_dkv_kernel<true, false>);
     return drop ? dkv(relbias_bwd_dkv_kernel<false, true>) : dkv(relbias_bwd_dkv_kernel<false, false>);

@@ -82,6 +82,26 @@ def test_forward_and_backward(cuda, b, S, H, n, reach, two, causal):
     compare(res, qkv, table, dout, H, reach, two, causal)
 
 
+@pytest.mark.parametrize("b,S,H,n,reach,two,causal", [
+    (65, 40, 8, 32, 128, True, False), (65, 33, 8, 6, 9, False, True), (40, 150, 8, 32, 128, False, True), (33, 257, 6, 10, 40, True, False)])
+def test_launches_that_fill_the_card(cuda, b, S, H, n, reach, two, causal):
+    """More than two blocks a compute unit: dQ's other form."""
+    qkv, table, dout = make(S + n, b, S, H, n)
+    res = run(cuda, qkv, table, dout, H, max_distance=reach, bidirectional=two, causal=causal)
+    compare(res, qkv, table, dout, H, reach, two, causal)
+
+
+def test_padded_batch_that_fills_the_card(cuda):
+    lengths = [(37 * i) % 151 for i in range(100)]
+    qkv, table, dout = make(3, 100, 150, 8, 32)
+    for z, n in enumerate(lengths):
+        qkv[z, n:] = 0
+        dout[z, n:] = 0
+    for causal in (False, True):
+        res = run(cuda, qkv, table, dout, 8, lengths=lengths, causal=causal)
+        compare(res, qkv, table, dout, 8, 128, not causal, causal, lengths)
+
+
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("S,lengths", [(65, [65, 0, 1, 64]), (200, [129, 128, 33, 200]), (300, [0, 0, 0, 7]), (17, [17, -5, 900, 16])])
 def test_padded_batches(cuda, S, lengths, causal):
