@@ -252,12 +252,13 @@ __device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) 
 // ---------------------------------------------------------------------------------------------
 // One pass over the keys with a running maximum and sum; a wave holds 32 queries, a block of four waves 128, and the 64-key
 // tiles pass through three LDS stages, so that a transfer has two tiles' arithmetic to arrive in.  Three blocks a CU: all 768
-// of the encoder shape are resident at once.  Bound by vector instructions: a score costs a multiply-add, an exponential, an
-// addition, half a maximum and half a conversion.  [12, 512] x 16 heads: 24 us, 0.54 PFLOP/s, vector pipe 62 % and matrix pipe
+// of the encoder shape are resident at once.  Bound by vector instructions: a score costs a multiply-add, an exponential (at a
+// quarter of the rate), an addition, half a maximum and half a conversion, 28 cycles, against 16 of the matrix pipe.  [12, 512] x 16 heads: 24 us, 0.54 PFLOP/s, vector pipe 62 % and matrix pipe
 // 28 % of the cycles (8 us of it fixed: launch, prologue, results); [1, 8192] x 16 heads, causal: 164 .. 179 us from card to
 // card, 0.80 PFLOP/s of the visible half, vector pipe 72 %, matrix pipe 42 %, HBM 65 + 17 MB.
 // Without effect or worse: four parallel chains for the maximum, products pinned between the exponentials (184 for 177 us), no
-// maximum unless a sum of weights gets large (198 us: the test stands between the exponentials and the products).
+// maximum unless a sum of weights gets large (198 us: the test stands between the exponentials and the products), the next tile's
+// scores between this one's exponentials with two waves a SIMD (0 to 5 % slower even where the card is half empty).
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArgs rel, const bf16_t *qkv, bf16_t *out, float *lse,
                                                                const int32_t *lengths, int S, int H, float scale,
