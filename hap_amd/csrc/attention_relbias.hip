@@ -19,9 +19,10 @@
 // lanes 0 .. 31 with zeros above: the swap of half waves delivers that for the two rows of an accumulator register at
 // once.  That is 4 vector instructions a register, and no atomics: LDS float additions of the 16 registers cost 180 cycles
 // each on this chip (the dQ kernel of [12, 512] x 16 heads took 274 us with them and 46 us without; 38 us by now).  The vector is
-// added to the wave's own
-// window in LDS; the block adds its four windows and sums the buckets' ranges, the dK / dV kernel adds the blocks, all in a
+// added to the wave's own window in LDS; the block adds its four windows and sums the buckets' ranges, the dK / dV kernel adds the blocks, all in a
 // fixed order: the same bits every time.
+#include <atomic>
+
 #include "common.h"
 #include "attention_tile.h"
 
@@ -1052,10 +1053,16 @@ bool fits_two_a_cu(int64_t blocks, bool padded) { return (padded ? blocks * 2 / 
 
 bool aligned(const void *p, uintptr_t n) { return (uintptr_t)p % n == 0; }
 
-// more than 64 KiB of LDS a block has to be asked for once per kernel and device; asking again is harmless
-template <typename F> int allow_lds(const char *name, F kernel, size_t bytes) {
-    const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+// More than 64 KiB of LDS a block has to be asked for, once per kernel and device (`asked`: a bit for every device); each time would
+// cost the host as much as the checks of all operands.  Asking again is harmless: two threads may.
+template <typename F> int allow_lds(const char *name, F kernel, size_t most, std::atomic<uint64_t> &asked) {
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (e == hipSuccess && (asked.load(std::memory_order_relaxed) & bit)) return HAPMI_OK;
+    if (e == hipSuccess) e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     HAPMI_REQUIRE(e == hipSuccess, HAPMI_ELAUNCH, "%s: %s", name, hipGetErrorString(e));
+    asked.fetch_or(bit, std::memory_order_relaxed);
     return HAPMI_OK;
 }
 
@@ -1123,9 +1130,10 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
     const float ks = drop ? 1.0f / (1.0f - p) : 1.0f;
     hipStream_t st = (hipStream_t)stream;
     dim3 grid((unsigned)row_blocks, (unsigned)(b * H)), block(AT_THREADS);
-    auto dq = [&](auto kernel) -> int {
+    static std::atomic<uint64_t> asked[6];                    // one for each of dQ's kernels
+    auto dq = [&](auto kernel, int which) -> int {
         const size_t lds = (size_t)dq_lds_words(W) * 4;
-        rc = allow_lds(name, kernel, lds);
+        rc = allow_lds(name, kernel, (size_t)dq_lds_words(window_of(REL_MAX_REACH)) * 4, asked[which]);
         if (rc) return rc;
         hipLaunchKernelGGL(kernel, grid, block, lds, st, a, (const bf16_t *)qkv, (const bf16_t *)out, (const bf16_t *)dout, lse, delta_ws,
                            (bf16_t *)dqkv, workspace, lengths, (int)S, (int)H, scale, keep_rows, ks);
@@ -1139,9 +1147,9 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
         HAPMI_CHECK_LAUNCH(name);
         return HAPMI_OK;
     };
-    if (drop) rc = causal ? dq(relbias_bwd_dq_kernel<true, true, false>) : dq(relbias_bwd_dq_kernel<false, true, false>);
-    else if (fits_two_a_cu(row_blocks * b * H, lengths != nullptr)) rc = causal ? dq(relbias_bwd_dq_kernel<true, false, true>) : dq(relbias_bwd_dq_kernel<false, false, true>);
-    else rc = causal ? dq(relbias_bwd_dq_kernel<true, false, false>) : dq(relbias_bwd_dq_kernel<false, false, false>);
+    if (drop) rc = causal ? dq(relbias_bwd_dq_kernel<true, true, false>, 0) : dq(relbias_bwd_dq_kernel<false, true, false>, 1);
+    else if (fits_two_a_cu(row_blocks * b * H, lengths != nullptr)) rc = causal ? dq(relbias_bwd_dq_kernel<true, false, true>, 2) : dq(relbias_bwd_dq_kernel<false, false, true>, 3);
+    else rc = causal ? dq(relbias_bwd_dq_kernel<true, false, false>, 4) : dq(relbias_bwd_dq_kernel<false, false, false>, 5);
     if (rc) return rc;
     if (causal) return drop ? dkv(relbias_bwd_dkv_kernel<true, true>) : dkv(relbias_bwd_dkv_kernel<true, false>);
     return drop ? dkv(relbias_bwd_dkv_kernel<false, true>) : dkv(relbias_bwd_dkv_kernel<false, false>);

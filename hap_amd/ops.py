@@ -1050,25 +1050,23 @@ def relative_bucket_starts(n_buckets: int, max_distance: int, bidirectional: boo
 
 @functools.lru_cache(maxsize=None)
 def _bucket_array(n_buckets, max_distance, bidirectional):
+    """The buckets' first distances for the C ABI, and their address."""
     starts = relative_bucket_starts(n_buckets, max_distance, bidirectional)
-    return (ctypes.c_int32 * len(starts))(*starts)
+    array = (ctypes.c_int32 * len(starts))(*starts)
+    return array, ctypes.addressof(array)
 
 
 def _relbias(what, table, H, max_distance, bidirectional, causal):
     """The bias description of the C ABI; ``table`` may be the columns of a wider one."""
-    if table.dim() != 2 or table.shape[1] != H or table.dtype != torch.float32 or (H > 1 and table.stride(1) != 1) or table.stride(0) < H:
+    shape, stride = table.shape, table.stride()
+    if len(shape) != 2 or shape[1] != H or table.dtype != torch.float32 or (H > 1 and stride[1] != 1) or stride[0] < H:
         raise ValueError(f"{what}: the table must be a float32 [buckets, {H}] tensor with unit column stride and rows apart")
-    n = table.shape[0]
+    n = shape[0]
     bidirectional = (not causal) if bidirectional is None else bool(bidirectional)
-    arr = _bucket_array(n, int(max_distance), bidirectional)
-    a = _lib.RelBias(table.data_ptr(), table.stride(0), n, bidirectional, ctypes.addressof(arr))
-    a._keep = arr
+    array, address = _bucket_array(n, int(max_distance), bidirectional)
+    a = _lib.RelBias(table.data_ptr(), stride[0], n, bidirectional, address)
+    a._keep = array
     return a
-
-
-def _rows_span(t):
-    """Address range of a 2-d tensor of float32 rows that may be strided."""
-    return t.data_ptr(), t.data_ptr() + 4 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])
 
 
 _RELBIAS_FWD_TYPES = (torch.bfloat16, torch.float32, torch.bfloat16, torch.int32, torch.int32)
@@ -1108,8 +1106,7 @@ def attention_relbias_workspace_elems(table, b, S, H, max_distance=128, bidirect
 
 @functools.lru_cache(maxsize=256)
 def _relbias_workspace_elems(n_buckets, max_distance, bidirectional, b, S, H):
-    arr = _bucket_array(n_buckets, max_distance, bidirectional)
-    rel = _lib.RelBias(0, H, n_buckets, bidirectional, ctypes.addressof(arr))
+    rel = _lib.RelBias(0, H, n_buckets, bidirectional, _bucket_array(n_buckets, max_distance, bidirectional)[1])
     need = ctypes.c_int64()
     check(_lib._load().hapmi_attention_relbias_workspace_elems(ctypes.byref(rel), b, S, H, ctypes.byref(need)))
     return need.value
@@ -1123,20 +1120,25 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     ``workspace``: float32 scratch of ``attention_relbias_workspace_elems`` (None: taken from torch's allocator)."""
     what = "attention_relbias_bwd"
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
-    if dtable.shape != table.shape or dtable.dtype != torch.float32 or (H > 1 and dtable.stride(1) != 1) or dtable.stride(0) < H:
+    stride = dtable.stride()
+    if dtable.shape != table.shape or dtable.dtype != torch.float32 or (H > 1 and stride[1] != 1) or stride[0] < H:
         raise ValueError(f"{what}: dtable must be float32 of the table's shape with unit column stride and rows apart")
     if (keep_rows is None) != (keep_cols is None):
         raise ValueError(f"{what}: keep_rows and keep_cols come together")
-    _on_device(what, table, qkv)
-    _on_device(what, dtable, qkv)
-    _apart(what, [(*_rows_span(table), False), (*_rows_span(dtable), True)])
-    need = attention_relbias_workspace_elems(table, b, S, H, max_distance, bidirectional, causal)
+    device = qkv.get_device()
+    if table.get_device() != device or dtable.get_device() != device:
+        _on_device(what, table, qkv)
+        _on_device(what, dtable, qkv)
+    grad, last = dtable.data_ptr(), rel.n_buckets - 1
+    if grad < rel.table + 4 * (last * rel.ld + H) and rel.table < grad + 4 * (last * stride[0] + H):
+        raise ValueError(f"{what}: an output shares memory with another operand")
+    need = _relbias_workspace_elems(rel.n_buckets, max_distance, rel.bidirectional, b, S, H)
     workspace = _scratch(what, workspace, need, qkv.device)
     n, words = b * S * H, attention_keep_words(b, S, H) if keep_rows is not None else 0
     stream, (dq_, dl_, ws_, q_, o_, do_, l_, n_, kr_, kc_) = _operands(
         what, ("dqkv", "delta_ws", "workspace", "qkv", "out", "dout", "lse", "lengths", "keep_rows", "keep_cols"), _RELBIAS_BWD_TYPES,
         (dqkv, delta_ws, workspace, qkv, out, dout, lse, lengths, keep_rows, keep_cols), (n * 192, n, need, n * 192, n * 64, n * 64, n, b, words, words), 3, ("lengths",))
-    check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), dtable.stride(0), accumulate,
+    check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, grad, stride[0], accumulate,
                                             dl_, _kept(ws_, workspace), workspace.numel(), b, S, H, scale, kr_, kc_, p, stream))
 
 
