@@ -107,7 +107,7 @@ struct TileStream {
         const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char *)lds_tile + wave * 1024;
         int o[LOADS] = {off, off};
         const bf16_t *from[LOADS] = {base, base + 32 * ld};
-        if (rows_left < TILE) {
+        if (__builtin_expect(rows_left < TILE, 0)) {
             int tid = threadIdx.x;
             asm volatile("" : "+v"(tid));                     // (nothing of this is kept in registers over the whole tiles)
             from[1] = base;
@@ -142,12 +142,15 @@ __device__ __forceinline__ void issue_own_rows(const bf16_t *first_row, int ld, 
                      : "memory");
     }
 }
-__device__ __forceinline__ void own_frags(const char *lds, int c, int h, bool valid, frag_t (&f)[4]) {
+__device__ __forceinline__ void own_frags(const char *lds, int c, int h, int rows, frag_t (&f)[4]) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) f[s] = frag_rowk(lds, c, s, h);
+    if (rows >= 32) return;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        f[s] = frag_rowk(lds, c, s, h);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[s].v[e] = valid ? f[s].v[e] : (bf16_t)0.f;
+        const u32x4 bits = __builtin_bit_cast(u32x4, f[s].v);
+        f[s].v = __builtin_bit_cast(bf16x8, c < rows ? bits : (u32x4)(0u));
     }
 }
 
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
         __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): queries and first tile have landed
         if (TILE < kv_end) issue_tile(TILE, 1);
         frag_t qf[4];
-        own_frags(own, c, h, q < n, qf);
+        own_frags(own, c, h, n - qw, qf);
         int buf = 0;
         for (int kv0 = 0; kv0 < kv_end; kv0 += TILE) {
             if (kv0 + TILE < kv_end) __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | PER_TILE);   // vmcnt: only the next tile may be outstanding
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
                 for (int s = 0; s < 4; ++s)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) st[t] = mma(kf[t][s], qf[s], st[t]);
-                if (!whole) {
+                if (__builtin_expect(!whole, 0)) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -477,8 +480,8 @@ __global__ __launch_bounds__(AT_THREADS, AHEAD ? 2 : 3) void relbias_bwd_dq_kern
         rel.expand<false, CAUSAL>(win, hh, scale);            // published by the loop's first barrier
         __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): queries, dO and the first tile have landed
         frag_t qf[4], dof[4];
-        own_frags(own_q, c, h, qok, qf);
-        own_frags(own_do, c, h, qok, dof);
+        own_frags(own_q, c, h, n - qw, qf);
+        own_frags(own_do, c, h, n - qw, dof);
         float delta_q = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -525,7 +528,7 @@ __global__ __launch_bounds__(AT_THREADS, AHEAD ? 2 : 3) void relbias_bwd_dq_kern
             // block (nb, nt) into (xs, xd).  Behind the last block that is some old tile's data, whose result nobody uses.
             auto block = [&](f32x16 &sc, f32x16 &dp, f32x16 &xs, f32x16 &xd, int cbuf, int t, int k0, int nb, int nt) {
                 const char *Ks = Kst[cbuf];
-                if (k0 + 32 > n) {                            // keys behind the end
+                if (__builtin_expect(k0 + 32 > n, 0)) {                            // keys behind the end
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (k0 + acc_row(r, h) >= n) sc[r] = -INFINITY;
@@ -677,7 +680,7 @@ __global__ __launch_bounds__(AT_THREADS, AHEAD ? 2 : 3) void relbias_bwd_dq_kern
                         const int at = rel.at<32>(D, c, h);
                         st = bias_tile(win + at);
                         products();
-                        if (!whole) {
+                        if (__builtin_expect(!whole, 0)) {
 #pragma unroll
                             for (int r = 0; r < 16; ++r)
                                 if (k0 + acc_row(r, h) >= n) st[r] = -INFINITY;
@@ -828,8 +831,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
         if constexpr (DROP) keep2 = keep2_next;
         __builtin_amdgcn_s_waitcnt(0x0F70);                   // vmcnt(0): keys, values and the first tile have landed
         frag_t kf[4], vf[4];
-        own_frags(Qs3[1] + wave * 4096, c, h, kok, kf);
-        own_frags(dOs3[1] + wave * 4096, c, h, kok, vf);
+        own_frags(Qs3[1] + wave * 4096, c, h, n - kvw, kf);
+        own_frags(dOs3[1] + wave * 4096, c, h, n - kvw, vf);
         __syncthreads();
         int buf = 0, nbuf = 1;
         if (q_begin + TILE < n) fetch(q_begin + TILE, 1);
