@@ -255,9 +255,9 @@ __device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) 
 // One pass over the keys with a running maximum and sum; a wave holds 32 queries, a block of four waves 128, and the 64-key
 // tiles pass through three LDS stages, so that a transfer has two tiles' arithmetic to arrive in.  Three blocks a CU: all 768
 // of the encoder shape are resident at once.  Bound by vector instructions: a score costs a multiply-add, an exponential (at a
-// quarter of the rate), an addition, half a maximum and half a conversion, 28 cycles, against 16 of the matrix pipe.  [12, 512] x 16 heads: 24 us, 0.54 PFLOP/s, vector pipe 62 % and matrix pipe
-// 28 % of the cycles (8 us of it fixed: launch, prologue, results); [1, 8192] x 16 heads, causal: 164 .. 179 us from card to
-// card, 0.80 PFLOP/s of the visible half, vector pipe 72 %, matrix pipe 42 %, HBM 65 + 17 MB.
+// quarter of the rate), an addition, half a maximum and half a conversion, 28 cycles, against 16 of the matrix pipe.  [12, 512] x 16 heads: 24 us, 0.54 PFLOP/s, vector pipe 58 % and matrix pipe
+// 28 % of the cycles (8 us of it fixed: launch, prologue, results); [1, 8192] x 16 heads, causal: 164 .. 185 us as the power limit
+// lets it, 0.80 PFLOP/s of the visible half, vector pipe 70 %, matrix pipe 41 %, HBM 67 + 17 MB.
 // Without effect or worse: four parallel chains for the maximum, products pinned between the exponentials (184 for 177 us), no
 // maximum unless a sum of weights gets large (198 us: the test stands between the exponentials and the products), the next tile's
 // scores between this one's exponentials with two waves a SIMD (0 to 5 % slower even where the card is half empty).
@@ -419,9 +419,9 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // ---------------------------------------------------------------------------------------------
 // 13 matrix products and about 80 vector instructions a lane for a 32 x 32 block of scores, 64 more where it touches the bias
 // window (the diagonal sums).  Three waves a SIMD hide each other's latencies; where the launch does not fill the card, two
-// that also work on the next block's scores are faster (AHEAD; fits_two_a_cu has both sides).  [12, 512] x 16 heads: 38 us, matrix pipe 27 %, vector pipe
-// 54 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one; [2, 4096] x 16 heads, causal:
-// 137 us, matrix pipe 43 %, vector pipe 61 %.
+// that also work on the next block's scores are faster (AHEAD; fits_two_a_cu has both sides).  [12, 512] x 16 heads: 38 us, matrix pipe 28 %, vector pipe
+// 51 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one; [2, 4096] x 16 heads, causal:
+// 137 .. 142 us, matrix pipe 44 %, vector pipe 61 %.
 __host__ __device__ __forceinline__ int round4(int n) { return (n + 3) & ~3; }
 // a window, and the waves' sums, whose room their dO rows pass through first
 __host__ __device__ __forceinline__ int dq_lds_words(int W) { return round4(W) + (W > 1024 ? 4 * round4(W) : 4096); }
@@ -768,8 +768,8 @@ __device__ __forceinline__ void table_gradient(const float *part, float *dtable,
 // lse = +inf, and dP starts from -delta.  Plain blocks with three waves a SIMD instead: 36.9 us for 37.3 on [12, 512] x 16 heads,
 // but 29.0 for 25.2 us on [8, 512] and 88 for 74 us on [2, 2048].  What it spends adds up rather than overlaps (leaving out the
 // matrix products 108 of 182 us on [4, 2048], the LDS reads 138, the exponentials 178).  [12, 512] x 16 heads: 38 us, 0.68
-// PFLOP/s, matrix pipe 34 %, vector pipe 43 %, LDS 39 %, HBM 51 + 25 MB; [2, 4096] x 16 heads, causal: 153 .. 161 us, matrix
-// pipe 46 %, vector pipe 46 %, LDS 48 %.
+// PFLOP/s, matrix pipe 34 %, vector pipe 40 %, LDS 39 %, HBM 51 + 25 MB; [2, 4096] x 16 heads, causal: 153 .. 167 us, matrix
+// pipe 47 %, vector pipe 46 %, LDS 49 %.
 template <bool CAUSAL, bool DROP>
 __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const RelArgs rel, const bf16_t *qkv, const bf16_t *dout,
                                                                    const float *lse, const float *delta, bf16_t *dqkv,
