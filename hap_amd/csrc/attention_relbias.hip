@@ -28,7 +28,6 @@
 
 namespace {
 
-
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int REL_MAX_SIDE = HAPMI_RELBIAS_MAX_SIDE;
 constexpr int REL_MAX_REACH = HAPMI_RELBIAS_MAX_REACH;
@@ -419,9 +418,9 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // ---------------------------------------------------------------------------------------------
 // 13 matrix products and about 80 vector instructions a lane for a 32 x 32 block of scores, 64 more where it touches the bias
 // window (the diagonal sums).  Three waves a SIMD hide each other's latencies; where the launch does not fill the card, two
-// that also work on the next block's scores are faster (AHEAD; fits_two_a_cu has both sides).  [12, 512] x 16 heads: 38 us, matrix pipe 28 %, vector pipe
-// 51 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one; [2, 4096] x 16 heads, causal:
-// 137 .. 142 us, matrix pipe 44 %, vector pipe 61 %.
+// that also work on the next block's scores are faster (AHEAD; fits_two_a_cu has both sides).  [12, 512] x 16 heads: 38 us,
+// matrix pipe 28 %, vector pipe 51 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one;
+// [2, 4096] x 16 heads, causal: 137 .. 142 us, matrix pipe 44 %, vector pipe 61 %.
 __host__ __device__ __forceinline__ int round4(int n) { return (n + 3) & ~3; }
 // a window, and the waves' sums, whose room their dO rows pass through first
 __host__ __device__ __forceinline__ int dq_lds_words(int W) { return round4(W) + (W > 1024 ? 4 * round4(W) : 4096); }
