@@ -21,6 +21,10 @@ class HapmiError(RuntimeError):
     pass
 
 
+class SharedMemoryError(HapmiError, ValueError):
+    """An output shares memory with another operand (HAPMI_EALIAS)."""
+
+
 GEMM_MAX_SEGMENTS = 8
 
 
@@ -164,4 +168,4 @@ def _load() -> ctypes.CDLL:
 
 def check(rc: int) -> None:
     if rc != 0:
-        raise HapmiError(f"libhapmi error {rc}: {_load().hapmi_last_error().decode()}")
+        raise (SharedMemoryError if rc == -6 else HapmiError)(f"libhapmi error {rc}: {_load().hapmi_last_error().decode()}")

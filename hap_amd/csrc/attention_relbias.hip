@@ -1058,6 +1058,10 @@ bool fits_two_a_cu(int64_t blocks, bool padded) { return (padded ? blocks * 2 / 
 
 bool aligned(const void *p, uintptr_t n) { return (uintptr_t)p % n == 0; }
 
+// a strided float32 [n][ld] matrix of H columns; a row stride beyond any memory counts as 2^40
+HapmiSpan rows_span(const float *p, int64_t n, int64_t ld, int64_t H) { return {p, ((n - 1) * (ld < (1ll << 40) ? ld : 1ll << 40) + H) * 4}; }
+int64_t keep_bytes(int64_t b, int64_t S, int64_t H) { return b * H * S * 2 * hapmi_cdiv(S, TILE) * 4; }
+
 // More than 64 KiB of LDS a block has to be asked for, once per kernel and device (`asked`: a bit for every device); each time would
 // cost the host as much as the checks of all operands.  Asking again is harmless: two threads may.
 template <typename F> int allow_lds(const char *name, F kernel, size_t most, std::atomic<uint64_t> &asked) {
@@ -1085,6 +1089,10 @@ extern "C" int hapmi_attention_relbias_fwd(const void *qkv, const hapmi_relbias 
     HAPMI_REQUIRE(qkv && out && lse && a.table, HAPMI_EINVAL, "%s: null pointer", name);
     HAPMI_REQUIRE(aligned(qkv, 16) && aligned(out, 16) && aligned(keep_rows, 8) && aligned(lse, 4) && aligned(a.table, 4) && aligned(lengths, 4),
                   HAPMI_EALIGN, "%s: qkv and out must be 16-byte aligned (keep words: 8)", name);
+    const int64_t n = b * S * H;
+    rc = hapmi_apart(name, {{out, n * 128}, {lse, n * 4}},
+                     {{qkv, n * 384}, rows_span(a.table, bias_host->n_buckets, a.ld, H), {lengths, b * 4}, {keep_rows, keep_bytes(b, S, H)}});
+    if (rc) return rc;
     const float ks = keep_rows ? 1.0f / (1.0f - p) : 1.0f;
     const size_t lds = (size_t)window_of(a.R) * 4;
     dim3 grid((unsigned)hapmi_cdiv(S, 128), (unsigned)(b * H)), block(AT_THREADS);
@@ -1131,6 +1139,11 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
     const int64_t row_blocks = hapmi_cdiv(S, 128);
     const int64_t need = b * H * row_blocks * bias_host->n_buckets;
     HAPMI_REQUIRE(workspace_elems >= need, HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name, (long long)workspace_elems, (long long)need);
+    const int64_t n = b * S * H;
+    rc = hapmi_apart(name, {{dqkv, n * 384}, rows_span(dtable, bias_host->n_buckets, ld_dtable, H), {delta_ws, n * 4}, {workspace, need * 4}},
+                     {{qkv, n * 384}, rows_span(a.table, bias_host->n_buckets, a.ld, H), {out, n * 128}, {dout, n * 128}, {lse, n * 4}, {lengths, b * 4},
+                      {keep_rows, keep_bytes(b, S, H)}, {keep_cols, keep_bytes(b, S, H)}});
+    if (rc) return rc;
     const bool drop = keep_rows != nullptr;
     const float ks = drop ? 1.0f / (1.0f - p) : 1.0f;
     hipStream_t st = (hipStream_t)stream;

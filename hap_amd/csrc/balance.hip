@@ -258,6 +258,10 @@ extern "C" int hapmi_balance_loss_fwd(const float *probs, const int32_t *index, 
     const int64_t slab = bal_slab(B, S, E), slabs = hapmi_cdiv(S, slab), n = B * slabs * E;
     HAPMI_REQUIRE(slabs == 1 || (workspace && workspace_elems >= 3 * n), HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name,
                   (long long)(workspace ? workspace_elems : 0), (long long)(3 * n));
+    const int64_t records = B * S * 2 * 4, sums = B * E * 4;
+    const int rc2 = hapmi_apart(name, {{loss, 4}, {counts, sums}, {kept, sums}, {prob_sum, sums}, {slabs > 1 ? workspace : nullptr, 3 * n * 4}},
+                                {{probs, B * S * E * 4}, {index, records}, {slot, records}, {lengths, B * 4}});
+    if (rc2) return rc2;
     int32_t *pc = slabs > 1 ? (int32_t *)workspace : counts, *pk = slabs > 1 ? (int32_t *)workspace + n : kept;
     float *pp = slabs > 1 ? workspace + 2 * n : prob_sum;
     const dim3 grid((unsigned)slabs, (unsigned)B), block(BAL_THREADS);
@@ -291,6 +295,10 @@ extern "C" int hapmi_balance_loss_bwd(const float *probs, const int32_t *index, 
     while ((V << group_log2) < E) ++group_log2;
     HAPMI_REQUIRE(!dgate || ((uintptr_t)index % 8 == 0 && (uintptr_t)slot % 8 == 0 && (uintptr_t)dgate % 8 == 0), HAPMI_EALIGN,
                   "%s: index, slot and dgate must be 8-byte aligned", name);
+    const int64_t records = B * S * 2 * 4;
+    const int rc2 = hapmi_apart(name, {{dlogits, B * S * E * 4}},
+                                {{probs, B * S * E * 4}, {index, records}, {slot, records}, {dgate, records}, {counts, B * E * 4}, {lengths, B * 4}});
+    if (rc2) return rc2;
     const dim3 grid((unsigned)hapmi_cdiv(S, (BAL_THREADS >> group_log2) * BAL_TURNS), (unsigned)B), block(BAL_THREADS);
     if (V == 4) hipLaunchKernelGGL((balance_bwd_kernel<4>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, group_log2);
     else hipLaunchKernelGGL((balance_bwd_kernel<1>), grid, block, 0, (hipStream_t)stream, probs, index, slot, dgate, counts, lengths, dlogits, (int)B, (int)S, (int)E, coef, choices, group_log2);

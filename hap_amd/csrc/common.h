@@ -5,6 +5,8 @@
 #include <stdio.h>
 #include <stdarg.h>
 
+#include <initializer_list>
+
 #include "../../include/hapmi.h"
 
 typedef __bf16 bf16_t;
@@ -24,6 +26,23 @@ int hapmi_sumsq_static_setup();   // elementwise.hip: per-device set-up that hap
     do {                                                         \
         if (!(cond)) return hapmi_set_error((code), __VA_ARGS__); \
     } while (0)
+
+// Refuses outputs that share memory with each other or with an operand that is read (operands that are only read may share).
+struct HapmiSpan {
+    const void *at;                 // NULL: no such operand
+    int64_t bytes;
+};
+inline int hapmi_apart(const char *name, std::initializer_list<HapmiSpan> written, std::initializer_list<HapmiSpan> read) {
+    auto meet = [](const HapmiSpan &a, const HapmiSpan &b) {
+        const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+        return x && y && a.bytes > 0 && b.bytes > 0 && (x <= y ? y - x < (uintptr_t)a.bytes : x - y < (uintptr_t)b.bytes);
+    };
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        for (auto o = w + 1; o != written.end(); ++o) HAPMI_REQUIRE(!meet(*w, *o), HAPMI_EALIAS, "%s: an output shares memory with another operand", name);
+        for (auto &r : read) HAPMI_REQUIRE(!meet(*w, r), HAPMI_EALIAS, "%s: an output shares memory with another operand", name);
+    }
+    return HAPMI_OK;
+}
 
 #define HAPMI_CHECK_LAUNCH(name)                                                        \
     do {                                                                                \

@@ -365,6 +365,10 @@ extern "C" int hapmi_qk_norm_rotary_fwd(const void *qkv, void *out, const float 
     if (b == 0) return HAPMI_OK;
     HAPMI_REQUIRE(qkv && out, HAPMI_EINVAL, "%s: null pointer", name);
     HAPMI_REQUIRE((uintptr_t)qkv % 16 == 0 && (uintptr_t)out % 16 == 0, HAPMI_EALIGN, "%s: qkv and out must be 16-byte aligned", name);
+    const int64_t size = dtype == HAPMI_F32 ? 4 : 2, n = a.rows * 3 * D * size;
+    const int rc2 = hapmi_apart(name, {{out, n}}, {{out == qkv ? nullptr : qkv, n}, {q_gain, D * 4}, {k_gain, D * 4}, {angles, n_pos * rot * 4},
+                                                   {positions, b * S * 4}});
+    if (rc2) return rc2;
     const dim3 grid((unsigned)qn_blocks(a, 1 << 20)), block(QN_THREADS);
     if (dtype == HAPMI_F32) hipLaunchKernelGGL((qk_norm_rotary_fwd_kernel<float>), grid, block, 0, (hipStream_t)stream, a, (const float *)qkv, (float *)out);
     else hipLaunchKernelGGL((qk_norm_rotary_fwd_kernel<bf16_t>), grid, block, 0, (hipStream_t)stream, a, (const bf16_t *)qkv, (bf16_t *)out);
@@ -394,6 +398,10 @@ extern "C" int hapmi_qk_norm_rotary_bwd(const void *dout, const void *qkv, void 
     const bool gains = dq_gain || dk_gain;
     HAPMI_REQUIRE(!gains || (workspace && workspace_elems >= 2 * D * QN_MAX_BLOCKS), HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name,
                   (long long)(workspace ? workspace_elems : 0), (long long)(2 * D * QN_MAX_BLOCKS));
+    const int64_t size = dtype == HAPMI_F32 ? 4 : 2, n = a.rows * 3 * D * size;
+    int rc2 = hapmi_apart(name, {{dqkv, n}, {dq_gain, D * 4}, {dk_gain, D * 4}, {gains ? workspace : nullptr, 2 * D * QN_MAX_BLOCKS * 4}},
+                          {{dout == dqkv ? nullptr : dout, n}, {qkv, n}, {q_gain, D * 4}, {k_gain, D * 4}, {angles, n_pos * rot * 4}, {positions, b * S * 4}});
+    if (rc2) return rc2;
     const int64_t blocks = qn_blocks(a, gains ? QN_MAX_BLOCKS : 1 << 20);
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto kernel, auto zero) -> int {
@@ -402,7 +410,6 @@ extern "C" int hapmi_qk_norm_rotary_bwd(const void *dout, const void *qkv, void 
         HAPMI_CHECK_LAUNCH(name);
         return HAPMI_OK;
     };
-    int rc2;
     if (dtype == HAPMI_F32) rc2 = gains ? go(qk_norm_rotary_bwd_kernel<float, true>, 0.f) : go(qk_norm_rotary_bwd_kernel<float, false>, 0.f);
     else rc2 = gains ? go(qk_norm_rotary_bwd_kernel<bf16_t, true>, (bf16_t)0.f) : go(qk_norm_rotary_bwd_kernel<bf16_t, false>, (bf16_t)0.f);
     if (rc2 || !gains) return rc2;

@@ -74,37 +74,23 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _operands(what, names, dtypes, tensors, elems, written, exact=()):
+def _operands(what, names, dtypes, tensors, elems, exact=()):
     """Checks of a call's tensors in one pass: on the current device, of the element type, contiguous, at least ``elems`` long
-    (those named in ``exact``: just as long), and none of the first ``written`` ones shares memory with another.  None entries
-    are skipped, the first one is a tensor.  Returns the current stream and the pointers (0 for None), in order."""
-    ptrs, spans = [], []
+    (those named in ``exact``: just as long).  None entries are skipped, the first one is a tensor.  Returns the current stream
+    and the pointers (0 for None), in order.  (That no output shares memory with another operand, the library checks.)"""
     cur = tensors[0].get_device()
     if cur < 0 or cur != _current_device():
         _dev(tensors[0])
         raise _lib.HapmiError(f"{what}: {names[0]} is on {tensors[0].device}, not on the current device")
+    ptrs = []
     for t, dtype, n in zip(tensors, dtypes, elems):
         if t is None:
             ptrs.append(0)
             continue
-        size = t.numel()
-        if size != n or t.dtype is not dtype or t.get_device() != cur or not t.is_contiguous():
+        if t.numel() != n or t.dtype is not dtype or t.get_device() != cur or not t.is_contiguous():
             _odd_operand(what, names[len(ptrs)], t, dtype, n, cur, exact)
-        ptr = t.data_ptr()
-        if size:
-            spans.append((ptr, ptr + size * _ITEM[dtype], len(ptrs) < written))
-        ptrs.append(ptr)
-    spans.sort()
-    end = 0
-    for lo, hi, _ in spans:
-        if lo < end:                                                 # shared memory: allowed between operands that are only read
-            _apart(what, spans)
-            break
-        end = hi
+        ptrs.append(t.data_ptr())
     return _raw_stream(cur), ptrs
-
-
-_ITEM = {torch.float32: 4, torch.int32: 4, torch.bfloat16: 2}
 
 
 def _odd_operand(what, name, t, dtype, elems, cur, exact):
@@ -117,17 +103,6 @@ def _odd_operand(what, name, t, dtype, elems, cur, exact):
     if name in exact and t.numel() != elems:
         raise TypeError(f"{what}: {name} must have {elems} elements, not {t.numel()}")
     _need(t, elems, f"{what} {name}")
-
-
-def _apart(what, spans):
-    """No (start, end, written) range that is written may overlap another one."""
-    end = end_written = 0
-    for lo, hi, written in sorted(spans):
-        if lo < end_written or (written and lo < end):
-            raise ValueError(f"{what}: an output shares memory with another operand")
-        end = max(end, hi)
-        if written:
-            end_written = max(end_written, hi)
 
 
 def _scratch(what, workspace, elems: int, device):
@@ -888,12 +863,11 @@ def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None,
     what = "qk_norm_rotary_fwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
     code, n = dtype_code(qkv), b * S * 3 * H * D
-    apart = out.data_ptr() != qkv.data_ptr()
     dt = qkv.dtype
     stream, (o_, x_, q_, k_, r_, p_) = _operands(
         what, ("out", "qkv", "q_gain", "k_gain", "rotary", "positions"), (dt, dt, torch.float32, torch.float32, torch.float32, torch.int32),
-        (out, qkv if apart else None, q_gain, k_gain, rotary, positions), (n, n, D, D, n_pos * rot, b * S), 1, _QK_FWD_EXACT)
-    check(lib().hapmi_qk_norm_rotary_fwd(x_ if apart else o_, o_, q_, k_, r_, n_pos, rot, interleaved, p_, b, S, H, D, eps, code, stream))
+        (out, qkv, q_gain, k_gain, rotary, positions), (n, n, D, D, n_pos * rot, b * S), _QK_FWD_EXACT)
+    check(lib().hapmi_qk_norm_rotary_fwd(x_, o_, q_, k_, r_, n_pos, rot, interleaved, p_, b, S, H, D, eps, code, stream))
 
 
 @functools.lru_cache(maxsize=256)
@@ -916,14 +890,13 @@ def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_ga
         workspace = _scratch(what, workspace, ws_elems, qkv.device)
     else:
         workspace = None
-    apart = dqkv.data_ptr() != dout.data_ptr()
     dt, f32 = qkv.dtype, torch.float32
     stream, (dx_, dq_, dk_, ws_, do_, x_, q_, k_, r_, p_) = _operands(
         what, ("dqkv", "dq_gain", "dk_gain", "workspace", "dout", "qkv", "q_gain", "k_gain", "rotary", "positions"),
         (dt, f32, f32, f32, dt, dt, f32, f32, f32, torch.int32),
-        (dqkv, dq_gain, dk_gain, workspace, dout if apart else None, qkv, q_gain, k_gain, rotary, positions),
-        (n, D, D, ws_elems, n, n, D, D, n_pos * rot, b * S), 4, _QK_BWD_EXACT)
-    check(lib().hapmi_qk_norm_rotary_bwd(do_ if apart else dx_, x_, dx_, q_, k_, dq_, dk_, accumulate, r_, n_pos, rot, interleaved, p_, b, S, H, D,
+        (dqkv, dq_gain, dk_gain, workspace, dout, qkv, q_gain, k_gain, rotary, positions),
+        (n, D, D, ws_elems, n, n, D, D, n_pos * rot, b * S), _QK_BWD_EXACT)
+    check(lib().hapmi_qk_norm_rotary_bwd(do_, x_, dx_, q_, k_, dq_, dk_, accumulate, r_, n_pos, rot, interleaved, p_, b, S, H, D,
                                          eps, code, _kept(ws_, workspace), workspace.numel() if workspace is not None else 0, stream))
 
 
@@ -1087,7 +1060,7 @@ def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128
     what = "attention_relbias_fwd"
     n = b * S * H
     stream, (o_, l_, q_, n_, k_) = _operands(what, ("out", "lse", "qkv", "lengths", "keep_rows"), _RELBIAS_FWD_TYPES, (out, lse, qkv, lengths, keep_rows),
-                                             (n * 64, n, n * 192, b, attention_keep_words(b, S, H) if keep_rows is not None else 0), 2, ("lengths",))
+                                             (n * 64, n, n * 192, b, attention_keep_words(b, S, H) if keep_rows is not None else 0), ("lengths",))
     rel = _relbias(what, table, H, max_distance, bidirectional, causal)
     _on_device(what, table, qkv)
     check(lib().hapmi_attention_relbias_fwd(q_, ctypes.byref(rel), causal, n_, o_, l_, b, S, H, scale, k_, p, stream))
@@ -1129,16 +1102,13 @@ def attention_relbias_bwd(qkv, table, out, dout, lse, dqkv, dtable, delta_ws, b,
     if table.get_device() != device or dtable.get_device() != device:
         _on_device(what, table, qkv)
         _on_device(what, dtable, qkv)
-    grad, last = dtable.data_ptr(), rel.n_buckets - 1
-    if grad < rel.table + 4 * (last * rel.ld + H) and rel.table < grad + 4 * (last * stride[0] + H):
-        raise ValueError(f"{what}: an output shares memory with another operand")
     need = _relbias_workspace_elems(rel.n_buckets, max_distance, rel.bidirectional, b, S, H)
     workspace = _scratch(what, workspace, need, qkv.device)
     n, words = b * S * H, attention_keep_words(b, S, H) if keep_rows is not None else 0
     stream, (dq_, dl_, ws_, q_, o_, do_, l_, n_, kr_, kc_) = _operands(
         what, ("dqkv", "delta_ws", "workspace", "qkv", "out", "dout", "lse", "lengths", "keep_rows", "keep_cols"), _RELBIAS_BWD_TYPES,
-        (dqkv, delta_ws, workspace, qkv, out, dout, lse, lengths, keep_rows, keep_cols), (n * 192, n, need, n * 192, n * 64, n * 64, n, b, words, words), 3, ("lengths",))
-    check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, grad, stride[0], accumulate,
+        (dqkv, delta_ws, workspace, qkv, out, dout, lse, lengths, keep_rows, keep_cols), (n * 192, n, need, n * 192, n * 64, n * 64, n, b, words, words), ("lengths",))
+    check(lib().hapmi_attention_relbias_bwd(q_, ctypes.byref(rel), causal, n_, o_, do_, l_, dq_, dtable.data_ptr(), stride[0], accumulate,
                                             dl_, _kept(ws_, workspace), workspace.numel(), b, S, H, scale, kr_, kc_, p, stream))
 
 
@@ -1535,7 +1505,7 @@ def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, leng
     n, m = B * E, B * S * 2
     stream, (l_, c_, k_, ps_, ws_, p_, i_, s_, n_) = _operands(
         what, ("loss", "counts", "kept", "prob_sum", "workspace", "probs", "index", "slot", "lengths"), _BALANCE_FWD_TYPES,
-        (loss, counts, kept, prob_sum, workspace, probs, r["index"], r["slot"], lengths), (1, n, n, n, need, S * n, m, m, B), 5, _BALANCE_EXACT)
+        (loss, counts, kept, prob_sum, workspace, probs, r["index"], r["slot"], lengths), (1, n, n, n, need, S * n, m, m, B), _BALANCE_EXACT)
     check(lib().hapmi_balance_loss_fwd(p_, i_, s_, n_, l_, c_, k_, ps_, B, S, E, coef, choices, _kept(ws_, workspace),
                                        workspace.numel() if workspace is not None else 0, stream))
 
@@ -1549,7 +1519,7 @@ def balance_loss_bwd(r, counts, dlogits, choices=2, coef=0.01, grad=1.0, dgate=N
     n, m = B * E, B * S * 2
     stream, (d_, p_, i_, s_, g_, c_, n_) = _operands(
         what, ("dlogits", "probs", "index", "slot", "dgate", "counts", "lengths"), _BALANCE_BWD_TYPES,
-        (dlogits, probs, r["index"], r["slot"], dgate, counts, lengths), (S * n, S * n, m, m, m, n, B), 1, _BALANCE_EXACT)
+        (dlogits, probs, r["index"], r["slot"], dgate, counts, lengths), (S * n, S * n, m, m, m, n, B), _BALANCE_EXACT)
     check(lib().hapmi_balance_loss_bwd(p_, i_, s_, g_, c_, n_, d_, B, S, E, coef * grad, choices, stream))
 
 

@@ -37,7 +37,8 @@ enum {
     HAPMI_EALIGN = -2,   /* pointer or stride not aligned   */
     HAPMI_EARCH = -3,    /* device is not gfx950            */
     HAPMI_ELAUNCH = -4,  /* HIP reported a launch error     */
-    HAPMI_ELIMIT = -5    /* size beyond a documented limit  */
+    HAPMI_ELIMIT = -5,   /* size beyond a documented limit  */
+    HAPMI_EALIAS = -6    /* an output shares memory with another operand (checked where an entry point says so) */
 };
 #define HAPMI_MAX_RANKS 64
 

@@ -165,3 +165,68 @@ def test_bias_tables_whose_rows_overlap():
     for odd in (row.expand(8, 4), torch.zeros(8, 3), torch.zeros(8, 8)[:, ::2]):
         with pytest.raises(ValueError, match="dtable must be"):
             ops.attention_relbias_bwd(x, whole, x, x, x, x, odd, x, 1, 2, 4, 0.125, max_distance=8, causal=True)
+
+
+EALIAS = -6
+
+
+@pytest.mark.parametrize("shared", ["out/qkv", "lse/qkv", "lse/out", "out/table", "lse/lengths", "lse/keep", "out/qkv+8000"])
+def test_bias_forward_outputs_apart(shared):
+    """b 2, S 16, H 4: qkv 49152 bytes, out 16384, lse 512; an output that starts inside another operand is refused."""
+    at = dict(qkv=1 << 20, out=2 << 20, lse=3 << 20, table=4 << 20, lengths=5 << 20, keep=6 << 20)
+    name, other = shared.split("/")
+    other, _, off = other.partition("+")
+    at[name] = at[other] + int(off or 0) // 16 * 16
+    r = bias(table=at["table"])
+    rc = _load().hapmi_attention_relbias_fwd(at["qkv"], ctypes.byref(r), 0, at["lengths"], at["out"], at["lse"], 2, 16, 4, 0.125, at["keep"], 0.1, None)
+    refused(rc, EALIAS, "shares memory")
+
+
+@pytest.mark.parametrize("shared", ["dqkv/qkv", "dqkv/dout", "dtable/table", "dtable/dqkv", "delta/lse", "ws/delta", "ws/out", "dtable/ws", "delta/kc", "dqkv/lengths"])
+def test_bias_backward_outputs_apart(shared):
+    names = ("qkv", "out", "dout", "lse", "dqkv", "dtable", "delta", "ws", "table", "lengths", "kr", "kc")
+    at = {n: (i + 1) << 20 for i, n in enumerate(names)}
+    name, other = shared.split("/")
+    at[name] = at[other]
+    r = bias(table=at["table"])
+    rc = _load().hapmi_attention_relbias_bwd(at["qkv"], ctypes.byref(r), 0, at["lengths"], at["out"], at["dout"], at["lse"], at["dqkv"], at["dtable"], 8, 0,
+                                             at["delta"], at["ws"], 1 << 16, 2, 16, 4, 0.125, at["kr"], at["kc"], 0.1, None)
+    refused(rc, EALIAS, "shares memory")
+
+
+@pytest.mark.parametrize("shared", ["out/q", "out/k", "out/angles", "out/positions", "out/qkv+512"])
+def test_norm_forward_outputs_apart(shared):
+    at = {n: (i + 1) << 20 for i, n in enumerate(("qkv", "out", "q", "k", "angles", "positions"))}
+    name, other = shared.split("/")
+    other, _, off = other.partition("+")
+    at[name] = at[other] + int(off or 0)
+    rc = _load().hapmi_qk_norm_rotary_fwd(at["qkv"], at["out"], at["q"], at["k"], at["angles"], 64, 64, 0, at["positions"], 2, 16, 4, 64, 1e-6, BF16, None)
+    refused(rc, EALIAS, "shares memory")
+
+
+@pytest.mark.parametrize("shared", ["dqkv/qkv", "dq/dk", "dq/q", "dk/ws", "ws/dout", "dqkv/ws", "dqkv/dout+1024"])
+def test_norm_backward_outputs_apart(shared):
+    at = {n: (i + 1) << 20 for i, n in enumerate(("dout", "qkv", "dqkv", "q", "k", "dq", "dk", "angles", "positions", "ws"))}
+    name, other = shared.split("/")
+    other, _, off = other.partition("+")
+    at[name] = at[other] + int(off or 0)
+    rc = _load().hapmi_qk_norm_rotary_bwd(at["dout"], at["qkv"], at["dqkv"], at["q"], at["k"], at["dq"], at["dk"], 0, at["angles"], 64, 64, 0, at["positions"],
+                                          2, 16, 4, 64, 1e-6, BF16, at["ws"], 1 << 24, None)
+    refused(rc, EALIAS, "shares memory")
+
+
+@pytest.mark.parametrize("shared", ["loss/counts", "counts/kept", "kept/index", "sums/probs", "loss/lengths", "ws/probs", "ws/slot"])
+def test_balance_outputs_apart(shared):
+    at = {n: (i + 1) << 20 for i, n in enumerate(("probs", "index", "slot", "lengths", "loss", "counts", "kept", "sums", "ws"))}
+    name, other = shared.split("/")
+    at[name] = at[other]
+    rc = _load().hapmi_balance_loss_fwd(at["probs"], at["index"], at["slot"], at["lengths"], at["loss"], at["counts"], at["kept"], at["sums"], 2, 4096, 16, 0.01, 2,
+                                        at["ws"], 1 << 20, None)
+    refused(rc, EALIAS, "shares memory")
+
+
+@pytest.mark.parametrize("other", ["probs", "index", "slot", "dgate", "counts", "lengths"])
+def test_balance_gradient_apart(other):
+    at = {n: (i + 1) << 20 for i, n in enumerate(("probs", "index", "slot", "dgate", "counts", "lengths"))}
+    rc = _load().hapmi_balance_loss_bwd(at["probs"], at["index"], at["slot"], at["dgate"], at["counts"], at["lengths"], at[other], 2, 64, 16, 0.01, 2, None)
+    refused(rc, EALIAS, "shares memory")
