@@ -287,7 +287,8 @@ int hapmi_layernorm_bwd_dropout(const void *dy, const void *y, const float *rstd
  *                   [0, n_pos) gives NaN in the token's queries and keys
  * D at most 256 and a multiple of 8 (bf16) / 4 (float32); rot a multiple of twice that (interleaved: of that).
  * Backward: dqkv (== dout: in place) from dout and forward's input; dq_gain / dk_gain float32[D] or NULL, overwritten or
- * (accumulate) added to; they need float32 workspace of hapmi_qk_norm_rotary_workspace_elems(D).  No atomics. */
+ * (accumulate) added to; they need float32 workspace of hapmi_qk_norm_rotary_workspace_elems(D).  No atomics.
+ * In place means the same pointer; any other overlap of an output is refused (HAPMI_EALIAS). */
 int hapmi_qk_norm_rotary_fwd(const void *qkv, void *out, const float *q_gain, const float *k_gain, const float *angles, int64_t n_pos,
                              int64_t rot, int interleaved, const int32_t *positions, int64_t b, int64_t S, int64_t H, int64_t D,
                              float eps, int dtype, hapmi_stream_t stream);
@@ -371,7 +372,7 @@ typedef struct {
  * Backward takes out and lse as forward left them, writes dqkv completely and dtable[n_buckets][ld_dtable]'s columns
  * 0 .. H - 1 (accumulate != 0: adds to them; b >= 1); delta_ws is float32 scratch of b*H*S elements, workspace float32 scratch
  * of the number of elements that hapmi_attention_relbias_workspace_elems reports.  No atomics between waves: the same call
- * gives the same bits. */
+ * gives the same bits.  Outputs and scratch share no memory with each other or with what is read (HAPMI_EALIAS). */
 int hapmi_attention_relbias_fwd(const void *qkv, const hapmi_relbias *bias_host, int causal, const int32_t *lengths, void *out,
                                 float *lse, int64_t b, int64_t S, int64_t H, float scale, const uint32_t *keep_rows,
                                 float p, hapmi_stream_t stream);
@@ -472,7 +473,8 @@ int hapmi_top2_gate_bwd(const float *probs, const int32_t *index, const int32_t 
  *   loss[0] = coef * E / (rows with tokens) * sum_b sum_e counts[b, e] / (choices * n_b) * prob_sum[b, e] / n_b.
  * Backward: dlogits = softmax backward of coef's loss through prob_sum (counts carry no gradient), 0 for tokens that do not
  * count; with dgate also the result of hapmi_top2_gate_bwd, in the same pass.  coef there = coef of the loss times the
- * gradient that reaches it.  E <= 64.  workspace: hapmi_balance_workspace_elems floats (0: may be NULL). */
+ * gradient that reaches it.  E <= 64.  workspace: hapmi_balance_workspace_elems floats (0: may be NULL).  Outputs and
+ * scratch share no memory with each other or with what is read (HAPMI_EALIAS). */
 int hapmi_balance_workspace_elems(int64_t B, int64_t S, int64_t E, int64_t *elems_host);
 int hapmi_balance_loss_fwd(const float *probs, const int32_t *index, const int32_t *slot, const int32_t *lengths, float *loss,
                            int32_t *counts, int32_t *kept, float *prob_sum, int64_t B, int64_t S, int64_t E, float coef, int choices,
