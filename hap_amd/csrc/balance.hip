@@ -16,6 +16,7 @@ namespace {
 
 constexpr int BAL_THREADS = 256;
 constexpr int BAL_MAX_E = 64;
+constexpr int BAL_SMALL_WAVES = 16;                // waves of the block that does a small call alone
 constexpr int BAL_BLOCKS = 512;                     // a row is cut into slabs until about this many blocks run
 
 __device__ __forceinline__ int bal_length(const int32_t *lengths, int b, int S) {
@@ -149,6 +150,92 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(const int32_t *lengt
     }
 }
 
+// A small call in one launch: a block, whose waves take a row each in turn.  Lanes hold V experts of 64 V / E tokens at a time.
+template <int V>
+__global__ __launch_bounds__(BAL_SMALL_WAVES * 64) void balance_small_kernel(const float *probs, const int32_t *index, const int32_t *slot,
+                                                                          const int32_t *lengths, int32_t *counts, int32_t *kept, float *psum,
+                                                                          float *loss, int B, int S, int E, float coef, int choices) {
+    __shared__ int32_t cnt[BAL_SMALL_WAVES][2][BAL_MAX_E];
+    __shared__ float part[BAL_SMALL_WAVES][64 * V];
+    __shared__ float red[2][BAL_SMALL_WAVES];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int cols = E / V, per = 64 / cols, c = lane % cols, r = lane / cols;
+    float v = 0.f, rows = 0.f;
+    for (int b = wave; b < B; b += BAL_SMALL_WAVES) {
+        const int n = bal_length(lengths, b, S);
+        cnt[wave][0][lane] = 0;                     // (a wave's LDS accesses are carried out in their order)
+        cnt[wave][1][lane] = 0;
+        asm volatile("" ::: "memory");
+        for (int s0 = lane; s0 < n; s0 += 4 * 64) {
+            int e[4][2], sl[4][2];                  // the records of four tokens are on their way at once
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int s = s0 + j * 64;
+                const int64_t rec = ((int64_t)b * S + (s < n ? s : s0)) * 2;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const bool counts_here = s < n && k < choices;
+                    e[j][k] = counts_here ? index[rec + k] : -1;
+                    sl[j][k] = counts_here ? slot[rec + k] : 0;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (e[j][k] >= 0 && e[j][k] < E) {        // whole numbers: the order of these additions does not show
+                        atomicAdd(&cnt[wave][0][e[j][k]], 1);
+                        if (sl[j][k] > 0) atomicAdd(&cnt[wave][1][e[j][k]], 1);
+                    }
+        }
+        float acc[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        if (r < per) {
+            const float *p = probs + (int64_t)b * S * E + c * V;
+#pragma unroll 8
+            for (int s = r; s < n; s += per) {
+                if (V == 4) {
+                    const f32x4 x = *(const f32x4 *)(p + (int64_t)s * E);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] += x[i];
+                } else {
+                    acc[0] += p[(int64_t)s * E];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[wave][lane * V + i] = acc[i];
+        asm volatile("" ::: "memory");
+        if (lane < E) {
+            float sum = 0.f;
+            for (int i = 0; i < per; ++i) sum += part[wave][i * E + lane];
+            const int named = cnt[wave][0][lane];
+            const int64_t at = (int64_t)b * E + lane;
+            counts[at] = named;
+            kept[at] = cnt[wave][1][lane];
+            psum[at] = sum;
+            if (n > 0) v += (float)named / (float)n * (sum / (float)n);
+        }
+        asm volatile("" ::: "memory");
+        rows += n > 0 ? 1.f : 0.f;
+    }
+    v = wave_sum(v);
+    if (lane == 0) {
+        red[0][wave] = v;
+        red[1][wave] = rows;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float t = 0.f, G = 0.f;
+        for (int i = 0; i < BAL_SMALL_WAVES; ++i) {
+            t += red[0][i];
+            G += red[1][i];
+        }
+        loss[0] = G > 0.f ? coef * (float)E / (G * (float)choices) * t : 0.f;
+    }
+}
+
 // a group of lanes per token, V experts a lane; BAL_TURNS tokens of a lane are loaded before the first one is worked on
 constexpr int BAL_TURNS = 4;
 template <int V>
@@ -227,6 +314,16 @@ int bal_check(const char *name, int64_t B, int64_t S, int64_t E, int choices) {
     return HAPMI_OK;
 }
 
+// Whether one block does it all: up to 256 KiB of probabilities (a compute unit reads about 100 GB/s), and few steps for a wave (a
+// load of 64 V / E tokens; 64 tokens' records and their LDS additions count 16).  One launch against two, in a graph / called from the
+// host: 4 rows of 64 tokens, 16 experts 3.9 against 5.8 / 8.0 against 10.9 us; 11 of 90, 33 experts 6.6 against 5.9 / 7.8 against
+// 10.5; beyond the limits 16 of 128, 64 experts 7.9 against 6.2 / 8.0 against 11.4; 2 of 1024, 8 experts 10.8 against 7.3 / 10.8
+// against 11.8; 16 of 512, 16 experts 13.1 against 6.3 / 13.1 against 11.5.
+bool bal_small(int64_t B, int64_t S, int64_t E) {
+    const int64_t per = 64 / (E % 4 == 0 ? E / 4 : E), loads = hapmi_cdiv(S, per), records = 16 * hapmi_cdiv(S, 64);
+    return B * S * E <= 65536 && hapmi_cdiv(B, BAL_SMALL_WAVES) * (loads > records ? loads : records) <= 96;
+}
+
 // tokens a block takes: about 16 KiB of probabilities at least, whole rows once there are BAL_BLOCKS of them
 int64_t bal_slab(int64_t B, int64_t S, int64_t E) {
     const int64_t least = hapmi_cdiv(4096, E);
@@ -241,7 +338,7 @@ extern "C" int hapmi_balance_workspace_elems(int64_t B, int64_t S, int64_t E, in
     const int rc = bal_check("balance_workspace_elems", B, S, E, 1);
     if (rc) return rc;
     HAPMI_REQUIRE(elems_host, HAPMI_EINVAL, "balance_workspace_elems: null pointer");
-    const int64_t slabs = B ? hapmi_cdiv(S, bal_slab(B, S, E)) : 1;
+    const int64_t slabs = B && !bal_small(B, S, E) ? hapmi_cdiv(S, bal_slab(B, S, E)) : 1;
     *elems_host = slabs > 1 ? 3 * B * slabs * E : 0;
     return HAPMI_OK;
 }
@@ -255,13 +352,24 @@ extern "C" int hapmi_balance_loss_fwd(const float *probs, const int32_t *index, 
     HAPMI_REQUIRE(B >= 1, HAPMI_EINVAL, "%s: empty batch (the loss would stay unwritten)", name);
     HAPMI_REQUIRE(probs && index && slot && loss && counts && kept && prob_sum, HAPMI_EINVAL, "%s: null pointer", name);
     HAPMI_REQUIRE((uintptr_t)probs % 16 == 0, HAPMI_EALIGN, "%s: probs must be 16-byte aligned", name);
-    const int64_t slab = bal_slab(B, S, E), slabs = hapmi_cdiv(S, slab), n = B * slabs * E;
+    const bool small = bal_small(B, S, E);
+    const int64_t slab = small ? S : bal_slab(B, S, E), slabs = hapmi_cdiv(S, slab), n = B * slabs * E;
     HAPMI_REQUIRE(slabs == 1 || (workspace && workspace_elems >= 3 * n), HAPMI_ELIMIT, "%s: workspace of %lld floats, %lld needed", name,
                   (long long)(workspace ? workspace_elems : 0), (long long)(3 * n));
     const int64_t records = B * S * 2 * 4, sums = B * E * 4;
     const int rc2 = hapmi_apart(name, {{loss, 4}, {counts, sums}, {kept, sums}, {prob_sum, sums}, {slabs > 1 ? workspace : nullptr, 3 * n * 4}},
                                 {{probs, B * S * E * 4}, {index, records}, {slot, records}, {lengths, B * 4}});
     if (rc2) return rc2;
+    if (small) {
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(1), dim3(BAL_SMALL_WAVES * 64), 0, (hipStream_t)stream, probs, index, slot, lengths, counts, kept, prob_sum, loss,
+                               (int)B, (int)S, (int)E, coef, choices);
+        };
+        if (E % 4 == 0) go(balance_small_kernel<4>);
+        else go(balance_small_kernel<1>);
+        HAPMI_CHECK_LAUNCH(name);
+        return HAPMI_OK;
+    }
     int32_t *pc = slabs > 1 ? (int32_t *)workspace : counts, *pk = slabs > 1 ? (int32_t *)workspace + n : kept;
     float *pp = slabs > 1 ? workspace + 2 * n : prob_sum;
     const dim3 grid((unsigned)slabs, (unsigned)B), block(BAL_THREADS);

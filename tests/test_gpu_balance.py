@@ -29,7 +29,10 @@ def outputs(cuda, B, S, E):
 
 CASES = [(1, 1, 2, 1, None, False), (2, 7, 4, 2, None, False), (3, 64, 5, 1, None, True), (4, 33, 16, 2, [33, 0, 1, 20], False), (2, 512, 64, 2, None, False),
          (1, 3000, 63, 2, [2999], False), (16, 512, 16, 1, None, False), (600, 5, 8, 2, None, False), (3, 900, 24, 1, [0, 0, 0], True), (1, 4097, 3, 2, None, False),
-         (5, 300, 61, 2, [300, 299, -4, 1000, 1], False)]
+         (5, 300, 61, 2, [300, 299, -4, 1000, 1], False),
+         # one block's work: several rows a wave, one token or few a load, tokens that do not fill a wave, empty rows
+         (40, 6, 5, 2, [i % 7 for i in range(40)], False), (17, 64, 33, 2, None, False), (16, 63, 64, 1, None, True), (3, 300, 8, 2, [300, 257, 0], False),
+         (1, 96, 63, 2, None, False), (7, 257, 2, 2, None, False), (48, 96, 4, 1, None, True), (2, 65, 3, 2, [65, 64], False)]
 
 
 @pytest.mark.parametrize("B,S,E,choices,lengths,switch", CASES)
