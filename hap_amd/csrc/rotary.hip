@@ -10,13 +10,16 @@
 // holds one head of a token, every lane two 16-byte vectors chosen so that both halves of every rotated pair are its
 // own: the rotation needs no exchange, the mean one butterfly over the group.  The lane takes the query and the key of
 // its (token, head) together and reads the angles once for both.  bf16, 16 heads of 64: forward of [12, 512] 16.4 us, 75 MB at
-// 4.6 TB/s; backward of [4, 8192] with both gains 117 us, 547 MB at 4.7 TB/s (a large copy: 5.2 TB/s).
+// 4.6 TB/s; backward of [4, 8192] with both gains 113 us, 547 MB at 4.8 TB/s (a large copy: 5.2 TB/s).
 #include "common.h"
 
 namespace {
 
 constexpr int QN_THREADS = 256;
 constexpr int QN_MAX_DIM = 256;
+// backward with gains: rows of up to this many blocks are one block's, which needs no second launch.  Two, 8 tokens of 16 heads of 64:
+// 11.6 for 14.4 us from the host, 9.5 for 8.6 in a graph; four: 17.9 for 14.4 and 17.8 for 8.6
+constexpr int QN_TURNS = 2;
 constexpr int QN_MAX_BLOCKS = 768;                  // backward: blocks whose gain sums a second kernel adds; 3 a CU are resident
 
 struct QnArgs {
@@ -139,8 +142,8 @@ template <int V> __device__ __forceinline__ void qn_gain(const float *g, const Q
 
 // A position outside the table poisons the token's rotated heads instead of reading beyond it (as an id outside an
 // embedding table does).
-__device__ __forceinline__ int64_t qn_position(const QnArgs &p, int64_t token, bool &bad) {
-    const int64_t pos = p.positions ? p.positions[token] : token % p.S;
+__device__ __forceinline__ int64_t qn_position(const QnArgs &p, int64_t token, int S, bool &bad) {
+    const int64_t pos = p.positions ? p.positions[token] : token % S;
     bad = pos < 0 || pos >= p.n_pos;
     return bad ? 0 : pos;
 }
@@ -169,7 +172,7 @@ __global__ __launch_bounds__(QN_THREADS) void qk_norm_rotary_fwd_kernel(const Qn
         bool bad = false;
         QnAngles<V> w;
         if (p.rot) {
-            const int64_t pos = qn_position(p, token, bad);
+            const int64_t pos = qn_position(p, token, p.S, bad);
             if (l.turn_a || l.turn_b) w = qn_angles<V>(p, l, p.angles + pos * p.rot);
         }
 #pragma unroll
@@ -200,19 +203,18 @@ __global__ __launch_bounds__(QN_THREADS) void qk_norm_rotary_fwd_kernel(const Qn
 }
 
 template <typename T, bool GAINS>
-__global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const QnArgs p, const T *dout, const T *qkv, T *dqkv, float *part) {
+__global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const QnArgs p, const T *dout, const T *qkv, T *dqkv, float *part,
+                                                                          float *dq_gain, float *dk_gain, int accumulate) {
     constexpr int V = Vec16<T>::N;
-    __shared__ float red[GAINS ? 4 * 2 * QN_MAX_DIM : 1];
+    __shared__ __attribute__((aligned(16))) float red[GAINS ? QN_THREADS * 4 * V : 1];      // 2 D sums a group, and D <= 2 V a lane
     __shared__ __attribute__((aligned(16))) float gains[2][QN_MAX_DIM];     // read again for every row: 32 registers less a lane
     for (int i = threadIdx.x; i < p.D; i += QN_THREADS) {
         gains[0][i] = p.q_gain ? p.q_gain[i] : 1.f;
         gains[1][i] = p.k_gain ? p.k_gain[i] : 1.f;
     }
     __syncthreads();
-    const int group = 1 << p.group_log2, j = threadIdx.x & (group - 1);
-    const QnLane l = qn_lane<T>(p, j);
+    const int group = 1 << p.group_log2;
     const int E = p.H * p.D;
-    const int ga = (l.a < 0 ? 0 : l.a) * V, gb = (l.b < 0 ? 0 : l.b) * V;
     float acc[2][2][V];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -220,23 +222,26 @@ __global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const
         for (int e = 0; e < V; ++e) acc[t][0][e] = acc[t][1][e] = 0.f;
     const int64_t step = (int64_t)gridDim.x * (QN_THREADS >> p.group_log2);
     for (int64_t row = (int64_t)blockIdx.x * (QN_THREADS >> p.group_log2) + (threadIdx.x >> p.group_log2); row < p.rows; row += step) {
-        const int64_t token = row / p.H, at = token * 3 * E + (row - token * p.H) * p.D;
+        int heads = p.H, S = p.S, tid = threadIdx.x;          // (reciprocals, the lane's part and its addresses are made for every
+        asm volatile("" : "+s"(heads), "+s"(S), "+v"(tid));   // row: kept over the loop they cost spills)
+        const QnLane m = qn_lane<T>(p, tid & (group - 1));
+        const int64_t token = row / heads, at = token * 3 * E + (row - token * heads) * p.D;
         QnPair<T> x[2], d[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            x[t].load(qkv + at + t * E, l);
-            d[t].load(dout + at + t * E, l);
+            x[t].load(qkv + at + t * E, m);
+            d[t].load(dout + at + t * E, m);
         }
         if (dqkv != dout) {
             QnPair<T> v;
-            v.load(dout + at + 2 * E, l);
-            v.store(dqkv + at + 2 * E, l);
+            v.load(dout + at + 2 * E, m);
+            v.store(dqkv + at + 2 * E, m);
         }
         bool bad = false;
         QnAngles<V> w;
         if (p.rot) {
-            const int64_t pos = qn_position(p, token, bad);
-            if (l.turn_a || l.turn_b) w = qn_angles<V>(p, l, p.angles + pos * p.rot);
+            const int64_t pos = qn_position(p, token, S, bad);
+            if (m.turn_a || m.turn_b) w = qn_angles<V>(p, m, p.angles + pos * p.rot);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -251,8 +256,9 @@ __global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const
             }
             sq = group_sum(sq, p.group_log2);
             const float r = bad ? NAN : 1.0f / sqrtf(sq / p.D + p.eps);
-            if (l.turn_a || l.turn_b) qn_turn<V>(p, l, w, -1.f, da, db);
+            if (m.turn_a || m.turn_b) qn_turn<V>(p, m, w, -1.f, da, db);
             asm volatile("" ::: "memory");                    // (the gains are not to be hoisted into registers)
+            const int ga = (m.a < 0 ? 0 : m.a) * V, gb = (m.b < 0 ? 0 : m.b) * V;
             float dot = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -272,30 +278,36 @@ __global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const
                 x[t].a.set(e, r * (da[e] - a[e] * dot));
                 x[t].b.set(e, r * (db[e] - b[e] * dot));
             }
-            x[t].store(dqkv + at + t * E, l);
+            x[t].store(dqkv + at + t * E, m);
         }
     }
     if (!GAINS) return;
-    // gain sums: over the wave's groups by a butterfly, over the four waves through LDS, both in a fixed order
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // gain sums over the block's groups, in their order: a row of 2 D sums for each of them (exchanges between lanes, 1 .. 6 for each of
+    // the lane's 32 values, took 6 us of a block's time: 14.9 us for 8.6 at 32 tokens of 16 heads of 64, 117 for 113 at [4, 8192])
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const QnLane l = qn_lane<T>(p, tid & (group - 1));
+    float *own = red + (tid >> p.group_log2) * 2 * p.D;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+            const int vec = k ? l.b : l.a;
+            if (vec < 0) continue;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float v = acc[t][k][e];
-                for (int o = group; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-                const int vec = k ? l.b : l.a;
-                if (lane < group && vec >= 0) red[(wave * 2 + t) * QN_MAX_DIM + vec * V + e] = v;
-            }
+            for (int e = 0; e < V; ++e) own[t * p.D + vec * V + e] = acc[t][k][e];
+        }
     __syncthreads();
+    const int groups = QN_THREADS >> p.group_log2;
     for (int i = threadIdx.x; i < 2 * p.D; i += QN_THREADS) {
-        const int t = i / p.D, d = i - t * p.D;
         float v = 0.f;
-#pragma unroll
-        for (int wv = 0; wv < 4; ++wv) v += red[(wv * 2 + t) * QN_MAX_DIM + d];
-        part[(int64_t)blockIdx.x * 2 * p.D + i] = v;
+#pragma unroll 8
+        for (int r = 0; r < groups; ++r) v += red[r * 2 * p.D + i];
+        if (gridDim.x > 1) part[(int64_t)blockIdx.x * 2 * p.D + i] = v;
+        else if (float *g = i < p.D ? dq_gain : dk_gain) {              // nothing to join
+            g += i < p.D ? i : i - p.D;
+            *g = accumulate ? *g + v : v;
+        }
     }
 }
 
@@ -402,17 +414,17 @@ extern "C" int hapmi_qk_norm_rotary_bwd(const void *dout, const void *qkv, void 
     int rc2 = hapmi_apart(name, {{dqkv, n}, {dq_gain, D * 4}, {dk_gain, D * 4}, {gains ? workspace : nullptr, 2 * D * QN_MAX_BLOCKS * 4}},
                           {{dout == dqkv ? nullptr : dout, n}, {qkv, n}, {q_gain, D * 4}, {k_gain, D * 4}, {angles, n_pos * rot * 4}, {positions, b * S * 4}});
     if (rc2) return rc2;
-    const int64_t blocks = qn_blocks(a, gains ? QN_MAX_BLOCKS : 1 << 20);
+    const int64_t blocks = gains && qn_blocks(a, 1 << 20) <= QN_TURNS ? 1 : qn_blocks(a, gains ? QN_MAX_BLOCKS : 1 << 20);
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto kernel, auto zero) -> int {
         typedef decltype(zero) T;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(QN_THREADS), 0, st, a, (const T *)dout, (const T *)qkv, (T *)dqkv, workspace);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(QN_THREADS), 0, st, a, (const T *)dout, (const T *)qkv, (T *)dqkv, workspace, dq_gain, dk_gain, accumulate);
         HAPMI_CHECK_LAUNCH(name);
         return HAPMI_OK;
     };
     if (dtype == HAPMI_F32) rc2 = gains ? go(qk_norm_rotary_bwd_kernel<float, true>, 0.f) : go(qk_norm_rotary_bwd_kernel<float, false>, 0.f);
     else rc2 = gains ? go(qk_norm_rotary_bwd_kernel<bf16_t, true>, (bf16_t)0.f) : go(qk_norm_rotary_bwd_kernel<bf16_t, false>, (bf16_t)0.f);
-    if (rc2 || !gains) return rc2;
+    if (rc2 || !gains || blocks == 1) return rc2;
     hipLaunchKernelGGL(qk_gain_sum_kernel, dim3((unsigned)hapmi_cdiv(2 * D, 32)), dim3(1024), 0, st, (const float *)workspace, (int)blocks, (int)D, dq_gain,
                        dk_gain, accumulate);
     HAPMI_CHECK_LAUNCH(name);
