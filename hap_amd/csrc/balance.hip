@@ -8,7 +8,7 @@
 // The gate's own gradient (softmax backward of the kept choices' gate gradients) has the same form, so one pass over the
 // probabilities serves both.  Memory bound at large sizes and launch bound at small ones: forward is one pass and one
 // small joining launch, backward one launch.  64 padded rows of 2048 tokens, 64 experts: counts 8 us, joining 5 us, backward
-// 15 us (37 MB of real tokens read, 34 MB written: 4.7 TB/s); 16 rows of 512 tokens, 16 experts: 4, 2.6 and 4.2 us, most of
+// 15 us (with the gate's gradient: the probabilities and records of all tokens, 37 MB, read and 34 MB written: 4.7 TB/s); 16 rows of 512 tokens, 16 experts: 4, 2.6 and 4.2 us, most of
 // which a launch takes that does nothing.
 #include "common.h"
 
@@ -236,7 +236,9 @@ __global__ __launch_bounds__(BAL_SMALL_WAVES * 64) void balance_small_kernel(con
     }
 }
 
-// a group of lanes per token, V experts a lane; BAL_TURNS tokens of a lane are loaded before the first one is worked on
+// a group of lanes per token, V experts a lane; BAL_TURNS tokens of a lane are loaded before the first one is worked on.  A token
+// that does not count and that no gate gradient reaches gets zeros whatever its probabilities hold (0 * NaN would pass its padding
+// on to the router's weights); without the gate's gradient they are not read.
 constexpr int BAL_TURNS = 4;
 template <int V>
 __global__ __launch_bounds__(BAL_THREADS) void balance_bwd_kernel(const float *probs, const int32_t *index, const int32_t *slot,
@@ -258,7 +260,7 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_bwd_kernel(const float *p
         for (int i = 0; i < V; ++i) p[t][i] = 0.f;
         at[t][0] = at[t][1] = -1;
         dg[t][0] = dg[t][1] = 0.f;
-        if (s >= S) continue;
+        if (s >= (dgate ? S : n)) continue;
         if (V == 4) {
             if (e0 < E) {
                 const f32x4 x = *(const f32x4 *)(probs + tok * E + e0);
@@ -297,13 +299,14 @@ __global__ __launch_bounds__(BAL_THREADS) void balance_bwd_kernel(const float *p
         }
         dot = group_sum(dot, group_log2);
         if (s >= S || e0 >= E) continue;
+        const bool none = s >= n && dg[t][0] == 0.f && dg[t][1] == 0.f;
         if (V == 4) {
             f32x4 x;
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = p[t][i] * (g[i] - dot);
+            for (int i = 0; i < V; ++i) x[i] = none ? 0.f : p[t][i] * (g[i] - dot);
             *(f32x4 *)(dlogits + tok * E + e0) = x;
         } else {
-            dlogits[tok * E + e0] = p[t][0] * (g[0] - dot);
+            dlogits[tok * E + e0] = none ? 0.f : p[t][0] * (g[0] - dot);
         }
     }
 }

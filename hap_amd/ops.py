@@ -1512,7 +1512,8 @@ def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, leng
 
 def balance_loss_bwd(r, counts, dlogits, choices=2, coef=0.01, grad=1.0, dgate=None, lengths=None):
     """Gradient of ``grad`` times the balance loss with respect to the router's logits, from forward's ``counts``; with
-    ``dgate`` (float32 [B, S, 2]) ``dlogits`` also holds what ``top2_gate_bwd`` gives for it, in the same pass."""
+    ``dgate`` (float32 [B, S, 2]) ``dlogits`` also holds what ``top2_gate_bwd`` gives for it, in the same pass.  Tokens behind
+    ``lengths`` that no gate gradient reaches get zeros, whatever their probabilities hold."""
     what = "balance_loss_bwd"
     probs = r["probs"]
     B, S, E = probs.shape

@@ -472,7 +472,8 @@ int hapmi_top2_gate_bwd(const float *probs, const int32_t *index, const int32_t 
  *   prob_sum[b, e] = sum of the probabilities,
  *   loss[0] = coef * E / (rows with tokens) * sum_b sum_e counts[b, e] / (choices * n_b) * prob_sum[b, e] / n_b.
  * Backward: dlogits = softmax backward of coef's loss through prob_sum (counts carry no gradient), 0 for tokens that do not
- * count; with dgate also the result of hapmi_top2_gate_bwd, in the same pass.  coef there = coef of the loss times the
+ * count; with dgate also the result of hapmi_top2_gate_bwd, in the same pass.  A token that does not count may hold anything in
+ * probs (no dgate, or its dgate is zero or of choices without a slot: it gets 0); one that a gate gradient reaches must be finite.  coef there = coef of the loss times the
  * gradient that reaches it.  E <= 64.  workspace: hapmi_balance_workspace_elems floats (0: may be NULL).  Outputs and
  * scratch share no memory with each other or with what is read (HAPMI_EALIAS). */
 int hapmi_balance_workspace_elems(int64_t B, int64_t S, int64_t E, int64_t *elems_host);

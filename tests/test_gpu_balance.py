@@ -146,3 +146,33 @@ def test_refused_calls(cuda):
         ops.balance_loss_bwd(r, counts, r["probs"])
     with pytest.raises(ops._lib.HapmiError):
         ops.balance_loss_bwd(r, counts, d, dgate=dgate[:, :4].to(cuda).contiguous())
+
+
+@pytest.mark.parametrize("B,S,E,lengths", [(3, 100, 16, [60, 0, 100]), (2, 50, 5, [49, 1]), (4, 300, 64, [299, 7, 150, 300]), (5, 9, 33, [-3, 40, 8, 0, 9])])
+@pytest.mark.parametrize("filler", [float("nan"), float("inf")])
+def test_padding_may_hold_anything(cuda, B, S, E, lengths, filler):
+    """Tokens that do not count: their probabilities are not finite, and no gate gradient reaches them (zero, or of a choice
+    without a slot).  They get zeros, the others the bits that a clean padding gives."""
+    r, dgate = routing(cuda, S, B, S, E)
+    loss, counts, kept, sums, d = outputs(cuda, B, S, E)
+    ln = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    pad = torch.arange(S, device=cuda)[None] >= ln[:, None]
+    dirty = {k: v.clone() for k, v in r.items()}
+    dirty["probs"][pad] = filler
+    dirty["index"][pad] = -7
+    dg = dgate.to(cuda)
+    dg[pad] = 0.0
+    dropped = dg.clone()
+    dropped[pad] = filler
+    dirty["slot"][pad] = 0
+    clean = outputs(cuda, B, S, E)
+    ops.balance_loss_fwd(r, *clean[:4], lengths=ln)
+    ops.balance_loss_fwd(dirty, loss, counts, kept, sums, lengths=ln)
+    assert torch.equal(loss, clean[0]) and torch.equal(counts, clean[1]) and torch.equal(kept, clean[2]) and torch.equal(sums, clean[3])
+    for clean_gate, dirty_gate in ((None, None), (dg, dg), (dg, dropped)):
+        want = clean[4]
+        ops.balance_loss_bwd(r, counts, want, dgate=clean_gate, lengths=ln)
+        d.fill_(float("nan"))
+        ops.balance_loss_bwd(dirty, counts, d, dgate=dirty_gate, lengths=ln)
+        assert (d[pad] == 0).all()
+        assert torch.equal(d[~pad], want[~pad])
