@@ -126,6 +126,13 @@ template <typename T> struct QnPair {
             for (int e = 0; e < V; ++e) b.set(e, 0.f);
         }
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            a.set(e, 0.f);
+            b.set(e, 0.f);
+        }
+    }
     __device__ __forceinline__ void store(T *row, const QnLane &l) const {
         if (l.a >= 0) *(Vec16<T> *)(row + l.a * V) = a;
         if (l.b >= 0) *(Vec16<T> *)(row + l.b * V) = b;
@@ -140,8 +147,8 @@ template <int V> __device__ __forceinline__ void qn_gain(const float *g, const Q
     }
 }
 
-// A position outside the table poisons the token's rotated heads instead of reading beyond it (as an id outside an
-// embedding table does).
+// A position outside the table poisons the token's queries and keys in forward instead of reading beyond it, and leaves the
+// token out of backward: no gradient for its queries and keys, nothing in the gains' (as an id outside an embedding table does).
 __device__ __forceinline__ int64_t qn_position(const QnArgs &p, int64_t token, int S, bool &bad) {
     const int64_t pos = p.positions ? p.positions[token] : token % S;
     bad = pos < 0 || pos >= p.n_pos;
@@ -243,6 +250,13 @@ __global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const
             const int64_t pos = qn_position(p, token, S, bad);
             if (m.turn_a || m.turn_b) w = qn_angles<V>(p, m, p.angles + pos * p.rot);
         }
+        if (__builtin_expect(bad, 0)) {                       // (its rows may hold anything: zeros in their place, and r = 0 below)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                x[t].clear();
+                d[t].clear();
+            }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             float a[V], b[V], da[V], db[V], sq = 0.f;
@@ -255,7 +269,7 @@ __global__ __launch_bounds__(QN_THREADS, 3) void qk_norm_rotary_bwd_kernel(const
                 sq += a[e] * a[e] + b[e] * b[e];
             }
             sq = group_sum(sq, p.group_log2);
-            const float r = bad ? NAN : 1.0f / sqrtf(sq / p.D + p.eps);
+            const float r = bad ? 0.f : 1.0f / sqrtf(sq / p.D + p.eps);
             if (m.turn_a || m.turn_b) qn_turn<V>(p, m, w, -1.f, da, db);
             asm volatile("" ::: "memory");                    // (the gains are not to be hoisted into registers)
             const int ga = (m.a < 0 ? 0 : m.a) * V, gb = (m.b < 0 ? 0 : m.b) * V;

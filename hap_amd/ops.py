@@ -859,7 +859,7 @@ def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None,
     """Queries and keys of the packed projection ``qkv`` [b, S, 3 * H * head_dim] normalised per head (root mean square,
     float32 gains [head_dim]) and rotated by position (``rotary`` from ``rotary_table``; its first 2 * shape[1] dimensions;
     None: norm only), values copied; ``out`` may be ``qkv`` itself (in place).  ``positions``: int32 [b, S] (None: the index
-    inside the sequence); one outside the table gives NaN.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
+    inside the sequence); one outside the table gives NaN in the token's queries and keys.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
     what = "qk_norm_rotary_fwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
     code, n = dtype_code(qkv), b * S * 3 * H * D
@@ -881,7 +881,8 @@ def qk_norm_rotary_workspace_elems(D: int) -> int:
 def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_gain=None, dk_gain=None, rotary=None,
                        positions=None, interleaved=False, eps=1e-6, accumulate=False, workspace=None):
     """Backward of ``qk_norm_rotary_fwd``: ``dqkv`` from ``dout`` (``dqkv`` may be ``dout``: in place) and forward's input
-    ``qkv``; ``dq_gain`` / ``dk_gain`` float32 [head_dim] (None: not wanted; ``accumulate``: added to)."""
+    ``qkv``; ``dq_gain`` / ``dk_gain`` float32 [head_dim] (None: not wanted; ``accumulate``: added to).  A token whose position
+    lies outside the table is left out: zeros for its queries and keys, nothing in the gains' gradients."""
     what = "qk_norm_rotary_bwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
     code, n, ws_elems = dtype_code(qkv), b * S * 3 * H * D, 0

@@ -205,3 +205,32 @@ def test_refused_calls(cuda):
     g = torch.empty(64, device=cuda)
     with pytest.raises(ValueError):
         ops.qk_norm_rotary_bwd(out, x, torch.empty_like(x), 1, 4, 1, dq_gain=g, dk_gain=g)
+
+
+@pytest.mark.parametrize("dtype,inter,H,D", [(torch.bfloat16, False, 2, 64), (torch.float32, True, 3, 32), (torch.bfloat16, True, 1, 24)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_backward_leaves_out_tokens_without_a_position(cuda, dtype, inter, H, D, accumulate):
+    """A token whose position lies outside the table (padding marked with -1) has no gradient: zeros for its queries and keys,
+    nothing in the gains' gradients, whatever its rows hold; its value rows are copied.  The others are the bits of the same
+    call with that token's rows zero and its position valid (zero rows add nothing to the gains)."""
+    b, S = 2, 37
+    qkv, dout, qg, kg, table, _ = make(7, b, S, H, D, dtype, 16, 0)
+    pos = torch.arange(S).repeat(b, 1).int()
+    bad = torch.zeros(b, S, dtype=torch.bool)
+    bad[0, 5] = bad[1, 30:] = True
+    dirty, ddirty, gone = qkv.clone(), dout.clone(), pos.clone()
+    dirty[bad], gone[bad] = float("nan"), -1
+    gone[0, 5] = S
+    ddirty.view(b, S, 3, H * D)[:, :, :2][bad] = float("inf")
+    qkv[bad] = 0
+    dout.view(b, S, 3, H * D)[:, :, :2][bad] = 0
+    res = []
+    for x, d, at in ((qkv, dout, pos), (dirty, ddirty, gone)):
+        dx = torch.full_like(x, float("nan"), device=cuda)
+        dq, dk = torch.full((D,), 2.0, device=cuda), torch.full((D,), -1.0, device=cuda)
+        ops.qk_norm_rotary_bwd(d.to(cuda), x.to(cuda), dx, b, S, H, q_gain=qg.to(cuda), k_gain=kg.to(cuda), dq_gain=dq, dk_gain=dk, rotary=table.to(cuda),
+                               positions=at.to(cuda), interleaved=inter, accumulate=accumulate)
+        res.append((dx, dq, dk))
+    (want, wq, wk), (got, dq, dk) = res
+    assert torch.equal(got, want) and torch.equal(dq, wq) and torch.equal(dk, wk)
+    assert (got.cpu().view(b, S, 3, H * D)[:, :, :2][bad] == 0).all()
