@@ -153,6 +153,11 @@ __device__ __forceinline__ void own_frags(const char *lds, int c, int h, int row
     }
 }
 
+// A wave adds to its window of ds sums by load, add and store, and a word that one lane adds to belongs to another lane in the next
+// addition: the order of the accesses counts although no thread meets its own word again.  The wave's LDS accesses are carried out
+// in their order; this keeps the compiler from moving a load above the store before it.
+__device__ __forceinline__ void window_order() { asm volatile("" ::: "memory"); }
+
 // the same in all lanes, in a scalar register
 __device__ __forceinline__ float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 
@@ -577,7 +582,10 @@ __global__ __launch_bounds__(AT_THREADS, AHEAD ? 2 : 3) void relbias_bwd_dq_kern
                     for (int r = 0; r < 16; ++r) sum += dp[r];
                     far_sum[far_hi ? 1 : 0] += sum;
                 } else {
-                    own[rel.at<32>(D, 0, 0) + 31 - lane] += diagonal_sums(dp);
+                    const float sums_of_lane = diagonal_sums(dp);
+                    window_order();
+                    own[rel.at<32>(D, 0, 0) + 31 - lane] += sums_of_lane;
+                    window_order();
                 }
             };
             sc0 = bias_tile(win + rel.at<32>(-qw, c, h));
@@ -690,7 +698,10 @@ __global__ __launch_bounds__(AT_THREADS, AHEAD ? 2 : 3) void relbias_bwd_dq_kern
                         db[1] = acc_to_b(dp, 1);
                         asm volatile("" : "+v"(db[0].v), "+v"(db[1].v));      // rounded here: the sums below then need no copies of dp
                         // lane l of the sums: diagonal (last row) - l; `at` is row 0's word of column c
-                        own[at - 4 * h + c + 31 - lane] += diagonal_sums(dp);
+                        const float sums_of_lane = diagonal_sums(dp);
+                        window_order();
+                        own[at - 4 * h + c + 31 - lane] += sums_of_lane;
+                        window_order();
                     }
 #pragma unroll
                     for (int sp = 0; sp < 2; ++sp) {
@@ -701,6 +712,7 @@ __global__ __launch_bounds__(AT_THREADS, AHEAD ? 2 : 3) void relbias_bwd_dq_kern
             }
         }
         const float lo = group_sum(far_sum[0], 6), hi = group_sum(far_sum[1], 6);
+        window_order();
         if (lane == 0) {
             own[0] += lo;
             own[W - 1] += hi;

@@ -297,3 +297,14 @@ def test_refused_calls(cuda):
                     (dict(delta_ws=lse), ValueError), (dict(keep_rows=torch.zeros(64, dtype=torch.int32, device=cuda)), ValueError)):
         with pytest.raises(err):
             g(**kw)
+
+
+@pytest.mark.parametrize("b,S,H,causal", [(1, 640, 1, False), (1, 640, 1, True), (33, 257, 9, False), (33, 257, 9, True)])
+def test_table_gradient_where_every_block_meets_its_neighbours_words(cuda, b, S, H, causal):
+    """A window that reaches over (nearly) the whole sequence: every 32 x 32 block's diagonals go into it, each word is added to by
+    one lane in one block and by another in the next one.  Few blocks and a launch that fills the card: both forms of dQ."""
+    qkv, table, dout = make(S + b, b, S, H, 128 if not causal else 64)
+    kw = dict(max_distance=1000, bidirectional=not causal, causal=causal)
+    res = run(cuda, qkv, table, dout, H, **kw)
+    want = L.relbias_backward(qkv, table, res[0].cpu(), dout, res[1].cpu(), H, SCALE, 1000, not causal, causal)["dtable"]
+    within(res[3], want[0], F * want[2], "dtable")
