@@ -1071,7 +1071,10 @@ bool fits_two_a_cu(int64_t blocks, bool padded) { return (padded ? blocks * 2 / 
 bool aligned(const void *p, uintptr_t n) { return (uintptr_t)p % n == 0; }
 
 // a strided float32 [n][ld] matrix of H columns; a row stride beyond any memory counts as 2^40
-HapmiSpan rows_span(const float *p, int64_t n, int64_t ld, int64_t H) { return {p, ((n - 1) * (ld < (1ll << 40) ? ld : 1ll << 40) + H) * 4}; }
+HapmiSpan rows_span(const float *p, int64_t n, int64_t ld, int64_t H) {
+    if (ld > 1ll << 40) ld = 1ll << 40;
+    return {p, ((n - 1) * ld + H) * 4, H * 4, ld > H ? ld * 4 : 0};
+}
 int64_t keep_bytes(int64_t b, int64_t S, int64_t H) { return b * H * S * 2 * hapmi_cdiv(S, TILE) * 4; }
 
 // More than 64 KiB of LDS a block has to be asked for, once per kernel and device (`asked`: a bit for every device); each time would

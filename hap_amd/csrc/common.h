@@ -30,16 +30,27 @@ int hapmi_sumsq_static_setup();   // elementwise.hip: per-device set-up that hap
 // Refuses outputs that share memory with each other or with an operand that is read (operands that are only read may share).
 struct HapmiSpan {
     const void *at;                 // NULL: no such operand
-    int64_t bytes;
+    int64_t bytes;                  // from the first byte to behind the last one
+    int64_t row = 0, pitch = 0;     // a strided matrix: bytes of a row, from row to row (0: the whole span is used)
 };
+// Whether two spans share a byte.  A matrix leaves the gaps between its rows to others: columns beside it in the same buffer
+// (equal pitch), or something that fits into one gap.  Matrices of different pitches whose ranges meet count as sharing.
+inline bool hapmi_meet(const HapmiSpan &a, const HapmiSpan &b) {
+    const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+    if (!x || !y || a.bytes <= 0 || b.bytes <= 0) return false;
+    if (x <= y ? y - x >= (uintptr_t)a.bytes : x - y >= (uintptr_t)b.bytes) return false;
+    if (a.pitch != b.pitch && a.pitch && b.pitch) return true;
+    const uintptr_t pitch = (uintptr_t)(a.pitch ? a.pitch : b.pitch);
+    if (!pitch) return true;
+    const uintptr_t ra = a.pitch ? (uintptr_t)a.row : (uintptr_t)a.bytes, rb = b.pitch ? (uintptr_t)b.row : (uintptr_t)b.bytes;
+    // b's rows begin `d` bytes behind a's, within a pitch: apart if they begin behind a's row and end before a's next one
+    const uintptr_t d = x <= y ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
+    return d < ra || d + rb > pitch;
+}
 inline int hapmi_apart(const char *name, std::initializer_list<HapmiSpan> written, std::initializer_list<HapmiSpan> read) {
-    auto meet = [](const HapmiSpan &a, const HapmiSpan &b) {
-        const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
-        return x && y && a.bytes > 0 && b.bytes > 0 && (x <= y ? y - x < (uintptr_t)a.bytes : x - y < (uintptr_t)b.bytes);
-    };
     for (auto w = written.begin(); w != written.end(); ++w) {
-        for (auto o = w + 1; o != written.end(); ++o) HAPMI_REQUIRE(!meet(*w, *o), HAPMI_EALIAS, "%s: an output shares memory with another operand", name);
-        for (auto &r : read) HAPMI_REQUIRE(!meet(*w, r), HAPMI_EALIAS, "%s: an output shares memory with another operand", name);
+        for (auto o = w + 1; o != written.end(); ++o) HAPMI_REQUIRE(!hapmi_meet(*w, *o), HAPMI_EALIAS, "%s: an output shares memory with another operand", name);
+        for (auto &r : read) HAPMI_REQUIRE(!hapmi_meet(*w, r), HAPMI_EALIAS, "%s: an output shares memory with another operand", name);
     }
     return HAPMI_OK;
 }

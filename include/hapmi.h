@@ -374,7 +374,8 @@ typedef struct {
  * Backward takes out and lse as forward left them, writes dqkv completely and dtable[n_buckets][ld_dtable]'s columns
  * 0 .. H - 1 (accumulate != 0: adds to them; b >= 1); delta_ws is float32 scratch of b*H*S elements, workspace float32 scratch
  * of the number of elements that hapmi_attention_relbias_workspace_elems reports.  No atomics between waves: the same call
- * gives the same bits.  Outputs and scratch share no memory with each other or with what is read (HAPMI_EALIAS). */
+ * gives the same bits.  Outputs and scratch share no memory with each other or with what is read (HAPMI_EALIAS); the
+ * columns beside a table's in the same buffer are apart from it, so table and gradient may be columns of one buffer. */
 int hapmi_attention_relbias_fwd(const void *qkv, const hapmi_relbias *bias_host, int causal, const int32_t *lengths, void *out,
                                 float *lse, int64_t b, int64_t S, int64_t H, float scale, const uint32_t *keep_rows,
                                 float p, hapmi_stream_t stream);

@@ -308,3 +308,18 @@ def test_table_gradient_where_every_block_meets_its_neighbours_words(cuda, b, S,
     res = run(cuda, qkv, table, dout, H, **kw)
     want = L.relbias_backward(qkv, table, res[0].cpu(), dout, res[1].cpu(), H, SCALE, 1000, not causal, causal)["dtable"]
     within(res[3], want[0], F * want[2], "dtable")
+
+
+def test_table_and_gradient_as_columns_of_one_buffer(cuda):
+    """Tables and gradients of two groups of heads side by side in one buffer share no memory: the calls are taken, give the bits
+    of buffers of their own and leave the other columns alone."""
+    qkv, table, dout = make(4, 2, 90, 3, 32)
+    want = run(cuda, qkv, table, dout, 3)
+    buf = torch.full((32, 12), 7.0, device=cuda)
+    buf[:, 2:5] = table.to(cuda)
+    buf[:, 5:8] = 0.0
+    res = run(cuda, qkv, buf[:, 2:5], dout, 3, dtable=buf[:, 5:8])
+    assert all(torch.equal(a, b) for a, b in zip(res, want))
+    assert (buf[:, :2] == 7).all() and (buf[:, 8:] == 7).all() and torch.equal(buf[:, 2:5], table.to(cuda))
+    with pytest.raises(ValueError):
+        run(cuda, qkv, buf[:, 2:5], dout, 3, dtable=buf[:, 4:7])

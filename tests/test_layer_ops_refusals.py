@@ -230,3 +230,16 @@ def test_balance_gradient_apart(other):
     at = {n: (i + 1) << 20 for i, n in enumerate(("probs", "index", "slot", "dgate", "counts", "lengths"))}
     rc = _load().hapmi_balance_loss_bwd(at["probs"], at["index"], at["slot"], at["dgate"], at["counts"], at["lengths"], at[other], 2, 64, 16, 0.01, 2, None)
     refused(rc, EALIAS, "shares memory")
+
+
+@pytest.mark.parametrize("off,ldd,ws", [(0, 8, None), (12, 8, None), (20, 8, None), (28, 8, None), (32, 8, None), (16, 12, None), (-92, 8, None), (16, 8, 20),
+                                        (16, 8, 36)])
+def test_table_gradients_among_the_tables_columns(off, ldd, ws):
+    """A table of 4 heads in rows of 8 floats leaves its columns 4 .. 7 to others: a gradient (or scratch) that begins or ends in the
+    table's own columns, or has rows of another length, is refused."""
+    table = 8 << 20
+    at = {n: (i + 1) << 20 for i, n in enumerate(("qkv", "out", "dout", "lse", "dqkv", "delta", "ws"))}
+    r = bias(table=table)
+    rc = _load().hapmi_attention_relbias_bwd(at["qkv"], ctypes.byref(r), 0, None, at["out"], at["dout"], at["lse"], at["dqkv"], table + off, ldd, 0,
+                                             at["delta"], table + ws if ws else at["ws"], 1 << 16, 2, 16, 4, 0.125, None, None, 0.0, None)
+    refused(rc, EALIAS, "shares memory")
