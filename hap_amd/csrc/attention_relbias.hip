@@ -1057,6 +1057,8 @@ int check_shape(const char *name, int64_t b, int64_t S, int64_t H, float scale, 
     HAPMI_REQUIRE(b >= 0 && S >= 1 && H >= 1, HAPMI_EINVAL, "%s: bad shape", name);
     HAPMI_REQUIRE(S < (1ll << 24) && H <= 4096 && b <= 65535 / H, HAPMI_ELIMIT, "%s: b * H above 65535, H above 4096 or S too long", name);
     HAPMI_REQUIRE(scale > 0.f && scale < INFINITY, HAPMI_EINVAL, "%s: scale = %g must be positive", name, (double)scale);
+    // the window holds bias / scale in float32: 1e8 / 1e-20 is far inside its range, and 1e20 loses no bias above 1e-17
+    HAPMI_REQUIRE(scale >= 1e-20f && scale <= 1e20f, HAPMI_ELIMIT, "%s: scale = %g must lie in [1e-20, 1e20]", name, (double)scale);
     HAPMI_REQUIRE(p >= 0.f && p < 1.f, HAPMI_EINVAL, "%s: p = %g must lie in [0, 1)", name, (double)p);
     return HAPMI_OK;
 }

@@ -1057,7 +1057,7 @@ def attention_relbias_fwd(qkv, table, out, lse, b, S, H, scale, max_distance=128
     others stay below 1e8 in size (scores are float32, and a weight made from a score of size x is good to x * 2^-22).  ``lengths`` (int32 [b]): the sequences of a padded
     batch; rows behind a sequence's end get zeros and lse = -inf, its keys there are not read (inside it, pairs that the causal
     mask or the bias hides are multiplied with weight zero: non-finite values there spread).  ``keep_rows`` / ``p``:
-    dropout of the probabilities, as in ``attention_fwd``."""
+    dropout of the probabilities, as in ``attention_fwd``.  ``scale`` lies in [1e-20, 1e20]."""
     what = "attention_relbias_fwd"
     n = b * S * H
     stream, (o_, l_, q_, n_, k_) = _operands(what, ("out", "lse", "qkv", "lengths", "keep_rows"), _RELBIAS_FWD_TYPES, (out, lse, qkv, lengths, keep_rows),

@@ -370,7 +370,7 @@ typedef struct {
  * zeros (out, dqkv) and -inf (lse).  A query that sees nothing gets the same.  A pair hidden by the causal mask or by its
  * bias has weight zero, but is multiplied: an infinity or NaN in a key or value inside a sequence's length may reach the
  * other queries of the sequence, as it does in a product with explicit zeros.  keep_rows / keep_cols / p: dropout of the
- * probabilities as in hapmi_attention_fwd_dropout (NULL = none).  scale > 0.
+ * probabilities as in hapmi_attention_fwd_dropout (NULL = none).  scale lies in [1e-20, 1e20] (the bias is kept divided by it).
  * Backward takes out and lse as forward left them, writes dqkv completely and dtable[n_buckets][ld_dtable]'s columns
  * 0 .. H - 1 (accumulate != 0: adds to them; b >= 1); delta_ws is float32 scratch of b*H*S elements, workspace float32 scratch
  * of the number of elements that hapmi_attention_relbias_workspace_elems reports.  No atomics between waves: the same call

@@ -323,3 +323,23 @@ def test_table_and_gradient_as_columns_of_one_buffer(cuda):
     assert (buf[:, :2] == 7).all() and (buf[:, 8:] == 7).all() and torch.equal(buf[:, 2:5], table.to(cuda))
     with pytest.raises(ValueError):
         run(cuda, qkv, buf[:, 2:5], dout, 3, dtable=buf[:, 4:7])
+
+
+@pytest.mark.parametrize("exponent", [-62, 66])
+def test_scales_near_the_ends_of_their_range(cuda, exponent):
+    """Queries and keys of size 2^(-exponent / 2) under a scale of 2^exponent / 8 give ordinary scores; so does the bias that the
+    window holds divided by it.  Powers of two leave every rounding where it is: the bits of the usual scale, but for dqkv's
+    queries and keys, which carry the power."""
+    qkv, table, dout = make(4, 1, 90, 2, 32)
+    want = run(cuda, qkv, table, dout, 2)
+    moved = qkv.view(1, 90, 3, 2, HD).clone()
+    half = 2.0 ** (-exponent // 2)
+    moved[:, :, :2] *= half
+    x, t, d = moved.view_as(qkv).to(cuda), table.to(cuda), dout.to(cuda)
+    out, lse, dx, dt = (torch.empty_like(w) for w in want)
+    scale = SCALE * 2.0 ** exponent
+    ops.attention_relbias_fwd(x, t, out, lse, 1, 90, 2, scale)
+    ops.attention_relbias_bwd(x, t, out, d, lse, dx, dt, torch.empty_like(lse), 1, 90, 2, scale)
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and torch.equal(dt, want[3])
+    dx, dw = dx.view(1, 90, 3, 2, HD), want[2].view(1, 90, 3, 2, HD)
+    assert torch.equal(dx[:, :, 2], dw[:, :, 2]) and torch.equal(dx[:, :, :2].float() * half, dw[:, :, :2].float())

@@ -243,3 +243,12 @@ def test_table_gradients_among_the_tables_columns(off, ldd, ws):
     rc = _load().hapmi_attention_relbias_bwd(at["qkv"], ctypes.byref(r), 0, None, at["out"], at["dout"], at["lse"], at["dqkv"], table + off, ldd, 0,
                                              at["delta"], table + ws if ws else at["ws"], 1 << 16, 2, 16, 4, 0.125, None, None, 0.0, None)
     refused(rc, EALIAS, "shares memory")
+
+
+@pytest.mark.parametrize("scale", [1e-38, 9e-21, 1.1e20, 3e38])
+def test_scales_that_the_bias_window_cannot_hold(scale):
+    """The bias is kept divided by the scale: a bias of 1e7 over 1e-38 is beyond float32, one of 1 over 3e38 below it."""
+    refused(rel_fwd(scale=scale), ELIMIT, "1e-20")
+    r = bias()
+    rc = _load().hapmi_attention_relbias_bwd(P, ctypes.byref(r), 0, None, P, P, P, P, P, 8, 0, P, P, 1 << 30, 2, 16, 4, scale, None, None, 0.0, None)
+    refused(rc, ELIMIT, "1e-20")
