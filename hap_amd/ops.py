@@ -882,7 +882,8 @@ def qk_norm_rotary_bwd(dout, qkv, dqkv, b, S, H, q_gain=None, k_gain=None, dq_ga
                        positions=None, interleaved=False, eps=1e-6, accumulate=False, workspace=None):
     """Backward of ``qk_norm_rotary_fwd``: ``dqkv`` from ``dout`` (``dqkv`` may be ``dout``: in place) and forward's input
     ``qkv``; ``dq_gain`` / ``dk_gain`` float32 [head_dim] (None: not wanted; ``accumulate``: added to).  A token whose position
-    lies outside the table is left out: zeros for its queries and keys, nothing in the gains' gradients."""
+    lies outside the table is left out: zeros for its queries and keys, nothing in the gains' gradients.  ``workspace``: float32
+    scratch of ``qk_norm_rotary_workspace_elems``, for the gains only (None: taken from torch's allocator)."""
     what = "qk_norm_rotary_bwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
     code, n, ws_elems = dtype_code(qkv), b * S * 3 * H * D, 0
@@ -1486,7 +1487,8 @@ _BALANCE_BWD_TYPES = (torch.float32, torch.float32, torch.int32, torch.int32, to
 
 
 @functools.lru_cache(maxsize=256)
-def _balance_workspace_elems(B, S, E):
+def balance_workspace_elems(B: int, S: int, E: int) -> int:
+    """Float32 elements of the scratch buffer that ``balance_loss_fwd`` needs (0: none)."""
     need = ctypes.c_int64()
     check(_lib._load().hapmi_balance_workspace_elems(B, S, E, ctypes.byref(need)))
     return need.value
@@ -1497,11 +1499,12 @@ def balance_loss_fwd(r, loss, counts, kept, prob_sum, choices=2, coef=0.01, leng
     made of: ``counts`` (int32 [B, E]: choices of every expert before capacity; ``choices`` = 1: first choices, 2: both),
     ``kept`` (int32 [B, E]: those that got a slot), ``prob_sum`` (float32 [B, E]).
     loss = coef * E * mean over the rows of sum_e counts / (choices * n) * prob_sum / n, n the row's tokens: all S, or
-    ``lengths`` (int32 [B]) of a padded batch (empty rows do not enter the mean).  Perfectly even routing gives coef."""
+    ``lengths`` (int32 [B]) of a padded batch (empty rows do not enter the mean).  Perfectly even routing gives coef.
+    ``workspace``: float32 scratch of ``balance_workspace_elems`` (None: taken from torch's allocator)."""
     what = "balance_loss_fwd"
     probs = r["probs"]
     B, S, E = probs.shape
-    need = _balance_workspace_elems(B, S, E)
+    need = balance_workspace_elems(B, S, E)
     workspace = _scratch(what, workspace, need, loss.device) if need else None
     n, m = B * E, B * S * 2
     stream, (l_, c_, k_, ps_, ws_, p_, i_, s_, n_) = _operands(

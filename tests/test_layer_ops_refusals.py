@@ -252,3 +252,16 @@ def test_scales_that_the_bias_window_cannot_hold(scale):
     r = bias()
     rc = _load().hapmi_attention_relbias_bwd(P, ctypes.byref(r), 0, None, P, P, P, P, P, 8, 0, P, P, 1 << 30, 2, 16, 4, scale, None, None, 0.0, None)
     refused(rc, ELIMIT, "1e-20")
+
+
+@pytest.mark.parametrize("B,S,E", [(4, 64, 16), (16, 512, 16), (64, 2048, 64), (1, 4097, 3), (600, 5, 8), (2, 1 << 20, 64)])
+def test_scratch_of_the_balance_loss_is_what_the_library_asks_for(B, S, E):
+    need = ops.balance_workspace_elems(B, S, E)
+
+    def fwd(ws, elems):
+        # an index that shares memory with the loss: what a call that passes the scratch check is refused for
+        return _load().hapmi_balance_loss_fwd(P, 1 << 40, 2 << 40, None, 1 << 40, 3 << 40, 4 << 40, 5 << 40, B, S, E, 0.01, 2, ws, elems, None)
+    if need:
+        refused(fwd(6 << 40, need - 1), ELIMIT, "workspace")
+        refused(fwd(None, need), ELIMIT, "workspace")
+    refused(fwd(6 << 40 if need else None, need), EALIAS, "shares memory")
