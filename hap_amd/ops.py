@@ -858,7 +858,8 @@ _QK_BWD_EXACT = ("dqkv", "dout", "q_gain", "k_gain", "dq_gain", "dk_gain", "posi
 def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None, positions=None, interleaved=False, eps=1e-6):
     """Queries and keys of the packed projection ``qkv`` [b, S, 3 * H * head_dim] normalised per head (root mean square,
     float32 gains [head_dim]) and rotated by position (``rotary`` from ``rotary_table``; its first 2 * shape[1] dimensions;
-    None: norm only), values copied; ``out`` may be ``qkv`` itself (in place).  ``positions``: int32 [b, S] (None: the index
+    None: norm only), values copied; ``out`` may be ``qkv`` itself (in place: backward, which needs
+    this input, then has to be given a copy).  ``positions``: int32 [b, S] (None: the index
     inside the sequence); one outside the table gives NaN in the token's queries and keys.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
     what = "qk_norm_rotary_fwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)

@@ -290,7 +290,8 @@ int hapmi_layernorm_bwd_dropout(const void *dy, const void *y, const float *rstd
  * D at most 256 and a multiple of 8 (bf16) / 4 (float32); rot a multiple of twice that (interleaved: of that).
  * Backward: dqkv (== dout: in place) from dout and forward's input; dq_gain / dk_gain float32[D] or NULL, overwritten or
  * (accumulate) added to; they need float32 workspace of hapmi_qk_norm_rotary_workspace_elems(D).  No atomics.
- * In place means the same pointer; any other overlap of an output is refused (HAPMI_EALIAS). */
+ * In place means the same pointer; any other overlap of an output is refused (HAPMI_EALIAS).  Forward in place overwrites the input
+ * that backward needs: it is for inference, or where the input is kept elsewhere. */
 int hapmi_qk_norm_rotary_fwd(const void *qkv, void *out, const float *q_gain, const float *k_gain, const float *angles, int64_t n_pos,
                              int64_t rot, int interleaved, const int32_t *positions, int64_t b, int64_t S, int64_t H, int64_t D,
                              float eps, int dtype, hapmi_stream_t stream);

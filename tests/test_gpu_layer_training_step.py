@@ -154,3 +154,38 @@ def test_the_step_as_a_recorded_launch_list(cuda):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(step.results(), want)), i
         del junk
+
+
+def test_the_documented_step_gives_the_gradients_of_its_own_forward(cuda):
+    """The code block of the integration guide, run as it stands: the norm's backward has to find forward's input."""
+    import os
+    import re
+    guide = open(os.path.join(os.path.dirname(__file__), "..", "INTEGRATION.md")).read()
+    block = [b for b in re.findall(r"```python\n(.*?)```", guide, re.S) if "qk_norm_rotary_fwd" in b]
+    assert len(block) == 1
+    b, S_, H_, n = 2, 40, 2, [40, 23]
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    qkv, dout, table, qg, kg = r(b, S_, 3 * H_ * 64).bfloat16(), r(b, S_, H_ * 64).bfloat16(), r(32, H_), 1 + 0.2 * r(64), 1 + 0.2 * r(64)
+    dout[1, 23:] = 0
+    records = ops.top2_gate(r(b, S_, 4).to(cuda), 20)
+    up = lambda t: t.to(cuda)  # noqa: E731
+    f32 = lambda *s: torch.full(s, float("nan"), device=cuda)  # noqa: E731
+    x = up(qkv)
+    names = dict(ops=ops, b=b, S=S_, H=H_, dev=cuda, qkv=x, rot=torch.empty_like(x), dqkv=torch.empty_like(x), q_gain=up(qg), k_gain=up(kg),
+                 table=up(table), out=torch.empty_like(up(dout)), dout=up(dout), lse=f32(b, H_, S_), delta=f32(b, H_, S_), dtable=f32(32, H_),
+                 dq_gain=f32(64), dk_gain=f32(64), lengths=torch.tensor(n, dtype=torch.int32, device=cuda), records=records, loss=f32(1),
+                 counts=torch.empty(b, 4, dtype=torch.int32, device=cuda), kept=torch.empty(b, 4, dtype=torch.int32, device=cuda),
+                 prob_sum=f32(b, 4), dlogits=f32(b, S_, 4), dgate=up(r(b, S_, 2)))
+    exec(block[0], names)
+    torch.cuda.synchronize()
+    p = {k: v.double().requires_grad_(True) for k, v in (("qkv", qkv), ("table", table), ("qg", qg), ("kg", kg))}
+    angles = ops.rotary_table(S_, 64)[None].expand(b, S_, -1, 2)
+    rot = L.qk_norm_forward(p["qkv"], H_, p["qg"], p["kg"], angles, False, 1e-6).reshape(b, S_, -1)
+    att = L.relbias_forward(rot, p["table"], H_, 0.125, 128, True, False, torch.tensor(n))[0].reshape(b, S_, -1)
+    (att * dout.double()).sum().backward()
+    rel = lambda a, w: ((a.double().cpu() - w).norm() / w.norm()).item()  # noqa: E731
+    for k, got in (("qkv", names["dqkv"]), ("table", names["dtable"]), ("qg", names["dq_gain"]), ("kg", names["dk_gain"])):
+        assert rel(got, p[k].grad) < 2e-2, (k, rel(got, p[k].grad))
+    _, counts, _, _, _ = L.balance(records["probs"].cpu(), records["index"].cpu(), records["slot"].cpu(), 2, 0.01)
+    assert torch.equal(names["counts"].cpu(), counts)
