@@ -176,3 +176,29 @@ def test_padding_may_hold_anything(cuda, B, S, E, lengths, filler):
         ops.balance_loss_bwd(dirty, counts, d, dgate=dirty_gate, lengths=ln)
         assert (d[pad] == 0).all()
         assert torch.equal(d[~pad], want[~pad])
+
+
+@pytest.mark.parametrize("B,S,E,choices,ragged", [(3000, 4, 8, 2, True), (1025, 40, 64, 2, True), (2049, 33, 33, 1, True), (1500, 3, 64, 1, False), (5000, 7, 2, 2, True)])
+def test_more_rows_than_the_joining_block_has_threads(cuda, B, S, E, choices, ragged):
+    """A row for every short sequence: the joining block walks the rows and their lengths in turns."""
+    r, _ = routing(cuda, B, B, S, E)
+    ln = torch.tensor([(i * 7) % (S + 2) - 1 for i in range(B)], dtype=torch.int32) if ragged else None
+    n = ln.clamp(0, S).double() if ragged else torch.full((B,), float(S), dtype=torch.float64)
+    loss, counts, kept, sums, d = outputs(cuda, B, S, E)
+    up = None if ln is None else ln.to(cuda)
+    ops.balance_loss_fwd(r, loss, counts, kept, sums, choices=choices, coef=0.02, lengths=up)
+    ops.balance_loss_bwd(r, counts, d, choices=choices, coef=0.02, lengths=up)
+    inside = torch.arange(S)[None] < n[:, None]
+    p, index, slot = r["probs"].double().cpu(), r["index"].cpu().long()[..., :choices], r["slot"].cpu()[..., :choices]
+    hit = torch.nn.functional.one_hot(index, E) * inside[:, :, None, None]
+    wc, wk = hit.sum((1, 2)), (hit * (slot > 0)[..., None]).sum((1, 2))
+    ws = (p * inside[..., None]).sum(1)
+    w = 0.02 * E * wc.double() / ((n > 0).sum() * choices * n.clamp(min=1)[:, None] ** 2)
+    want = (w * ws).sum().item()
+    assert torch.equal(counts.cpu().long(), wc) and torch.equal(kept.cpu().long(), wk)
+    assert ((sums.double().cpu() - ws).abs() <= S * E24 * ws).all()
+    # a thread adds B E / 1024 products one after the other, the block 16 + 6 more, each product has 8 roundings and S of its sum
+    assert abs(loss.item() - want) <= (S + 32 + B * E / 1024) * E24 * want
+    g = torch.where(inside[..., None], w[:, None], torch.zeros(1, 1, 1, dtype=torch.float64))
+    dot = (p * g).sum(-1, keepdim=True)
+    assert ((d.double().cpu() - p * (g - dot)).abs() <= 32 * E24 * p * (g + dot) + 1e-30).all()

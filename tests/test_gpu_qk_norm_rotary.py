@@ -234,3 +234,32 @@ def test_backward_leaves_out_tokens_without_a_position(cuda, dtype, inter, H, D,
     (want, wq, wk), (got, dq, dk) = res
     assert torch.equal(got, want) and torch.equal(dq, wq) and torch.equal(dk, wk)
     assert (got.cpu().view(b, S, 3, H * D)[:, :, :2][bad] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,b,S,H,D,rot,inter", [(torch.bfloat16, 2, 4501, 12, 64, 64, False), (torch.float32, 1, 12001, 5, 64, 32, True),
+                                                     (torch.bfloat16, 3, 9000, 5, 24, 16, True)])
+def test_backward_over_more_rows_than_resident_blocks_hold(cuda, dtype, b, S, H, D, rot, inter):
+    """768 blocks take all rows in turns: every lane adds the gain terms of two or more rows in its registers before the joining
+    launch.  A gain's sum runs over up to 3 rows a lane, 128 groups a block and 768 blocks in 32 runs of 24: below 200 roundings."""
+    lanes = 1
+    while lanes < (D // (8 if dtype == torch.bfloat16 else 4) + 1) // 2:
+        lanes *= 2
+    assert b * S * H > 768 * (256 // lanes)
+    qkv, dout, qg, kg, table, _ = make(11, b, S, H, D, dtype, rot, 0)
+    x, d, t, a, c = (v.to(cuda) for v in (qkv, dout, table, qg, kg))
+    dx, dq, dk = torch.full_like(x, float("nan")), torch.full_like(a, float("nan")), torch.full_like(c, float("nan"))
+    ops.qk_norm_rotary_bwd(d, x, dx, b, S, H, q_gain=a, k_gain=c, dq_gain=dq, dk_gain=dk, rotary=t, interleaved=inter, eps=1e-5)
+    wd, wq, wk, sq, sk = L.qk_norm_backward(dout, qkv, H, qg, kg, rows(table, None, b, S), inter, 1e-5)
+    big = lambda v: v.abs().amax(-1, keepdim=True)  # noqa: E731
+    xs = qkv.double().view(b, S, 3, H, D)
+    r = 1 / torch.sqrt((xs * xs).mean(-1, keepdim=True) + 1e-5)
+    size = r * big(dout.double().view(b, S, 3, H, D)) * 2 * max(qg.abs().max(), kg.abs().max()).item() * (1 + big(xs * r))
+    got = dx.view(b, S, 3, H, D)
+    within(got[:, :, :2], wd[:, :, :2], (U[dtype] * wd.abs() + F * size)[:, :, :2], "dqkv")
+    assert torch.equal(got[:, :, 2], d.view(b, S, 3, H, D)[:, :, 2])
+    # a term is off by 16 roundings of its own, the sum by 200 of the partial sums
+    within(dq, wq, 216 * 2.0 ** -24 * sq, "dq_gain")
+    within(dk, wk, 216 * 2.0 ** -24 * sk, "dk_gain")
+    again = torch.full_like(a, 1.5)
+    ops.qk_norm_rotary_bwd(d, x, dx, b, S, H, q_gain=a, k_gain=c, dq_gain=again, rotary=t, interleaved=inter, eps=1e-5, accumulate=True)
+    assert torch.equal(again, dq + 1.5)
