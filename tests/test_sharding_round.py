@@ -92,3 +92,25 @@ def test_overshoot_is_an_error():
         hap_amd.sharding_lengths(10, [0.8, 0.8])
     with pytest.raises(AssertionError):
         ref.sharding_round(10, [0.8, 0.8])
+
+
+def _in_float64(n, ratios):
+    """The rule in the arithmetic it is defined in: ratio - length / full_length as float64, the last largest one grows."""
+    out = [int(r * float(n)) for r in ratios]
+    while sum(out) < n:
+        keys = [r - float(l) / float(n) for r, l in zip(ratios, out)]
+        out[max(range(len(keys)), key=lambda i: (keys[i], i))] += 1
+    return out
+
+
+@pytest.mark.parametrize("weights,n", [([1, 1, 44, 4, 47, 47, 48, 64], 100000), ([32, 32, 32, 32, 32, 32, 32, 32], 12), ([60, 60, 60, 76], 99999)])
+@pytest.mark.parametrize("name,fn", IMPLS)
+def test_ties_are_those_of_float64(name, fn, weights, n):
+    """Dyadic ratios are exact in float64, quotients by a length that is no power of two are not: in the first case the deficits
+    44 / 256 - 17187 / 100000 and 4 / 256 - 1562 / 100000 are equal as fractions and 2^-54 apart in float64, so the unit goes to the
+    larger float64 one and not to the last of the two."""
+    ratios = [w / 256 for w in weights]
+    assert fn(n, ratios) == _in_float64(n, ratios)
+    if n == 100000:
+        assert Fraction(44, 256) - Fraction(17187, n) == Fraction(4, 256) - Fraction(1562, n)
+        assert 44 / 256 - 17187 / n > 4 / 256 - 1562 / n
