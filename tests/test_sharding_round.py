@@ -107,7 +107,7 @@ def _in_float64(n, ratios):
 @pytest.mark.parametrize("name,fn", IMPLS)
 def test_ties_are_those_of_float64(name, fn, weights, n):
     """Dyadic ratios are exact in float64, quotients by a length that is no power of two are not: in the first case the deficits
-    44 / 256 - 17187 / 100000 and 4 / 256 - 1562 / 100000 are equal as fractions and 2^-54 apart in float64, so the unit goes to the
+    44 / 256 - 17187 / 100000 and 4 / 256 - 1562 / 100000 are equal as fractions and 5.2e-18 apart in float64, so the unit goes to the
     larger float64 one and not to the last of the two."""
     ratios = [w / 256 for w in weights]
     assert fn(n, ratios) == _in_float64(n, ratios)
