@@ -423,7 +423,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // ---------------------------------------------------------------------------------------------
 // 13 matrix products and about 80 vector instructions a lane for a 32 x 32 block of scores, 64 more where it touches the bias
 // window (the diagonal sums).  Three waves a SIMD hide each other's latencies; where the launch does not fill the card, two
-// that also work on the next block's scores are faster (AHEAD; fits_two_a_cu has both sides).  [12, 512] x 16 heads: 38 us,
+// that also work on the next block's scores are faster (AHEAD; ahead_holds has both sides).  [12, 512] x 16 heads: 38 us,
 // matrix pipe 28 %, vector pipe 51 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one;
 // [2, 4096] x 16 heads, causal: 137 .. 142 us, matrix pipe 44 %, vector pipe 61 %.
 __host__ __device__ __forceinline__ int round4(int n) { return (n + 3) & ~3; }
@@ -1063,12 +1063,18 @@ int check_shape(const char *name, int64_t b, int64_t S, int64_t H, float scale, 
     return HAPMI_OK;
 }
 
-// Whether two blocks on each of the 256 CUs hold the whole launch.  Then a third wave a SIMD has nothing to work on, and the kernels that
-// keep two busy with the next block's scores are ahead (dQ, two a CU for three: [2, 2048] x 16 heads, 512 blocks, 69.9 us for 74.7;
-// [1, 4096] x 8 causal, 256 blocks, 80.6 for 90.9; [8, 512] x 16, 512 blocks, 29.0 for 29.7), beyond it they are behind ([12, 512] x 16
-// heads, 768 blocks: 46.0 for 41.8; [2, 4096] causal, 1024 blocks: 147 for 141).  Of a padded batch two thirds are taken to be there
-// ([6, 1001] x 12 heads of 334 .. 1001 tokens, 576 blocks: 48.6 for 50.6).
-bool fits_two_a_cu(int64_t blocks, bool padded) { return (padded ? blocks * 2 / 3 : blocks) <= 2 * 256; }
+// Whether the blocks that fit the 256 CUs at once hold the whole launch: two on each, or one where the bias window and the waves' sums
+// fill the LDS (R from 697 on).  Then a third wave a SIMD has nothing to work on, and the kernels that keep two busy with the next
+// block's scores are ahead (dQ, two a CU for three: [2, 2048] x 16 heads, 512 blocks, 69.9 us for 74.7; [1, 4096] x 8 causal, 256
+// blocks, 80.6 for 90.9; [8, 512] x 16, 512 blocks, 29.0 for 29.7), beyond it they are behind ([12, 512] x 16 heads, 768 blocks: 46.0
+// for 41.8; [2, 4096] causal, 1024 blocks: 147 for 141; with one a CU, R = 729, whole backward of 512 blocks [2, 2048] x 16: 179 for
+// 154, [1, 4096] x 16 causal: 192 for 190).  The plain kernels themselves drop from three blocks a CU to two above R = 424.
+// Of a padded batch two thirds of the blocks are taken to be there ([6, 1001] x 12 heads of 334 .. 1001 tokens, 576 blocks: 48.6 for
+// 50.6): the lengths are not known here, and a nearly full batch of 513 .. 768 blocks gets the form that is a tenth slower for it.
+bool ahead_holds(int64_t blocks, bool padded, int W) {
+    const int64_t lds = 3 * 2 * TILE_BYTES + 2 * REL_MAX_SIDE * 2 * 4 + (int64_t)dq_lds_words(W) * 4;      // of one block
+    return (padded ? blocks * 2 / 3 : blocks) <= (lds <= 160 * 1024 / 2 ? 2 : 1) * 256;
+}
 
 bool aligned(const void *p, uintptr_t n) { return (uintptr_t)p % n == 0; }
 
@@ -1183,7 +1189,7 @@ extern "C" int hapmi_attention_relbias_bwd(const void *qkv, const hapmi_relbias 
         return HAPMI_OK;
     };
     if (drop) rc = causal ? dq(relbias_bwd_dq_kernel<true, true, false>, 0) : dq(relbias_bwd_dq_kernel<false, true, false>, 1);
-    else if (fits_two_a_cu(row_blocks * b * H, lengths != nullptr)) rc = causal ? dq(relbias_bwd_dq_kernel<true, false, true>, 2) : dq(relbias_bwd_dq_kernel<false, false, true>, 3);
+    else if (ahead_holds(row_blocks * b * H, lengths != nullptr, W)) rc = causal ? dq(relbias_bwd_dq_kernel<true, false, true>, 2) : dq(relbias_bwd_dq_kernel<false, false, true>, 3);
     else rc = causal ? dq(relbias_bwd_dq_kernel<true, false, false>, 4) : dq(relbias_bwd_dq_kernel<false, false, false>, 5);
     if (rc) return rc;
     if (causal) return drop ? dkv(relbias_bwd_dkv_kernel<true, true>) : dkv(relbias_bwd_dkv_kernel<true, false>);

@@ -343,3 +343,17 @@ def test_scales_near_the_ends_of_their_range(cuda, exponent):
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and torch.equal(dt, want[3])
     dx, dw = dx.view(1, 90, 3, 2, HD), want[2].view(1, 90, 3, 2, HD)
     assert torch.equal(dx[:, :, 2], dw[:, :, 2]) and torch.equal(dx[:, :, :2].float() * half, dw[:, :, :2].float())
+
+
+@pytest.mark.parametrize("b,S,H,causal,lengths", [(6, 760, 8, False, None), (5, 900, 7, True, None), (7, 800, 8, False, [800, 1, 700, 333, 0, 799, 512]), (1, 1100, 3, False, None)])
+def test_windows_that_fill_the_lds(cuda, b, S, H, causal, lengths):
+    """Windows from 697 distances a side on leave room for one block of dQ's look-ahead form a compute unit: launches of more than 256
+    blocks (padded: 384) take the other form, smaller ones keep it."""
+    n, reach = (64, 950) if not causal else (32, 950)
+    assert ops.relative_bucket_starts(n, reach, not causal)[-1] > 697
+    qkv, table, dout = make(S, b, S, H, n)
+    for z, k in enumerate(lengths or []):
+        qkv[z, k:] = 0
+        dout[z, k:] = 0
+    res = run(cuda, qkv, table, dout, H, lengths=lengths, max_distance=reach, causal=causal)
+    compare(res, qkv, table, dout, H, reach, not causal, causal, lengths)
