@@ -21,6 +21,13 @@
 // each on this chip (the dQ kernel of [12, 512] x 16 heads took 274 us with them and 46 us without; 38 us by now).  The vector is
 // added to the wave's own window in LDS; the block adds its four windows and sums the buckets' ranges, the dK / dV kernel adds the blocks, all in a
 // fixed order: the same bits every time.
+//
+// Roundings.  Scores, statistics, sums and accumulators are float32.  Probabilities and score gradients are rounded to bf16 where they
+// become operands of a matrix instruction (P before PV and dV, dS before dQ and dK), as in the kernels without a bias: a float32 or split
+// operand would take three or more times the matrix work.  Each is off by 2^-8 of itself at most, independently of the
+// others, so a result carries its own rounding to bf16 once more (norm-wise 1.7e-3 from the operands next to 1.7e-3 of the result's own:
+// 2.2e-3 .. 2.4e-3 measured against float64).  The sum of weights adds the unrounded ones: rounded ones would shift lse, which backward takes for exact.  The table's
+// gradient adds unrounded dS.
 #include <atomic>
 
 #include "common.h"
@@ -258,10 +265,14 @@ __device__ __forceinline__ int row_length(const int32_t *lengths, int b, int S) 
 // ---------------------------------------------------------------------------------------------
 // One pass over the keys with a running maximum and sum; a wave holds 32 queries, a block of four waves 128, and the 64-key
 // tiles pass through three LDS stages, so that a transfer has two tiles' arithmetic to arrive in.  Three blocks a CU: all 768
-// of the encoder shape are resident at once.  Bound by vector instructions: a score costs a multiply-add, an exponential (at a
-// quarter of the rate), an addition, half a maximum and half a conversion, 28 cycles, against 16 of the matrix pipe.  [12, 512] x 16 heads: 24 us, 0.54 PFLOP/s, vector pipe 58 % and matrix pipe
-// 28 % of the cycles (8 us of it fixed: launch, prologue, results); [1, 8192] x 16 heads, causal: 164 .. 185 us as the power limit
-// lets it, 0.80 PFLOP/s of the visible half, vector pipe 70 %, matrix pipe 41 %, HBM 67 + 17 MB.
+// of the encoder shape are resident at once (two blocks where the bias window takes the room, which is given out in pieces of 1280 bytes:
+// R above 480, encoder shape 28 -> 30.4 us; with dropout above 96).
+// A score costs a multiply-add, an exponential (two multiply-adds' time, measured: 3.8 ns a wave instruction for 2.0 with four waves a
+// SIMD), an addition, half a maximum and half a conversion, 20 cycles of the vector pipe, against 16 of the matrix pipe; masks, window
+// reads, the running maximum and the operands' addresses come on top.
+// [12, 512] x 16 heads: 24 us, 0.54 PFLOP/s, vector pipe 58 % and matrix pipe 28 % of the cycles (8 us of it fixed: launch, prologue,
+// results), with dropout 30 us; [6, 1001] x 12 heads of 334 .. 1001 tokens: 28 us; [1, 8192] x 16 heads, causal: 164 .. 185 us as
+// the power limit lets it, 0.80 PFLOP/s of the visible half, vector pipe 70 %, matrix pipe 41 %, HBM 67 + 17 MB.
 // Without effect or worse: four parallel chains for the maximum, products pinned between the exponentials (184 for 177 us), no
 // maximum unless a sum of weights gets large (198 us: the test stands between the exponentials and the products), the next tile's
 // scores between this one's exponentials with two waves a SIMD (0 to 5 % slower even where the card is half empty).
@@ -426,6 +437,7 @@ __global__ __launch_bounds__(AT_THREADS, 3) void relbias_fwd_kernel(const RelArg
 // that also work on the next block's scores are faster (AHEAD; ahead_holds has both sides).  [12, 512] x 16 heads: 38 us,
 // matrix pipe 28 %, vector pipe 51 %, HBM 64 + 14 MB, a quarter of the time before the first tile and behind the last one;
 // [2, 4096] x 16 heads, causal: 137 .. 142 us, matrix pipe 44 %, vector pipe 61 %.
+// The plain form with the full mask needs one register more than the 168 of three waves a SIMD: 8 bytes a lane go to scratch.
 __host__ __device__ __forceinline__ int round4(int n) { return (n + 3) & ~3; }
 // a window, and the waves' sums, whose room their dO rows pass through first
 __host__ __device__ __forceinline__ int dq_lds_words(int W) { return round4(W) + (W > 1024 ? 4 * round4(W) : 4096); }
@@ -861,7 +873,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void relbias_bwd_dkv_kernel(const Re
         };
         if constexpr (DROP) {
             // The mask keeps delta out of the products and needs the keep words, and the look-ahead below then spills (backward of
-            // [12, 512] x 16 heads with dropout: 134 us with it, 102 us with these plain blocks).
+            // [12, 512] x 16 heads with dropout: 134 us with it, 102 us with these plain blocks when that was tried, 88 us by now).
             for (int q0 = q_begin; q0 < n; q0 += TILE) {
                 const char *Qs = Qs3[buf], *dOs = dOs3[buf];
 #pragma unroll 1
@@ -1068,7 +1080,8 @@ int check_shape(const char *name, int64_t b, int64_t S, int64_t H, float scale, 
 // block's scores are ahead (dQ, two a CU for three: [2, 2048] x 16 heads, 512 blocks, 69.9 us for 74.7; [1, 4096] x 8 causal, 256
 // blocks, 80.6 for 90.9; [8, 512] x 16, 512 blocks, 29.0 for 29.7), beyond it they are behind ([12, 512] x 16 heads, 768 blocks: 46.0
 // for 41.8; [2, 4096] causal, 1024 blocks: 147 for 141; with one a CU, R = 729, whole backward of 512 blocks [2, 2048] x 16: 179 for
-// 154, [1, 4096] x 16 causal: 192 for 190).  The plain kernels themselves drop from three blocks a CU to two above R = 424.
+// 154, [1, 4096] x 16 causal: 192 for 190).  The plain kernels themselves drop from three blocks a CU to two above R = 352
+// (encoder shape, whole backward: 78 -> 87 us).
 // Of a padded batch two thirds of the blocks are taken to be there ([6, 1001] x 12 heads of 334 .. 1001 tokens, 576 blocks: 48.6 for
 // 50.6): the lengths are not known here, and a nearly full batch of 513 .. 768 blocks gets the form that is a tenth slower for it.
 bool ahead_holds(int64_t blocks, bool padded, int W) {

@@ -10,7 +10,8 @@
 // holds one head of a token, every lane two 16-byte vectors chosen so that both halves of every rotated pair are its
 // own: the rotation needs no exchange, the mean one butterfly over the group.  The lane takes the query and the key of
 // its (token, head) together and reads the angles once for both.  bf16, 16 heads of 64: forward of [12, 512] 16.4 us, 75 MB at
-// 4.6 TB/s; backward of [4, 8192] with both gains 113 us, 547 MB at 4.8 TB/s (a large copy: 5.2 TB/s).
+// 4.6 TB/s; backward of [4, 8192] with both gains 113 us, 547 MB at 4.8 TB/s.  A copy of that size with one vector a thread and
+// non-temporal accesses reaches 6.6 TB/s (a library copy 5.2), which the looping grid and cached accesses here do not.
 #include "common.h"
 
 namespace {
