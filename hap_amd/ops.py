@@ -860,7 +860,7 @@ def qk_norm_rotary_fwd(qkv, out, b, S, H, q_gain=None, k_gain=None, rotary=None,
     float32 gains [head_dim]) and rotated by position (``rotary`` from ``rotary_table``; its first 2 * shape[1] dimensions;
     None: norm only), values copied; ``out`` may be ``qkv`` itself (in place: backward, which needs
     this input, then has to be given a copy).  ``positions``: int32 [b, S] (None: the index
-    inside the sequence); one outside the table gives NaN in the token's queries and keys.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
+    inside the sequence); one outside the table gives NaN in the token's queries and keys; without ``rotary`` they are not looked at.  ``interleaved``: pairs of neighbours instead of (i, i + rot / 2)."""
     what = "qk_norm_rotary_fwd"
     D, n_pos, rot = _head_dim(what, qkv, b, S, H, rotary)
     code, n = dtype_code(qkv), b * S * 3 * H * D

@@ -286,7 +286,8 @@ int hapmi_layernorm_bwd_dropout(const void *dy, const void *y, const float *rstd
  *   positions       int32[b * S] on the device, or NULL: the index inside the sequence.  A token whose position lies
  *                   outside [0, n_pos) gets NaN in its queries and keys in forward, and has no gradient: zeros for its
  *                   queries and keys in backward and nothing in the gains' gradients, whatever its rows hold (padding
- *                   marked with -1).  Every other token is expected to be finite: what is not reaches the gains' gradients
+ *                   marked with -1).  Every other token is expected to be finite: what is not reaches the gains' gradients.
+ *                   Without an angle table positions are not looked at
  * D at most 256 and a multiple of 8 (bf16) / 4 (float32); rot a multiple of twice that (interleaved: of that).
  * Backward: dqkv (== dout: in place) from dout and forward's input; dq_gain / dk_gain float32[D] or NULL, overwritten or
  * (accumulate) added to; they need float32 workspace of hapmi_qk_norm_rotary_workspace_elems(D).  No atomics.
